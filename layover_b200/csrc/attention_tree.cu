@@ -1,0 +1,662 @@
+// Attention for a tree of drafted tokens over the paged cache.
+//
+// A request holds `held` tokens and brings n drafts that form a tree: their keys and values lie behind the held ones,
+// draft j at place held + j. Row t of draft i (one row per draft and query head) attends to
+//
+//   every held key j < held          (with a window: positions[t] - j < window)
+//   the drafts j whose bit is set in tree[t]     (its ancestors and itself, as whoever drafted them says)
+//
+//   s_j = scale q.k_j,  or cap tanh(scale q.k_j / cap);   o = sum_j e^(s_j - m) v_j / (sum_j e^(s_j - m) + e^(sink - m))
+//
+// in one pass over the keys with a running maximum and sum in 32 bits. A row that sees no key is zero. The query heads of a
+// key/value head and the drafts are the rows of one tile (row = draft * group + head of the group), so every key and value is read
+// once for all of them. The reference has no drafts: it decodes one token a request and step (layover/engine.py:176-189).
+//
+// Blocks: (key/value head, sequence x row tile, chunk of the keys). Chunks have the same number of key tiles for every sequence, so
+// blocks take equally long whatever the lengths, and one that lies behind its sequence's end leaves at once. Where there is more
+// than one chunk each leaves its maxima, sums and unnormalised outputs in scratch memory of this call, and a second kernel joins them.
+//
+//   attention_tree_mma_kernel   bfloat16, mma.sync m16n8k16: RG groups of 16 rows, the four warps share a tile's 64 keys
+//   attention_tree_f32_kernel   float32, FFMA: 8 x 16 threads, RT / 8 rows and 4 keys (dim / 16 channels) each
+//
+// The values of a draft may be anything (a draft whose arithmetic overflowed): what a row does not see must not reach it, and
+// 0 x NaN is NaN. So in tiles that hold drafts, value rows that are not finite are taken out of the product and added one by
+// one to the rows that see them.
+#include <math.h>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int THREADS = 128;
+constexpr int KEYS = 64;        // keys per tile
+constexpr int PAD = 8;          // bf16 of padding per shared-memory row
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct TreeArgs {
+  const void *q, *k_pool, *v_pool;
+  void* out;
+  const int* block_table;
+  int table_width, n_pages;
+  const int *cu_q, *ctx_len, *positions, *tree;
+  int tree_words, tokens;
+  int q_heads, kv_heads, dim, page_tokens;
+  float scale_log2;             // scale * log2(e)
+  float cap_in, cap_out;        // 2 log2(e) scale / cap and cap / scale; 0: no cap
+  int window;
+  const float* sinks;
+  int row_tiles, chunk_tiles;   // row tiles of a sequence, key tiles of a block
+  float* partials;              // [unit][chunk][rows][dim] outputs, then [unit][chunk][rows][2] maxima and sums; null: one chunk
+  long partial_stats;           // where the second part begins, in floats
+};
+
+// What a block works on: its rows, and its share of the keys.
+struct Unit {
+  int seq, head, row0, rows;    // the sequence, the first row of its tile and how many of the tile's rows there are
+  int first, n, held, ctx;      // its first token, drafts, held tokens, keys
+  int key_lo;                   // no row sees a key below
+  int tile_begin, tile_end, chunks;
+  long index;                   // in the partial results
+};
+
+__device__ __forceinline__ Unit find_unit(const TreeArgs& a, int tile_rows, int seq, int row_tile, int head, int chunk, int n_chunks) {
+  Unit u;
+  u.seq = seq; u.head = head;
+  u.first = a.cu_q[seq];
+  u.n = min(a.cu_q[seq + 1], a.tokens) - u.first;
+  u.ctx = a.ctx_len[seq];
+  u.held = u.ctx - u.n;
+  const int group = a.q_heads / a.kv_heads;
+  u.row0 = row_tile * tile_rows;
+  u.rows = min(tile_rows, u.n * group - u.row0);
+  u.key_lo = a.window > 0 ? max(0, u.held - a.window + 1) : 0;      // the first draft's position is `held` at least
+  const int tile_lo = u.key_lo / KEYS, tiles = (u.ctx + KEYS - 1) / KEYS - tile_lo;
+  u.chunks = min(n_chunks, max(1, (tiles + a.chunk_tiles - 1) / a.chunk_tiles));
+  u.tile_begin = tile_lo + chunk * a.chunk_tiles;
+  u.tile_end = tile_lo + (chunk == n_chunks - 1 ? tiles : min(tiles, (chunk + 1) * a.chunk_tiles));
+  u.index = ((long)seq * a.kv_heads + head) * a.row_tiles + row_tile;
+  return u;
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Where key `key` of a sequence lies in its pool, in rows of one head's channels; -1 for a page that is not there.
+__device__ __forceinline__ long key_row(const TreeArgs& a, const int* table, int key, int head) {
+  const int index = key / a.page_tokens;
+  if (index >= a.table_width) return -1;
+  const int page = table[index];
+  if ((unsigned)page >= (unsigned)a.n_pages) return -1;
+  return ((long)page * a.kv_heads + head) * a.page_tokens + (key - index * a.page_tokens);
+}
+
+// Whether row `token` sees key `key`, `held` <= key < ctx or below: the tree decides among drafts, the window among held keys.
+__device__ __forceinline__ bool sees(const TreeArgs& a, const int* bits, int key, int held, int oldest) {
+  if (key < held) return key >= oldest;
+  const int j = key - held;
+  return (j >> 5) < a.tree_words && ((unsigned)bits[j >> 5] >> (j & 31)) & 1u;
+}
+
+// Keys [tile * 64, + 64) of one head into rows of `stride` elements of T; what lies outside [key_lo, ctx) becomes zeros.
+template <typename T>
+__device__ __forceinline__ void load_tile(T* to, const T* __restrict__ pool, const TreeArgs& a, const Unit& u, const int* table, int tile, int stride) {
+  constexpr int PER = 16 / (int)sizeof(T);
+  const int pieces = a.dim / PER;
+  for (int i = threadIdx.x; i < KEYS * pieces; i += THREADS) {
+    const int r = i / pieces, c = i - r * pieces, key = tile * KEYS + r;
+    const long row = key >= u.key_lo && key < u.ctx ? key_row(a, table, key, u.head) : -1;
+    cp_async16(to + r * stride + c * PER, pool + (row < 0 ? 0 : row * a.dim) + c * PER, row < 0 ? 0 : 16);
+  }
+}
+
+__device__ __forceinline__ bool not_finite(uint32_t two) {
+  return (two & 0x7F800000u) == 0x7F800000u || (two & 0x00007F80u) == 0x00007F80u;
+}
+
+// ------------------------------------------------------------------------------- bfloat16
+// A warp owns 16 rows and 64 / KG keys of every tile (KG = 4 / RG warps share a row group's keys and are joined at the end).
+template <int RG, int MAX_DIM>
+__global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tree_mma_kernel(const TreeArgs a) {
+  constexpr int KG = 4 / RG, NT = KEYS / KG / 8, KSTEPS = MAX_DIM / 16, NT_O = MAX_DIM / 8, STAGES = 2;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ unsigned bad_rows[4];                         // per 16 keys of a tile with drafts: value rows that are not finite
+  const int stride = a.dim + PAD, dk = a.dim >> 4;
+  bf16* q_s = reinterpret_cast<bf16*>(smem_raw);           // [16 RG][stride]
+  bf16* k_s = q_s + 16 * RG * stride;                      // [STAGES][KEYS][stride]
+  bf16* v_s = k_s + STAGES * KEYS * stride;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int seq = blockIdx.y / a.row_tiles;
+  const Unit u = find_unit(a, 16 * RG, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
+  if (u.rows <= 0 || (int)blockIdx.z >= u.chunks) return;
+  const int group = a.q_heads / a.kv_heads;
+  const int* table = a.block_table + (size_t)seq * a.table_width;
+  const bf16 *q = (const bf16*)a.q, *k_pool = (const bf16*)a.k_pool, *v_pool = (const bf16*)a.v_pool;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rg = warp % RG, kg = warp / RG;
+
+  {
+    const int pieces = a.dim >> 3;
+    for (int i = threadIdx.x; i < 16 * RG * pieces; i += THREADS) {
+      const int r = i / pieces, c = i - r * pieces, row = u.row0 + r;
+      const bool live = r < u.rows;
+      const long at = ((long)(u.first + (live ? row / group : 0)) * a.q_heads + u.head * group + (live ? row % group : 0)) * a.dim + c * 8;
+      cp_async16(q_s + r * stride + c * 8, q + at, live ? 16 : 0);
+    }
+  }
+  if (u.tile_begin < u.tile_end) {
+    load_tile(k_s, k_pool, a, u, table, u.tile_begin, stride);
+    load_tile(v_s, v_pool, a, u, table, u.tile_begin, stride);
+  }
+  cp_async_commit();
+
+  // the two rows of this lane: their masks, and the oldest held key they see
+  const int* bits[2];
+  int oldest[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = min(u.row0 + rg * 16 + g + 8 * r, u.n * group - 1), token = u.first + row / group;
+    bits[r] = a.tree + (size_t)token * a.tree_words;
+    oldest[r] = a.window > 0 ? max(a.positions[token], u.held) - a.window + 1 : 0;
+  }
+  uint32_t qf[KSTEPS][4];
+  float o[NT_O][4];
+#pragma unroll
+  for (int n = 0; n < NT_O; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  // ldmatrix lane addresses: K rows by key, V rows by key with the channel pieces swapped in
+  const int key_w = kg * NT * 8;                           // the warp's first key within a tile
+  const uint32_t k_lane = smem_u32(k_s) + (uint32_t)((key_w + (lane >> 4) * 8 + (lane & 7)) * stride + ((lane >> 3) & 1) * 8) * 2;
+  const uint32_t v_lane = smem_u32(v_s) + (uint32_t)((key_w + ((lane >> 3) & 1) * 8 + (lane & 7)) * stride + (lane >> 4) * 8) * 2;
+  const uint32_t buf_bytes = (uint32_t)KEYS * stride * 2;
+
+  for (int tile = u.tile_begin; tile < u.tile_end; ++tile) {
+    const int buf = (tile - u.tile_begin) & 1;
+    if (tile + 1 < u.tile_end) {
+      load_tile(k_s + (buf ^ 1) * KEYS * stride, k_pool, a, u, table, tile + 1, stride);
+      load_tile(v_s + (buf ^ 1) * KEYS * stride, v_pool, a, u, table, tile + 1, stride);
+      cp_async_commit();
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    if (tile == u.tile_begin) {
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k)
+        if (k < dk) ldmatrix_x4(qf[k], smem_u32(q_s + (rg * 16 + (lane & 15)) * stride + k * 16 + (lane >> 4) * 8));
+    }
+    const int key0 = tile * KEYS;
+    const bool drafts = key0 + KEYS > u.held;
+    if (drafts) {                                          // two threads look at a value row
+      bf16* row = v_s + buf * KEYS * stride + (threadIdx.x >> 1) * stride;
+      bool bad = false;
+      for (int c = (threadIdx.x & 1); c < a.dim >> 3; c += 2) {
+        const uint4 w = *reinterpret_cast<const uint4*>(row + c * 8);
+        bad |= not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w);
+      }
+      const unsigned both = __ballot_sync(0xffffffffu, bad && key0 + (int)(threadIdx.x >> 1) >= u.held);
+      unsigned rows = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) rows |= ((both >> (2 * i)) & 3u) ? 1u << i : 0u;
+      if (rows >> (lane >> 1) & 1u)
+        for (int c = (threadIdx.x & 1); c < a.dim >> 3; c += 2) *reinterpret_cast<uint4*>(row + c * 8) = make_uint4(0, 0, 0, 0);
+      if (lane == 0) bad_rows[warp] = rows;
+      __syncthreads();
+    }
+
+    // ---- scores
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KSTEPS; ++k) {
+      if (k >= dk) break;
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t b[4];
+        ldmatrix_x4(b, k_lane + buf * buf_bytes + (uint32_t)(n * 8 * stride + k * 16) * 2);
+        mma_bf16(s[n], qf[k], b[0], b[1]);
+        mma_bf16(s[n + 1], qf[k], b[2], b[3]);
+      }
+    }
+    if (a.cap_in != 0.f) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = a.cap_out - __fdividef(2.f * a.cap_out, 1.f + fast_exp2(s[n][e] * a.cap_in));
+    }
+    if (drafts || key0 < u.key_lo || a.window > 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + key_w + n * 8 + 2 * t + (e & 1);
+          if (key >= u.ctx || !sees(a, bits[e >> 1], key, u.held, oldest[e >> 1])) s[n][e] = -INFINITY;
+        }
+    }
+    // ---- weights
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) top = fmaxf(top, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = fmaxf(top, m_run[r]);
+      const float base = top == -INFINITY ? 0.f : top * a.scale_log2;
+      const float alpha = fast_exp2(m_run[r] * a.scale_log2 - base);       // 0 as long as nothing was seen
+      m_run[r] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float w = fast_exp2(fmaf(s[n][2 * r + e], a.scale_log2, -base));
+          s[n][2 * r + e] = w;
+          sum += w;
+        }
+      l_run[r] = l_run[r] * alpha + sum;
+#pragma unroll
+      for (int n = 0; n < NT_O; ++n) { o[n][2 * r] *= alpha; o[n][2 * r + 1] *= alpha; }
+    }
+    // ---- outputs
+#pragma unroll
+    for (int k = 0; k < NT / 2; ++k) {                     // 16 keys a step
+      const uint32_t p[4] = {pack_bf16(s[2 * k][0], s[2 * k][1]), pack_bf16(s[2 * k][2], s[2 * k][3]),
+                             pack_bf16(s[2 * k + 1][0], s[2 * k + 1][1]), pack_bf16(s[2 * k + 1][2], s[2 * k + 1][3])};
+#pragma unroll
+      for (int n = 0; n < NT_O; n += 2) {
+        if (n >= 2 * dk) break;
+        uint32_t b[4];
+        ldmatrix_x4_trans(b, v_lane + buf * buf_bytes + (uint32_t)(k * 16 * stride + n * 8) * 2);
+        mma_bf16(o[n], p, b[0], b[1]);
+        mma_bf16(o[n + 1], p, b[2], b[3]);
+      }
+    }
+    if (drafts && (bad_rows[0] | bad_rows[1] | bad_rows[2] | bad_rows[3])) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        for (int i = 0; i < 8; ++i) {
+          const int local = key_w + n * 8 + i;
+          if (!(bad_rows[local >> 4] >> (local & 15) & 1u)) continue;
+          const long from = key_row(a, table, key0 + local, u.head);       // a draft's row, which was read: it is there
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float w = __shfl_sync(0xffffffffu, i & 1 ? s[n][2 * r + 1] : s[n][2 * r], (lane & 28) | (i >> 1));
+            if (w == 0.f || from < 0) continue;
+#pragma unroll
+            for (int c = 0; c < NT_O; ++c)
+              if (c < 2 * dk) {
+                const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(v_pool + from * a.dim + c * 8 + 2 * t));
+                o[c][2 * r] += w * v.x;
+                o[c][2 * r + 1] += w * v.y;
+              }
+          }
+        }
+      }
+    }
+    __syncthreads();                                       // the buffer is loaded anew by the next step
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
+    l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
+  }
+
+  // ---- the warps that share a row group's keys are joined, in the order of their keys
+  if (KG > 1) {
+    float* parts = reinterpret_cast<float*>(k_s);          // [KG - 1][16 RG][dim + 2]: at most 48 rows in the room of 128 keys
+    const int width = a.dim + 2;
+    if (kg > 0) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float* to = parts + ((kg - 1) * 16 * RG + rg * 16 + g + 8 * r) * width;
+#pragma unroll
+        for (int n = 0; n < NT_O; ++n)
+          if (n < 2 * dk) { to[n * 8 + 2 * t] = o[n][2 * r]; to[n * 8 + 2 * t + 1] = o[n][2 * r + 1]; }
+        if (t == 0) { to[a.dim] = m_run[r]; to[a.dim + 1] = l_run[r]; }
+      }
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int p = 0; p < KG - 1; ++p) {
+        const float* from = parts + (p * 16 * RG + rg * 16 + g + 8 * r) * width;
+        const float m = from[a.dim], top = fmaxf(m_run[r], m), base = top == -INFINITY ? 0.f : top * a.scale_log2;
+        const float mine = fast_exp2(m_run[r] * a.scale_log2 - base), other = fast_exp2(m * a.scale_log2 - base);
+        m_run[r] = top;
+        l_run[r] = l_run[r] * mine + from[a.dim + 1] * other;
+#pragma unroll
+        for (int n = 0; n < NT_O; ++n)
+          if (n < 2 * dk) {
+            o[n][2 * r] = o[n][2 * r] * mine + from[n * 8 + 2 * t] * other;
+            o[n][2 * r + 1] = o[n][2 * r + 1] * mine + from[n * 8 + 2 * t + 1] * other;
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int local = rg * 16 + g + 8 * r, row = u.row0 + local;
+    if (local >= u.rows) continue;
+    if (u.chunks > 1) {
+      const long at = (u.index * gridDim.z + blockIdx.z) * (16 * RG) + local;
+      float* to = a.partials + at * a.dim;
+#pragma unroll
+      for (int n = 0; n < NT_O; ++n)
+        if (n < 2 * dk) *reinterpret_cast<float2*>(to + n * 8 + 2 * t) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+      if (t == 0) *reinterpret_cast<float2*>(a.partials + a.partial_stats + at * 2) = make_float2(m_run[r] * a.scale_log2, l_run[r]);
+    } else {
+      const int head = u.head * group + row % group;
+      float total = l_run[r];
+      float factor = 1.f;
+      if (a.sinks) {                                       // the sink may be the largest of all
+        const float sink = a.sinks[head] * LOG2E, m = m_run[r] * a.scale_log2, top = fmaxf(m, sink);
+        factor = fast_exp2(m - top);
+        total = total * factor + fast_exp2(sink - top);
+      }
+      const float inv = total == 0.f ? 0.f : factor / total;
+      bf16* to = (bf16*)a.out + ((size_t)(u.first + row / group) * a.q_heads + head) * a.dim;
+#pragma unroll
+      for (int n = 0; n < NT_O; ++n)
+        if (n < 2 * dk) *reinterpret_cast<uint32_t*>(to + n * 8 + 2 * t) = pack_bf16(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- float32
+template <int RT>
+__global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeArgs a) {
+  constexpr int RPT = RT / 8;                              // rows of a thread
+  constexpr int MAX_C = 4;                                 // blocks of 64 channels: head sizes up to 256
+  extern __shared__ __align__(16) float smem_f[];
+  __shared__ unsigned bad_rows[4];
+  const int stride = a.dim + 4;                            // rows 16 bytes apart modulo 128: eight rows' pieces lie in different banks
+  float* q_s = smem_f;                                     // [RT][stride]
+  float* k_s = q_s + RT * stride;                          // [KEYS][stride]
+  float* v_s = k_s + KEYS * stride;                        // [KEYS][stride]
+  float* p_s = v_s + KEYS * stride;                        // [RT][KEYS + 4]
+  constexpr int P_STRIDE = KEYS + 4;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int seq = blockIdx.y / a.row_tiles;
+  const Unit u = find_unit(a, RT, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
+  if (u.rows <= 0 || (int)blockIdx.z >= u.chunks) return;
+  const int group = a.q_heads / a.kv_heads;
+  const int* table = a.block_table + (size_t)seq * a.table_width;
+  const float *q = (const float*)a.q, *k_pool = (const float*)a.k_pool, *v_pool = (const float*)a.v_pool;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;  // rows ty + 8 i, keys tx + 16 j, channels 64 c + 4 tx ..
+  {
+    const int pieces = a.dim >> 2;
+    for (int i = threadIdx.x; i < RT * pieces; i += THREADS) {
+      const int r = i / pieces, c = i - r * pieces, row = u.row0 + r;
+      const bool live = r < u.rows;
+      const long at = ((long)(u.first + (live ? row / group : 0)) * a.q_heads + u.head * group + (live ? row % group : 0)) * a.dim + c * 4;
+      cp_async16(q_s + r * stride + c * 4, q + at, live ? 16 : 0);
+    }
+  }
+  if (u.tile_begin < u.tile_end) load_tile(k_s, k_pool, a, u, table, u.tile_begin, stride);
+  cp_async_commit();
+
+  const int* bits[RPT];
+  int oldest[RPT];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int row = min(u.row0 + ty + 8 * i, u.n * group - 1), token = u.first + row / group;
+    bits[i] = a.tree + (size_t)token * a.tree_words;
+    oldest[i] = a.window > 0 ? max(a.positions[token], u.held) - a.window + 1 : 0;
+  }
+  float o[RPT][MAX_C][4];
+  float m_run[RPT], l_run[RPT];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    m_run[i] = -INFINITY; l_run[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < MAX_C; ++c) o[i][c][0] = o[i][c][1] = o[i][c][2] = o[i][c][3] = 0.f;
+  }
+  for (int tile = u.tile_begin; tile < u.tile_end; ++tile) {
+    load_tile(v_s, v_pool, a, u, table, tile, stride);
+    cp_async_commit();
+    cp_async_wait<1>();                                    // the keys; the values come under the first product
+    __syncthreads();
+    const int key0 = tile * KEYS;
+    const bool drafts = key0 + KEYS > u.held;
+    float s[RPT][4];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int d = 0; d < a.dim; d += 4) {
+      float4 kv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * stride + d);
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const float4 qv = *reinterpret_cast<const float4*>(q_s + (ty + 8 * i) * stride + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j] = fmaf(qv.x, kv[j].x, s[i][j]); s[i][j] = fmaf(qv.y, kv[j].y, s[i][j]);
+          s[i][j] = fmaf(qv.z, kv[j].z, s[i][j]); s[i][j] = fmaf(qv.w, kv[j].w, s[i][j]);
+        }
+      }
+    }
+    const bool masked = drafts || key0 < u.key_lo || a.window > 0;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = key0 + tx + 16 * j;
+        if (a.cap_in != 0.f) s[i][j] = a.cap_out * tanhf(s[i][j] / a.cap_out);
+        if (masked && (key >= u.ctx || !sees(a, bits[i], key, u.held, oldest[i]))) s[i][j] = -INFINITY;
+        top = fmaxf(top, s[i][j]);
+      }
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      top = fmaxf(top, m_run[i]);
+      const float shift = top == -INFINITY ? 0.f : top;
+      const float alpha = exp2f((m_run[i] - shift) * a.scale_log2);
+      m_run[i] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w = exp2f((s[i][j] - shift) * a.scale_log2);      // the difference first: a product of the maximum would round with its size
+        p_s[(ty + 8 * i) * P_STRIDE + tx + 16 * j] = w;
+        sum += w;
+      }
+      l_run[i] = l_run[i] * alpha + sum;
+#pragma unroll
+      for (int c = 0; c < MAX_C; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][c][e] *= alpha;
+    }
+    cp_async_wait<0>();
+    __syncthreads();                                       // values and weights are there, the keys are done with
+    if (tile + 1 < u.tile_end) load_tile(k_s, k_pool, a, u, table, tile + 1, stride);
+    cp_async_commit();
+    if (drafts) {
+      const float* row = v_s + (threadIdx.x >> 1) * stride;
+      bool bad = false;
+      for (int c = threadIdx.x & 1; c < a.dim >> 2; c += 2) {
+        const float4 w = *reinterpret_cast<const float4*>(row + c * 4);
+        bad |= !isfinite(w.x) || !isfinite(w.y) || !isfinite(w.z) || !isfinite(w.w);
+      }
+      const unsigned both = __ballot_sync(0xffffffffu, bad);
+      if ((threadIdx.x & 31) == 0) bad_rows[threadIdx.x >> 5] = both;
+      __syncthreads();
+    }
+    const bool any_bad = drafts && (bad_rows[0] | bad_rows[1] | bad_rows[2] | bad_rows[3]);
+    for (int key = 0; key < KEYS; key += 4) {
+      float4 w[RPT];
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) w[i] = *reinterpret_cast<const float4*>(p_s + (ty + 8 * i) * P_STRIDE + key);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool bad = any_bad && (bad_rows[(key + e) >> 4] >> (2 * ((key + e) & 15)) & 3u);
+#pragma unroll
+        for (int c = 0; c < MAX_C; ++c) {
+          if (64 * c + 4 * tx >= a.dim) break;
+          const float4 v = *reinterpret_cast<const float4*>(v_s + (key + e) * stride + 64 * c + 4 * tx);
+#pragma unroll
+          for (int i = 0; i < RPT; ++i) {
+            const float p = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+            if (bad && p == 0.f) continue;                 // what a row does not see does not reach it
+            o[i][c][0] = fmaf(p, v.x, o[i][c][0]); o[i][c][1] = fmaf(p, v.y, o[i][c][1]);
+            o[i][c][2] = fmaf(p, v.z, o[i][c][2]); o[i][c][3] = fmaf(p, v.w, o[i][c][3]);
+          }
+        }
+      }
+    }
+    __syncthreads();                                       // values and weights are done with
+  }
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], x);
+    const int local = ty + 8 * i, row = u.row0 + local;
+    if (local >= u.rows) continue;
+    if (u.chunks > 1) {
+      const long at = (u.index * gridDim.z + blockIdx.z) * RT + local;
+#pragma unroll
+      for (int c = 0; c < MAX_C; ++c)
+        if (64 * c + 4 * tx < a.dim)
+          *reinterpret_cast<float4*>(a.partials + at * a.dim + 64 * c + 4 * tx) = make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
+      if (tx == 0) *reinterpret_cast<float2*>(a.partials + a.partial_stats + at * 2) = make_float2(m_run[i] * a.scale_log2, l_run[i]);
+    } else {
+      const int head = u.head * group + row % group;
+      float total = l_run[i], factor = 1.f;
+      if (a.sinks) {
+        const float sink = a.sinks[head] * LOG2E, m = m_run[i] * a.scale_log2, top = fmaxf(m, sink);
+        factor = exp2f(m - top);
+        total = total * factor + exp2f(sink - top);
+      }
+      const float inv = total == 0.f ? 0.f : factor / total;
+      float* to = (float*)a.out + ((size_t)(u.first + row / group) * a.q_heads + head) * a.dim;
+#pragma unroll
+      for (int c = 0; c < MAX_C; ++c)
+        if (64 * c + 4 * tx < a.dim)
+          *reinterpret_cast<float4*>(to + 64 * c + 4 * tx) = make_float4(o[i][c][0] * inv, o[i][c][1] * inv, o[i][c][2] * inv, o[i][c][3] * inv);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- the chunks' results
+// One warp per row: the chunks in order, relative to the largest of their maxima (kept in log2 units) and the sink.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) attention_tree_join_kernel(const TreeArgs a, int tile_rows, int n_chunks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int seq = blockIdx.y / a.row_tiles, row_tile = blockIdx.y - seq * a.row_tiles;
+  const Unit u = find_unit(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks);
+  const int local = blockIdx.z * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (local >= u.rows || u.chunks <= 1) return;
+  const int group = a.q_heads / a.kv_heads, row = u.row0 + local, head = u.head * group + row % group;
+  const long at = u.index * n_chunks * tile_rows + local;
+  const float2* stats = reinterpret_cast<const float2*>(a.partials + a.partial_stats);
+  float top = a.sinks ? a.sinks[head] * LOG2E : -INFINITY;
+  const float sink = top;
+  for (int c = lane; c < u.chunks; c += 32) top = fmaxf(top, stats[at + (long)c * tile_rows].x);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = a.sinks ? exp2f(sink - base) : 0.f;
+  constexpr int MAX_C = 2;                                 // 128 channels a step: head sizes up to 256
+  float4 sum[MAX_C] = {};
+  for (int c = 0; c < u.chunks; ++c) {
+    const float2 ml = stats[at + (long)c * tile_rows];
+    const float w = exp2f(ml.x - base);
+    total += w * ml.y;
+#pragma unroll
+    for (int i = 0; i < MAX_C; ++i) {
+      const int d = 128 * i + 4 * lane;
+      if (d < a.dim) {
+        const float4 v = *reinterpret_cast<const float4*>(a.partials + (at + (long)c * tile_rows) * a.dim + d);
+        if (w != 0.f) { sum[i].x += w * v.x; sum[i].y += w * v.y; sum[i].z += w * v.z; sum[i].w += w * v.w; }
+      }
+    }
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  T* to = (T*)a.out + ((size_t)(u.first + row / group) * a.q_heads + head) * a.dim;
+#pragma unroll
+  for (int i = 0; i < MAX_C; ++i) {
+    const int d = 128 * i + 4 * lane;
+    if (d >= a.dim) break;
+    Elem<T>::store(to + d, sum[i].x * inv); Elem<T>::store(to + d + 1, sum[i].y * inv);
+    Elem<T>::store(to + d + 2, sum[i].z * inv); Elem<T>::store(to + d + 3, sum[i].w * inv);
+  }
+}
+
+template <int RG, int MAX_DIM>
+int launch_mma(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
+  const size_t smem = (size_t)(16 * RG + 4 * KEYS) * (a.dim + PAD) * sizeof(bf16);
+  static LbPerDeviceOnce once;
+  if (!once.run(LB_ALLOW_SMEM((attention_tree_mma_kernel<RG, MAX_DIM>), (16 * RG + 4 * KEYS) * (MAX_DIM + PAD) * sizeof(bf16)))) return lb_last_error();
+  return lb_launch(attention_tree_mma_kernel<RG, MAX_DIM>, grid, THREADS, smem, stream, a);
+}
+template <int RT>
+int launch_f32(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
+  const size_t smem = ((size_t)(RT + 2 * KEYS) * (a.dim + 4) + RT * (KEYS + 4)) * sizeof(float);
+  static LbPerDeviceOnce once;
+  if (!once.run(LB_ALLOW_SMEM(attention_tree_f32_kernel<RT>, ((RT + 2 * KEYS) * (256 + 4) + RT * (KEYS + 4)) * sizeof(float)))) return lb_last_error();
+  return lb_launch(attention_tree_f32_kernel<RT>, grid, THREADS, smem, stream, a);
+}
+}  // namespace
+
+// `tile_rows`: rows of a block (16, 32 or 64). `chunks` blocks of `chunk_tiles` tiles of 64 keys share a row tile's keys (the
+// last takes what is left); with more than one, `partials` holds n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) floats.
+LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
+                                int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words, int tokens,
+                                int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, float scale, int window, const float* sinks,
+                                float softcap, int tile_rows, int row_tiles, int chunks, int chunk_tiles, float* partials, long partial_floats,
+                                cudaStream_t stream) {
+  if (tokens <= 0 || n_seqs <= 0) return 0;
+  if (dtype != LB_F32 && dtype != LB_BF16) return LB_ERR_DTYPE;
+  if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || dim <= 0 || dim > 256 || dim % (dtype == LB_BF16 ? 16 : 4) || page_tokens <= 0 ||
+      table_width <= 0 || n_pages <= 0 || tree_words <= 0 || window < 0 || softcap < 0.f || (window > 0 && !positions) || row_tiles <= 0 ||
+      chunks <= 0 || chunks > 65535 || chunk_tiles <= 0 || (long)n_seqs * row_tiles > 65535 || (tile_rows != 16 && tile_rows != 32 && tile_rows != 64))
+    return LB_ERR_SIZE;
+  const long partial_rows = (long)n_seqs * kv_heads * row_tiles * chunks * tile_rows;
+  if (chunks > 1 && (!partials || partial_floats < partial_rows * (dim + 2))) return LB_ERR_SIZE;
+  if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)partials) & 15) return LB_ERR_ALIGN;
+  TreeArgs a{q, k_pool, v_pool, out, block_table, table_width, n_pages, cu_q, ctx_len, positions, tree, tree_words, tokens, q_heads, kv_heads, dim,
+             page_tokens, scale * LOG2E, 0.f, 0.f, window, sinks, row_tiles, chunk_tiles, chunks > 1 ? partials : nullptr, partial_rows * dim};
+  if (softcap > 0.f) { a.cap_in = 2.f * LOG2E * scale / softcap; a.cap_out = softcap / scale; }
+  const dim3 grid(kv_heads, n_seqs * row_tiles, chunks);
+  int code;
+  if (dtype == LB_F32) {
+    code = tile_rows == 16 ? launch_f32<16>(a, grid, stream) : tile_rows == 32 ? launch_f32<32>(a, grid, stream) : launch_f32<64>(a, grid, stream);
+  } else if (dim <= 128) {
+    code = tile_rows == 16 ? launch_mma<1, 128>(a, grid, stream) : tile_rows == 32 ? launch_mma<2, 128>(a, grid, stream) : launch_mma<4, 128>(a, grid, stream);
+  } else {
+    code = tile_rows == 16 ? launch_mma<1, 256>(a, grid, stream) : tile_rows == 32 ? launch_mma<2, 256>(a, grid, stream) : launch_mma<4, 256>(a, grid, stream);
+  }
+  if (code || chunks == 1) return code ? code : lb_last_error();
+  const dim3 joined(kv_heads, n_seqs * row_tiles, tile_rows / (THREADS / 32));
+  code = dtype == LB_F32 ? lb_launch(attention_tree_join_kernel<float>, joined, THREADS, 0, stream, a, tile_rows, chunks)
+                         : lb_launch(attention_tree_join_kernel<bf16>, joined, THREADS, 0, stream, a, tile_rows, chunks);
+  return code ? code : lb_last_error();
+}

@@ -44,6 +44,9 @@ SOURCES: dict[str, tuple[str, tuple[str, ...]]] = {
     "gemm_tcgen05": ("gemm_tcgen05.cu", ()),
     "attention_mma": ("attention_mma.cu", ()),
     "attention_tcgen05": ("attention_tcgen05.cu", ()),
+    "attention_tree": ("attention_tree.cu", ()),
+    "cache_moves": ("cache_moves.cu", ()),
+    "beam": ("beam.cu", ()),
     "decode_attention_static": ("decode_attention_static.cu", ()),
 }
 

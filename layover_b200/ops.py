@@ -54,6 +54,15 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+def _here(what: str, *tensors: torch.Tensor | None) -> None:
+    """Every tensor is on the current CUDA device, on whose current stream the kernels are launched."""
+    for t in tensors:
+        if t is not None:
+            _ptr(t)
+            if t.get_device() != torch._C._cuda_getDevice():
+                raise ValueError(f"{what}: the tensors must be on the current CUDA device")
+
+
 def _stream() -> int:
     """The handle of the current device's current stream (without the Stream object around it)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
@@ -1270,6 +1279,179 @@ def attention_f32(q, cache, out, block_table, batch, q_heads, kv_heads, dim, pag
     attention_simt(q, cache.k_pool, cache.v_pool, out, block_table, batch.cu_q, batch.ctx_len, tiles.tile_seq, tiles.tile_q0,
                    tiles.count, q_heads, kv_heads, dim, page_tokens, scale, window, vdim, sinks, gates, chunk, keep_first,
                    softcap, out_scale, batch.max_q_len, max(batch.max_ctx, batch.plan_max_ctx))
+
+
+# ------------------------------------------------------------------ several hypotheses of a request: drafts and beams
+_TREE_KEYS = 64                          # keys of a tile (csrc/attention_tree.cu)
+_TREE_SCRATCH_FLOATS = 64 << 20          # the most that the chunks' results may take (256 MiB)
+
+
+@functools.lru_cache(maxsize=1024)      # of the sizes alone, asked for by every layer of a step
+def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, dim: int, sms: int) -> tuple[int, int, int, int]:
+    """(rows of a block, row tiles of a sequence, chunks, key tiles of a chunk) for `attention_tree`: row tiles no larger than the
+    rows ask for, and as many chunks of the keys as give every SM about four blocks."""
+    rows = max_nodes * (q_heads // kv_heads)
+    tile_rows = 16 if rows <= 16 else 32 if rows <= 32 else 64
+    row_tiles = -(-rows // tile_rows)
+    keys = min(max_ctx, max_nodes + window) if window else max_ctx
+    tiles = -(-keys // _TREE_KEYS) + (1 if window else 0)
+    units = n_seqs * kv_heads * row_tiles
+    most = max(1, _TREE_SCRATCH_FLOATS // (units * tile_rows * (dim + 2)))
+    chunks = max(1, min(-(-4 * sms // units), tiles // 2, most, 65535))
+    chunk_tiles = -(-tiles // chunks)
+    return tile_rows, row_tiles, -(-tiles // chunk_tiles), chunk_tiles
+
+
+def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
+                   cu_q: torch.Tensor, ctx_len: torch.Tensor, positions: torch.Tensor | None, tree: torch.Tensor, n_seqs: int, q_heads: int,
+                   kv_heads: int, dim: int, page_tokens: int, scale: float, max_nodes: int, max_ctx: int, window: int = 0,
+                   sinks: torch.Tensor | None = None, softcap: float = 0.0) -> torch.Tensor:
+    """Paged attention for drafted tokens that form a tree, float32 or bfloat16.
+
+    Sequence s brings the drafts (rows) cu_q[s] .. cu_q[s + 1], whose keys and values are in its pages behind the ones it
+    holds: ctx_len[s] counts both. A draft sees every held key and, of the sequence's drafts, those whose bit is set in its row of
+    `tree` (int32 [T, words]: bit j % 32 of word j // 32 stands for draft j of the same sequence); it sees itself only if its own bit is
+    set. A row that sees nothing is zero. q, out [T, q_heads * dim]; pools [pages, kv_heads, page_tokens, dim]; block_table
+    int32 [>= n_seqs, W]; cu_q int32 [n_seqs + 1]; ctx_len int32 [n_seqs].
+    `window` > 0: held key j is seen from position p (int32 `positions` [T], at least the number of held tokens) only where
+    p - j < window; among drafts `tree` alone decides. `sinks` float32 [q_heads] join the softmax's denominator only; `softcap` > 0: a
+    scaled score s becomes softcap * tanh(s / softcap). No sequence has more than `max_nodes` drafts or more than `max_ctx` keys
+    (what is above is not computed: rows, or not planned for: keys). Rows behind cu_q[n_seqs] stay as they are. Head sizes: multiples of
+    16 (float32: of 4) up to 256. What is in a draft's keys and values reaches only the rows that see it, infinities and NaN too."""
+    _need(q, None, "q"); _need(out, q.dtype, "out"); _need(k_pool, q.dtype, "k_pool"); _need(v_pool, q.dtype, "v_pool")
+    for name, t, dims in (("block_table", block_table, 2), ("cu_q", cu_q, 1), ("ctx_len", ctx_len, 1), ("tree", tree, 2)):
+        _need(t, torch.int32, name)
+        if t.dim() != dims:
+            raise ValueError(f"attention_tree: {name} must have {dims} dimension(s)")
+    if q_heads < 1 or kv_heads < 1 or q_heads % kv_heads:
+        raise ValueError(f"attention_tree: q_heads ({q_heads}) must be a multiple of kv_heads ({kv_heads})")
+    tokens = q.shape[0]
+    if tuple(q.shape) != (tokens, q_heads * dim) or out.shape != q.shape or k_pool.shape != v_pool.shape \
+            or tuple(k_pool.shape[1:]) != (kv_heads, page_tokens, dim):
+        raise ValueError("attention_tree: q, out or the pools do not match the heads")
+    if tree.shape[0] != tokens or block_table.shape[0] < n_seqs or cu_q.numel() < n_seqs + 1 or ctx_len.numel() < n_seqs:
+        raise ValueError("attention_tree: a row of tree per draft, a table row, an end and a length per sequence")
+    if max_nodes < 1 or max_ctx < 1 or window < 0 or softcap < 0:
+        raise ValueError("attention_tree: max_nodes and max_ctx are at least 1, window and softcap not negative")
+    if max_nodes > 32 * tree.shape[1]:
+        raise ValueError(f"attention_tree: {max_nodes} drafts need {-(-max_nodes // 32)} words a row of tree, got {tree.shape[1]}")
+    if window:
+        if positions is None:
+            raise ValueError("attention_tree: a window needs positions")
+        _need(positions, torch.int32, "positions")
+        if positions.numel() < tokens:
+            raise ValueError("attention_tree: a position per draft")
+    if sinks is not None:
+        _need(sinks, torch.float32, "sinks")
+        if sinks.numel() != q_heads:
+            raise ValueError("attention_tree: one sink per query head")
+    if q.dtype not in _DTYPE_CODE or dim % (16 if q.dtype == torch.bfloat16 else 4) or not 0 < dim <= 256:
+        raise ValueError(f"attention_tree: heads of {dim} channels in {q.dtype} are not supported")
+    _here("attention_tree", q, k_pool, v_pool, out, block_table, cu_q, ctx_len, positions if window else None, tree, sinks)
+    if tokens == 0 or n_seqs == 0:
+        return out
+    tile_rows, row_tiles, chunks, chunk_tiles = tree_plan(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, dim, sm_count(q.device))
+    partials = None
+    if chunks > 1:          # of this call alone, on its own stream
+        partials = torch.empty(n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2), dtype=torch.float32, device=q.device)
+    fn = _FUNCTIONS.get("lb_attention_tree") or _fn("attention_tree", "lb_attention_tree",
+             [c_int] + [c_void_p] * 5 + [c_int, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float, c_int, c_void_p, c_float] + [c_int] * 4
+             + [c_void_p, c_long, c_void_p])
+    _check(fn(dtype_code(q.dtype), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(block_table), block_table.shape[1], k_pool.shape[0],
+              _ptr(cu_q), _ptr(ctx_len), _ptr(positions if window else None), _ptr(tree), tree.shape[1], tokens, int(n_seqs), q_heads, kv_heads,
+              dim, page_tokens, float(scale), int(window), _ptr(sinks), float(softcap), tile_rows, row_tiles, chunks, chunk_tiles, _ptr(partials),
+              partials.numel() if partials is not None else 0, _stream()), "attention_tree")
+    if chunks > 1:
+        global LAUNCHES
+        LAUNCHES += 1          # the chunks' results are joined by a kernel of their own
+    return out
+
+
+def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
+    """pool[:, dst[i]] = pool[:, src[i]] for every i: pool [planes, pages, ...] of any type (the layers' pages of a cache, or the
+    layers' state slots), src and dst int32 [n] on the device. A page may be the source of several copies; no page is written twice or
+    read and written in one call. A pair with an index outside the pool is left out."""
+    _need(pool, None, "pool"); _need(src, torch.int32, "src"); _need(dst, torch.int32, "dst")
+    if pool.dim() < 2 or src.dim() != 1 or src.shape != dst.shape:
+        raise ValueError("copy_pages: pool [planes, pages, ...], src and dst one index per copy")
+    _here("copy_pages", pool, src, dst)
+    planes, pages = pool.shape[:2]
+    if pool.numel() == 0 or src.numel() == 0:
+        return pool
+    fn = _FUNCTIONS.get("lb_copy_pages") or _fn("cache_moves", "lb_copy_pages", [c_void_p] * 3 + [c_int] * 3 + [c_long, c_void_p])
+    _check(fn(_ptr(pool), _ptr(src), _ptr(dst), src.numel(), planes, pages, pool.numel() // (planes * pages) * pool.element_size(), _stream()), "copy_pages")
+    return pool
+
+
+def compact_tokens(pool: torch.Tensor, block_table: torch.Tensor, first: torch.Tensor, picked: torch.Tensor, cu_picked: torch.Tensor) -> torch.Tensor:
+    """The rows of the drafts that a sequence keeps move to the places right behind what it holds, in every plane and head of a
+    pool [planes, pages, heads, page_tokens, channels] of any type, in place: sequence s holds first[s] tokens and keeps its drafts
+    picked[cu_picked[s]] < picked[cu_picked[s] + 1] < ...; the row at place first[s] + picked[cu_picked[s] + i] goes to place first[s] + i. All
+    indices int32 on the device, block_table [S, W] the sequences' pages. Sequences do not share the pages these places are in. A draft that
+    lies outside its sequence's table, or whose page is outside the pool, is left out."""
+    _need(pool, None, "pool")
+    for name, t in (("block_table", block_table), ("first", first), ("picked", picked), ("cu_picked", cu_picked)):
+        _need(t, torch.int32, name)
+    n_seqs = first.numel()
+    if pool.dim() != 5 or block_table.dim() != 2 or block_table.shape[0] < n_seqs or cu_picked.numel() != n_seqs + 1:
+        raise ValueError("compact_tokens: pool [planes, pages, heads, page_tokens, channels], a table row and an end per sequence")
+    _here("compact_tokens", pool, block_table, first, picked, cu_picked)
+    planes, pages, heads, page_tokens, channels = pool.shape
+    if pool.numel() == 0 or picked.numel() == 0 or block_table.shape[1] == 0:
+        return pool
+    fn = _FUNCTIONS.get("lb_compact_tokens") or _fn("cache_moves", "lb_compact_tokens",
+             [c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_long, c_void_p])
+    _check(fn(_ptr(pool), _ptr(block_table), block_table.shape[1], _ptr(first), _ptr(picked), _ptr(cu_picked), n_seqs, planes, pages, heads,
+              page_tokens, channels * pool.element_size(), _stream()), "compact_tokens")
+    return pool
+
+
+BEAM_MAX_KEEP = 32      # the most continuations that `beam_select` chooses
+BEAM_MAX_BEAMS = 64     # the most beams of a request
+
+
+def _beam_chunk(rows: int, vocab: int, sms: int) -> int:
+    """Values of a row that a block of the first kernel reads: about three blocks an SM, at least 2,048 values each."""
+    chunks = max(1, min(-(-vocab // 2048), 3 * sms // rows))
+    return -(-vocab // chunks)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, next_scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor,
+                ended: torch.Tensor | None = None, pad: int = 0) -> None:
+    """The best continuations of every request's beams over the whole vocabulary, best first:
+
+        next_scores[r, k], parents[r, k], tokens[r, k] = the k-th largest scores[r, b] + log_softmax(logits[r * beams + b])[v], b, v
+
+    with equal ones in the order of b * vocab + v. logits float32 [requests * beams, V] (rows may be strided); scores float32 [requests,
+    beams], -inf for a beam that is not there; next_scores float32 [requests, keep], parents and tokens int32 alike, keep up to
+    BEAM_MAX_KEEP. `ended` int32 [requests, beams]: an ended beam (not 0) is one candidate, its own score with token `pad`. A beam whose
+    logits hold NaN or +inf, or nothing but -inf, has no candidates; places without a candidate get -inf, -1 and -1."""
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("beam_select: logits must be float32 [rows, vocab] with a contiguous vocabulary")
+    _need(scores, torch.float32, "scores"); _need(next_scores, torch.float32, "next_scores")
+    _need(parents, torch.int32, "parents"); _need(tokens, torch.int32, "tokens")
+    if scores.dim() != 2 or next_scores.dim() != 2 or parents.shape != next_scores.shape or tokens.shape != next_scores.shape \
+            or next_scores.shape[0] != scores.shape[0] or logits.shape[0] != scores.numel():
+        raise ValueError("beam_select: a row of logits per beam, scores [requests, beams], the outputs [requests, keep]")
+    requests, beams = scores.shape
+    keep, vocab = next_scores.shape[1], logits.shape[1]
+    if not 1 <= keep <= BEAM_MAX_KEEP or not 1 <= beams <= BEAM_MAX_BEAMS or not 0 <= pad < vocab:
+        raise ValueError(f"beam_select: keep is 1..{BEAM_MAX_KEEP}, beams 1..{BEAM_MAX_BEAMS}, pad a token of the vocabulary")
+    if ended is not None:
+        _need(ended, torch.int32, "ended")
+        if ended.shape != scores.shape:
+            raise ValueError("beam_select: ended must have scores' shape")
+    _here("beam_select", logits, scores, next_scores, parents, tokens, ended)
+    if requests == 0:
+        return
+    chunk = _beam_chunk(requests * beams, vocab, sm_count(logits.device))
+    scratch = torch.empty(requests * beams * -(-vocab // chunk) * (2 + 2 * keep), dtype=torch.int32, device=logits.device)     # of this call alone
+    fn = _FUNCTIONS.get("lb_beam_select") or _fn("beam", "lb_beam_select",
+             [c_void_p, c_long, c_void_p, c_void_p] + [c_int] * 6 + [c_void_p, c_long] + [c_void_p] * 4)
+    _check(fn(_ptr(logits), logits.stride(0), _ptr(scores), _ptr(ended), requests, beams, vocab, keep, int(pad), chunk, _ptr(scratch), scratch.numel(),
+              _ptr(next_scores), _ptr(parents), _ptr(tokens), _stream()), "beam_select")
+    global LAUNCHES
+    LAUNCHES += 1              # the chunks' lists are joined by a kernel of their own
 
 
 # ------------------------------------------------------------------ sampling

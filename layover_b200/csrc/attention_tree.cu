@@ -24,6 +24,8 @@
 // one to the rows that see them.
 #include <math.h>
 
+#include "attention_tree.cuh"
+#include "attention_tree_tcgen05.cuh"
 #include "common.cuh"
 
 namespace {
@@ -31,54 +33,6 @@ namespace {
 constexpr int THREADS = 128;
 constexpr int KEYS = 64;        // keys per tile
 constexpr int PAD = 8;          // bf16 of padding per shared-memory row
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct TreeArgs {
-  const void *q, *k_pool, *v_pool;
-  void* out;
-  const int* block_table;
-  int table_width, n_pages;
-  const int *cu_q, *ctx_len, *positions, *tree;
-  int tree_words, tokens;
-  int q_heads, kv_heads, dim, page_tokens;
-  float scale_log2;             // scale * log2(e)
-  float cap_in, cap_out;        // 2 log2(e) scale / cap and cap / scale; 0: no cap
-  int window;
-  const float* sinks;
-  int row_tiles, chunk_tiles;   // row tiles of a sequence, key tiles of a block
-  float* partials;              // [unit][chunk][rows][dim] outputs, then [unit][chunk][rows][2] maxima and sums; null: one chunk
-  long partial_stats;           // where the second part begins, in floats
-};
-
-// What a block works on: its rows, and its share of the keys.
-struct Unit {
-  int seq, head, row0, rows;    // the sequence, the first row of its tile and how many of the tile's rows there are
-  int first, n, held, ctx;      // its first token, drafts, held tokens, keys
-  int key_lo;                   // no row sees a key below
-  int tile_begin, tile_end, chunks;
-  long index;                   // in the partial results
-};
-
-__device__ __forceinline__ Unit find_unit(const TreeArgs& a, int tile_rows, int seq, int row_tile, int head, int chunk, int n_chunks) {
-  Unit u;
-  u.seq = seq; u.head = head;
-  u.first = a.cu_q[seq];
-  u.n = min(a.cu_q[seq + 1], a.tokens) - u.first;
-  u.ctx = a.ctx_len[seq];
-  u.held = u.ctx - u.n;
-  const int group = a.q_heads / a.kv_heads;
-  u.row0 = row_tile * tile_rows;
-  u.rows = min(tile_rows, u.n * group - u.row0);
-  u.key_lo = a.window > 0 ? max(0, u.held - a.window + 1) : 0;      // the first draft's position is `held` at least
-  const int tile_lo = u.key_lo / KEYS, tiles = (u.ctx + KEYS - 1) / KEYS - tile_lo;
-  u.chunks = min(n_chunks, max(1, (tiles + a.chunk_tiles - 1) / a.chunk_tiles));
-  u.tile_begin = tile_lo + chunk * a.chunk_tiles;
-  u.tile_end = tile_lo + (chunk == n_chunks - 1 ? tiles : min(tiles, (chunk + 1) * a.chunk_tiles));
-  u.index = ((long)seq * a.kv_heads + head) * a.row_tiles + row_tile;
-  return u;
-}
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
@@ -95,32 +49,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// Where key `key` of a sequence lies in its pool, in rows of one head's channels; -1 for a page that is not there.
-__device__ __forceinline__ long key_row(const TreeArgs& a, const int* table, int key, int head) {
-  const int index = key / a.page_tokens;
-  if (index >= a.table_width) return -1;
-  const int page = table[index];
-  if ((unsigned)page >= (unsigned)a.n_pages) return -1;
-  return ((long)page * a.kv_heads + head) * a.page_tokens + (key - index * a.page_tokens);
-}
-
-// Whether row `token` sees key `key`, `held` <= key < ctx or below: the tree decides among drafts, the window among held keys.
-__device__ __forceinline__ bool sees(const TreeArgs& a, const int* bits, int key, int held, int oldest) {
-  if (key < held) return key >= oldest;
-  const int j = key - held;
-  return (j >> 5) < a.tree_words && ((unsigned)bits[j >> 5] >> (j & 31)) & 1u;
-}
-
 // Keys [tile * 64, + 64) of one head into rows of `stride` elements of T; what lies outside [key_lo, ctx) becomes zeros.
 template <typename T>
 __device__ __forceinline__ void load_tile(T* to, const T* __restrict__ pool, const TreeArgs& a, const Unit& u, const int* table, int tile, int stride) {
@@ -131,10 +59,6 @@ __device__ __forceinline__ void load_tile(T* to, const T* __restrict__ pool, con
     const long row = key >= u.key_lo && key < u.ctx ? key_row(a, table, key, u.head) : -1;
     cp_async16(to + r * stride + c * PER, pool + (row < 0 ? 0 : row * a.dim) + c * PER, row < 0 ? 0 : 16);
   }
-}
-
-__device__ __forceinline__ bool not_finite(uint32_t two) {
-  return (two & 0x7F800000u) == 0x7F800000u || (two & 0x00007F80u) == 0x00007F80u;
 }
 
 // ------------------------------------------------------------------------------- bfloat16
@@ -151,7 +75,7 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.y / a.row_tiles;
-  const Unit u = find_unit(a, 16 * RG, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
+  const Unit u = find_unit<KEYS>(a, 16 * RG, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
   if (u.rows <= 0 || (int)blockIdx.z >= u.chunks) return;
   const int group = a.q_heads / a.kv_heads;
   const int* table = a.block_table + (size_t)seq * a.table_width;
@@ -407,7 +331,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeA
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.y / a.row_tiles;
-  const Unit u = find_unit(a, RT, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
+  const Unit u = find_unit<KEYS>(a, RT, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
   if (u.rows <= 0 || (int)blockIdx.z >= u.chunks) return;
   const int group = a.q_heads / a.kv_heads;
   const int* table = a.block_table + (size_t)seq * a.table_width;
@@ -572,7 +496,8 @@ __global__ void __launch_bounds__(THREADS) attention_tree_join_kernel(const Tree
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.y / a.row_tiles, row_tile = blockIdx.y - seq * a.row_tiles;
-  const Unit u = find_unit(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks);
+  const Unit u = tile_rows == wide::ROWS ? find_unit<wide::KEYS>(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks)
+                                          : find_unit<KEYS>(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks);
   const int local = blockIdx.z * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (local >= u.rows || u.chunks <= 1) return;
   const int group = a.q_heads / a.kv_heads, row = u.row0 + local, head = u.head * group + row % group;
@@ -626,7 +551,7 @@ int launch_f32(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
 }
 }  // namespace
 
-// `tile_rows`: rows of a block (16, 32 or 64). `chunks` blocks of `chunk_tiles` tiles of 64 keys share a row tile's keys (the
+// `tile_rows`: rows of a block: 16, 32 or 64, or 128 for the tcgen05 kernel. `chunks` blocks of `chunk_tiles` tiles of 64 keys (there: of 128) share a row tile's keys (the
 // last takes what is left); with more than one, `partials` holds n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) floats.
 LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
                                 int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words, int tokens,
@@ -637,7 +562,7 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
   if (dtype != LB_F32 && dtype != LB_BF16) return LB_ERR_DTYPE;
   if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || dim <= 0 || dim > 256 || dim % (dtype == LB_BF16 ? 16 : 4) || page_tokens <= 0 ||
       table_width <= 0 || n_pages <= 0 || tree_words <= 0 || window < 0 || softcap < 0.f || (window > 0 && !positions) || row_tiles <= 0 ||
-      chunks <= 0 || chunks > 65535 || chunk_tiles <= 0 || (long)n_seqs * row_tiles > 65535 || (tile_rows != 16 && tile_rows != 32 && tile_rows != 64))
+      chunks <= 0 || chunks > 65535 || chunk_tiles <= 0 || (long)n_seqs * row_tiles > 65535 || (tile_rows != 16 && tile_rows != 32 && tile_rows != 64 && tile_rows != 128))
     return LB_ERR_SIZE;
   const long partial_rows = (long)n_seqs * kv_heads * row_tiles * chunks * tile_rows;
   if (chunks > 1 && (!partials || partial_floats < partial_rows * (dim + 2))) return LB_ERR_SIZE;
@@ -647,7 +572,10 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
   if (softcap > 0.f) { a.cap_in = 2.f * LOG2E * scale / softcap; a.cap_out = softcap / scale; }
   const dim3 grid(kv_heads, n_seqs * row_tiles, chunks);
   int code;
-  if (dtype == LB_F32) {
+  if (tile_rows == 128) {
+    if (dtype != LB_BF16 || dim != 128 || page_tokens % 8 || 128 % page_tokens) return LB_ERR_SIZE;
+    code = wide::launch(a, grid, stream);
+  } else if (dtype == LB_F32) {
     code = tile_rows == 16 ? launch_f32<16>(a, grid, stream) : tile_rows == 32 ? launch_f32<32>(a, grid, stream) : launch_f32<64>(a, grid, stream);
   } else if (dim <= 128) {
     code = tile_rows == 16 ? launch_mma<1, 128>(a, grid, stream) : tile_rows == 32 ? launch_mma<2, 128>(a, grid, stream) : launch_mma<4, 128>(a, grid, stream);
@@ -659,4 +587,17 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
   code = dtype == LB_F32 ? lb_launch(attention_tree_join_kernel<float>, joined, THREADS, 0, stream, a, tile_rows, chunks)
                          : lb_launch(attention_tree_join_kernel<bf16>, joined, THREADS, 0, stream, a, tile_rows, chunks);
   return code ? code : lb_last_error();
+}
+
+LB_EXPORT void* lb_attention_tree_status_address() {
+  void* address = nullptr;
+  return cudaGetSymbolAddress(&address, g_tree_error) == cudaSuccess ? address : nullptr;
+}
+// What a bounded wait that ran out left, and clears it; synchronises.
+LB_EXPORT int lb_attention_tree_status() {
+  int code = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&code, g_tree_error, sizeof(int)) != cudaSuccess) return -1;
+  if (code) cudaMemcpyToSymbol(g_tree_error, &zero, sizeof(int));
+  return code;
 }

@@ -1282,22 +1282,27 @@ def attention_f32(q, cache, out, block_table, batch, q_heads, kv_heads, dim, pag
 
 
 # ------------------------------------------------------------------ several hypotheses of a request: drafts and beams
-_TREE_KEYS = 64                          # keys of a tile (csrc/attention_tree.cu)
 _TREE_SCRATCH_FLOATS = 64 << 20          # the most that the chunks' results may take (256 MiB)
 
 
+def attention_tree_on_tcgen05(rows: int, dim: int, page_tokens: int, dtype: torch.dtype) -> bool:
+    """Whether `attention_tree` takes these rows (drafts times heads of a group) to its tcgen05 kernel."""
+    return dtype == torch.bfloat16 and dim == 128 and page_tokens % 8 == 0 and 128 % page_tokens == 0 and rows > 16
+
+
 @functools.lru_cache(maxsize=1024)      # of the sizes alone, asked for by every layer of a step
-def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, dim: int, sms: int) -> tuple[int, int, int, int]:
-    """(rows of a block, row tiles of a sequence, chunks, key tiles of a chunk) for `attention_tree`: row tiles no larger than the
-    rows ask for, and as many chunks of the keys as give every SM about four blocks."""
+def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, dim: int, page_tokens: int, dtype: torch.dtype,
+              sms: int) -> tuple[int, int, int, int]:
+    """(rows of a block, row tiles of a sequence, chunks, key tiles of a chunk) for `attention_tree`."""
     rows = max_nodes * (q_heads // kv_heads)
-    tile_rows = 16 if rows <= 16 else 32 if rows <= 32 else 64
+    wide = attention_tree_on_tcgen05(rows, dim, page_tokens, dtype)
+    tile_rows, tile_keys, blocks = (128, 128, sms) if wide else (16 if rows <= 16 else 32 if rows <= 32 else 64, 64, 4 * sms)
     row_tiles = -(-rows // tile_rows)
     keys = min(max_ctx, max_nodes + window) if window else max_ctx
-    tiles = -(-keys // _TREE_KEYS) + (1 if window else 0)
+    tiles = -(-keys // tile_keys) + (1 if window else 0)
     units = n_seqs * kv_heads * row_tiles
     most = max(1, _TREE_SCRATCH_FLOATS // (units * tile_rows * (dim + 2)))
-    chunks = max(1, min(-(-4 * sms // units), tiles // 2, most, 65535))
+    chunks = max(1, min(-(-blocks // units), tiles // 2, most, 65535))
     chunk_tiles = -(-tiles // chunks)
     return tile_rows, row_tiles, -(-tiles // chunk_tiles), chunk_tiles
 
@@ -1350,7 +1355,8 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     _here("attention_tree", q, k_pool, v_pool, out, block_table, cu_q, ctx_len, positions if window else None, tree, sinks)
     if tokens == 0 or n_seqs == 0:
         return out
-    tile_rows, row_tiles, chunks, chunk_tiles = tree_plan(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, dim, sm_count(q.device))
+    tile_rows, row_tiles, chunks, chunk_tiles = tree_plan(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, dim, page_tokens, q.dtype,
+                                                           sm_count(q.device))
     partials = None
     if chunks > 1:          # of this call alone, on its own stream
         partials = torch.empty(n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2), dtype=torch.float32, device=q.device)
@@ -1365,6 +1371,14 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         global LAUNCHES
         LAUNCHES += 1          # the chunks' results are joined by a kernel of their own
     return out
+
+
+def attention_tree_status() -> int:
+    """0, or which bounded wait of the tcgen05 kernel of `attention_tree` ran out. Synchronises; clears the code."""
+    lib = build.load("attention_tree")
+    lib.lb_attention_tree_status.restype = c_int
+    torch.cuda.synchronize()
+    return lib.lb_attention_tree_status()
 
 
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
@@ -1498,7 +1512,8 @@ def sample(logits: torch.Tensor, tokens: torch.Tensor, records: torch.Tensor | N
 # normally returns to zero).
 _STATUS_LIBRARIES = (("gemm_tcgen05", "lb_gemm_tcgen05_status_address", "lb_gemm_tcgen05_status"),
                      ("attention_tcgen05", "lb_attention_tcgen05_status_address", "lb_attention_tcgen05_status"),
-                     ("gemm_simt", "lb_gemm_simt_status_address", "lb_gemm_simt_status"))
+                     ("gemm_simt", "lb_gemm_simt_status_address", "lb_gemm_simt_status"),
+                     ("attention_tree", "lb_attention_tree_status_address", "lb_attention_tree_status"))
 _status_words: dict[tuple[int, tuple[str, ...]], tuple[torch.Tensor, tuple[str, ...]]] = {}
 
 

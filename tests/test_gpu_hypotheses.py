@@ -113,6 +113,7 @@ class Trees:
 
     def check(self, got=None, finite=None):
         got = self.run() if got is None else got
+        assert ops().attention_tree_status() == 0
         want, sums, size = self.want()
         tokens = int(self.cu_q[-1])
         assert (got[tokens:] == 7.0).all()                                     # rows behind the last draft

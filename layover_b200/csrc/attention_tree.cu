@@ -496,8 +496,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_join_kernel(const Tree
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.y / a.row_tiles, row_tile = blockIdx.y - seq * a.row_tiles;
-  const Unit u = tile_rows == wide::ROWS ? find_unit<wide::KEYS>(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks)
-                                          : find_unit<KEYS>(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks);
+  const Unit u = find_unit<KEYS>(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks);
   const int local = blockIdx.z * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (local >= u.rows || u.chunks <= 1) return;
   const int group = a.q_heads / a.kv_heads, row = u.row0 + local, head = u.head * group + row % group;
@@ -551,31 +550,42 @@ int launch_f32(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
 }
 }  // namespace
 
-// `tile_rows`: rows of a block: 16, 32 or 64, or 128 for the tcgen05 kernel. `chunks` blocks of `chunk_tiles` tiles of 64 keys (there: of 128) share a row tile's keys (the
-// last takes what is left); with more than one, `partials` holds n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) floats.
+// What the three entries below check alike.
+static int check_tree(int dtype, const void* q, const void* k_pool, const void* v_pool, const void* out, int table_width, int n_pages, const int* positions,
+                      int tree_words, int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, int window, float softcap, int max_nodes) {
+  if (dtype != LB_F32 && dtype != LB_BF16) return LB_ERR_DTYPE;
+  if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || dim <= 0 || dim > 256 || dim % (dtype == LB_BF16 ? 16 : 4) || page_tokens <= 0 ||
+      table_width <= 0 || n_pages <= 0 || tree_words <= 0 || window < 0 || softcap < 0.f || (window > 0 && !positions) || max_nodes <= 0 || n_seqs > 65535 ||
+      (long)max_nodes * (q_heads / kv_heads) > 65535)
+    return LB_ERR_SIZE;
+  if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) return LB_ERR_ALIGN;
+  return 0;
+}
+
+// `tile_rows`: rows of a block (16, 32 or 64). `chunks` blocks of `chunk_tiles` tiles of 64 keys share a row tile's keys (the last takes
+// what is left); with more than one, `partials` holds n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) floats.
 LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
                                 int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words, int tokens,
                                 int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, float scale, int window, const float* sinks,
-                                float softcap, int tile_rows, int row_tiles, int chunks, int chunk_tiles, float* partials, long partial_floats,
-                                cudaStream_t stream) {
+                                float softcap, int max_nodes, int tile_rows, int row_tiles, int chunks, int chunk_tiles, float* partials,
+                                long partial_floats, cudaStream_t stream) {
   if (tokens <= 0 || n_seqs <= 0) return 0;
-  if (dtype != LB_F32 && dtype != LB_BF16) return LB_ERR_DTYPE;
-  if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || dim <= 0 || dim > 256 || dim % (dtype == LB_BF16 ? 16 : 4) || page_tokens <= 0 ||
-      table_width <= 0 || n_pages <= 0 || tree_words <= 0 || window < 0 || softcap < 0.f || (window > 0 && !positions) || row_tiles <= 0 ||
-      chunks <= 0 || chunks > 65535 || chunk_tiles <= 0 || (long)n_seqs * row_tiles > 65535 || (tile_rows != 16 && tile_rows != 32 && tile_rows != 64 && tile_rows != 128))
+  const int refused = check_tree(dtype, q, k_pool, v_pool, out, table_width, n_pages, positions, tree_words, n_seqs, q_heads, kv_heads, dim, page_tokens,
+                                 window, softcap, max_nodes);
+  if (refused) return refused;
+  if (row_tiles <= 0 || chunks <= 0 || chunks > 65535 || chunk_tiles <= 0 || (long)n_seqs * row_tiles > 65535 ||
+      (tile_rows != 16 && tile_rows != 32 && tile_rows != 64))
     return LB_ERR_SIZE;
   const long partial_rows = (long)n_seqs * kv_heads * row_tiles * chunks * tile_rows;
   if (chunks > 1 && (!partials || partial_floats < partial_rows * (dim + 2))) return LB_ERR_SIZE;
-  if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out | (uintptr_t)partials) & 15) return LB_ERR_ALIGN;
+  if ((uintptr_t)partials & 15) return LB_ERR_ALIGN;
   TreeArgs a{q, k_pool, v_pool, out, block_table, table_width, n_pages, cu_q, ctx_len, positions, tree, tree_words, tokens, q_heads, kv_heads, dim,
-             page_tokens, scale * LOG2E, 0.f, 0.f, window, sinks, row_tiles, chunk_tiles, chunks > 1 ? partials : nullptr, partial_rows * dim};
+             page_tokens, scale * LOG2E, 0.f, 0.f, window, sinks, row_tiles, chunk_tiles, chunks > 1 ? partials : nullptr, partial_rows * dim, n_seqs,
+             max_nodes, 0, 0, nullptr};
   if (softcap > 0.f) { a.cap_in = 2.f * LOG2E * scale / softcap; a.cap_out = softcap / scale; }
   const dim3 grid(kv_heads, n_seqs * row_tiles, chunks);
   int code;
-  if (tile_rows == 128) {
-    if (dtype != LB_BF16 || dim != 128 || page_tokens % 8 || 128 % page_tokens) return LB_ERR_SIZE;
-    code = wide::launch(a, grid, stream);
-  } else if (dtype == LB_F32) {
+  if (dtype == LB_F32) {
     code = tile_rows == 16 ? launch_f32<16>(a, grid, stream) : tile_rows == 32 ? launch_f32<32>(a, grid, stream) : launch_f32<64>(a, grid, stream);
   } else if (dim <= 128) {
     code = tile_rows == 16 ? launch_mma<1, 128>(a, grid, stream) : tile_rows == 32 ? launch_mma<2, 128>(a, grid, stream) : launch_mma<4, 128>(a, grid, stream);
@@ -586,6 +596,29 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
   const dim3 joined(kv_heads, n_seqs * row_tiles, tile_rows / (THREADS / 32));
   code = dtype == LB_F32 ? lb_launch(attention_tree_join_kernel<float>, joined, THREADS, 0, stream, a, tile_rows, chunks)
                          : lb_launch(attention_tree_join_kernel<bf16>, joined, THREADS, 0, stream, a, tile_rows, chunks);
+  return code ? code : lb_last_error();
+}
+
+// The tcgen05 kernel: bfloat16, heads of 128 channels, at most 128 query heads a key/value head, pages of 8 .. 128 tokens that divide 128. `blocks` blocks
+// share the keys; `rows2`: tiles of twice 128 / group drafts. `scratch` holds lb_attention_tree_scratch(blocks, rows2, n_seqs) floats.
+LB_EXPORT long lb_attention_tree_scratch(int blocks, int rows2, int n_seqs) { return wide::scratch_floats(blocks, rows2 != 0, n_seqs); }
+LB_EXPORT int lb_attention_tree_tcgen05(const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
+                                        int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words,
+                                        int tokens, int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, float scale, int window,
+                                        const float* sinks, float softcap, int max_nodes, int blocks, int rows2, float* scratch, long floats,
+                                        cudaStream_t stream) {
+  if (tokens <= 0 || n_seqs <= 0) return 0;
+  const int refused = check_tree(LB_BF16, q, k_pool, v_pool, out, table_width, n_pages, positions, tree_words, n_seqs, q_heads, kv_heads, dim, page_tokens,
+                                 window, softcap, max_nodes);
+  if (refused) return refused;
+  if (dim != 128 || q_heads / kv_heads > 128 || page_tokens % 8 || 128 % page_tokens || blocks <= 0 || blocks > 1024 || !scratch ||
+      floats < wide::scratch_floats(blocks, rows2 != 0, n_seqs))
+    return LB_ERR_SIZE;
+  if (((uintptr_t)scratch | (uintptr_t)out) & 31) return LB_ERR_ALIGN;
+  TreeArgs a{q, k_pool, v_pool, out, block_table, table_width, n_pages, cu_q, ctx_len, positions, tree, tree_words, tokens, q_heads, kv_heads, dim,
+             page_tokens, scale * LOG2E, 0.f, 0.f, window, sinks, 0, 0, scratch, 0, n_seqs, max_nodes, 0, 0, nullptr};
+  if (softcap > 0.f) { a.cap_in = 2.f * LOG2E * scale / softcap; a.cap_out = softcap / scale; }
+  const int code = rows2 ? wide::launch<true>(a, blocks, stream) : wide::launch<false>(a, blocks, stream);
   return code ? code : lb_last_error();
 }
 

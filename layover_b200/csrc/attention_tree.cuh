@@ -22,6 +22,9 @@ struct TreeArgs {
   int row_tiles, chunk_tiles;   // row tiles of a sequence, key tiles of a block
   float* partials;              // [unit][chunk][rows][dim] outputs, then [unit][chunk][rows][2] maxima and sums; null: one chunk
   long partial_stats;           // where the second part begins, in floats
+  int n_seqs, max_nodes;
+  int group, tile_drafts;       // query heads of a key/value head; drafts of a tile of 128 rows (the tcgen05 kernel's)
+  int* list;                    // the tcgen05 kernel's tiles, and how many lie before each sequence's
 };
 
 // What a block works on: its rows, and its share of the keys.
@@ -43,7 +46,7 @@ __device__ __forceinline__ Unit find_unit(const TreeArgs& a, int tile_rows, int 
   u.held = u.ctx - u.n;
   const int group = a.q_heads / a.kv_heads;
   u.row0 = row_tile * tile_rows;
-  u.rows = min(tile_rows, u.n * group - u.row0);
+  u.rows = min(tile_rows, min(u.n, a.max_nodes) * group - u.row0);
   u.key_lo = a.window > 0 ? max(0, u.held - a.window + 1) : 0;      // the first draft's position is `held` at least
   const int tile_lo = u.key_lo / KEYS, tiles = (u.ctx + KEYS - 1) / KEYS - tile_lo;
   u.chunks = min(n_chunks, max(1, (tiles + a.chunk_tiles - 1) / a.chunk_tiles));
@@ -55,11 +58,11 @@ __device__ __forceinline__ Unit find_unit(const TreeArgs& a, int tile_rows, int 
 
 // Bit i: whether a row sees key key0 + i, 32 of them: `bits` are its drafts, `oldest` the first held key it sees.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-__device__ __forceinline__ uint32_t seen_word(const TreeArgs& a, const int* bits, int key0, int held, int ctx, int oldest) {
+__device__ __forceinline__ uint32_t seen_word(int tree_words, const int* bits, int key0, int held, int ctx, int oldest) {
   const int j = key0 - held, w = j >> 5, shift = j & 31;          // the first key's draft; negative for held ones
   uint32_t drafts = 0;
   if (j > -32) {
-    const uint32_t lo = w >= 0 && w < a.tree_words ? (uint32_t)bits[w] : 0u, hi = w + 1 >= 0 && w + 1 < a.tree_words ? (uint32_t)bits[w + 1] : 0u;
+    const uint32_t lo = w >= 0 && w < tree_words ? (uint32_t)bits[w] : 0u, hi = w + 1 >= 0 && w + 1 < tree_words ? (uint32_t)bits[w + 1] : 0u;
     drafts = __funnelshift_r(lo, hi, shift);
   }
   const uint32_t kept = below(-j);

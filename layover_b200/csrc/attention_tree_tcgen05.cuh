@@ -1,10 +1,21 @@
 // Attention for trees of drafts on the 5th-generation tensor cores: bfloat16, heads of 128 channels, pages of 8 .. 128 tokens.
 //
-// A block takes up to 128 rows (draft * group + head of the group) of one key/value head and walks its chunk of the keys in tiles of
-// 128, dealt in turn to two warpgroups: each has scores and an output accumulator of its own in tensor memory, so one tile's
-// softmax runs under the other's products. K and V come page by page (TMA, one copy a lane) through one ring in the order in which the
-// products use them: K0, K1, V0, K2, V1, K3, ... The weights overwrite their scores in tensor memory and are the A operand of the
-// second product. At the end the two accumulators are joined in shared memory.
+// The work is a list of key tiles (128 keys of one key/value head for one tile of rows), sequence by sequence, and every block takes
+// an equal, contiguous share of the list: a few segments, each a row tile and a range of its keys. Blocks stay for the whole
+// launch, one an SM, so the loads of a segment run under the arithmetic and the stores of the one before. A row tile whose keys
+// lie in several blocks' shares leaves maxima, sums and unnormalised outputs in scratch memory, two places a block (its first and its last
+// segment), for `join_kernel`.
+//
+// A row tile holds 128 / group drafts with all their heads of the group, or, with ROWS2, twice as many. Two warpgroups of softmax
+// have scores and an output accumulator of their own in tensor memory: they take the key tiles in turn, or, with ROWS2, a half of
+// the rows each. Either way the products go through "turns" 0, 1, 2, ... of alternate warpgroups: O += P(t) V, then S(t + 2) = Q K^T,
+// so that one warpgroup's softmax runs under the other's products. K and V come through one ring in the order in which the products
+// use them, 16 bytes a thread (cp.async of two warps; a TMA copy of a page of 16 tokens takes 70 cycles whoever issues it, 1,150 for
+// the 32 KB of a tile with pages of 16, and 1,430 are what a tile may take at the memory's rate). The weights overwrite their scores in tensor
+// memory and are the A operand of the second product.
+//
+// Code that runs first is slow: a turn of softmax takes four times as long until its instructions have been fetched. So the warps run
+// through parts of it each, on nothing, while the first loads are under way.
 //
 // Rows that the tree does not have cost nothing but the tensor cores' time: their warps only hand tiles on. What a draft's values
 // hold that is not finite is zeroed in the tile and added at the end to the rows that see it.
@@ -23,22 +34,49 @@ namespace wide {
 constexpr int ROWS = 128, KEYS = 128, DIM = 128;
 constexpr int HALF_BYTES = 128 * 128;           // 64 channels of 128 rows
 constexpr int TILE_BYTES = 2 * HALF_BYTES;
-constexpr int STAGES = 5;
-constexpr int THREADS = 320;                    // warp 0 loads, warp 1 issues the products, warps 2-5 and 6-9 the softmax
-constexpr int PAGE_CACHE = 2048;                // block-table entries kept in shared memory
-constexpr int JOIN_STRIDE = DIM + 4;            // floats of a row that one warpgroup hands to the other
-constexpr int SMEM_BYTES = (1 + STAGES) * TILE_BYTES + 1024 + 512 + PAGE_CACHE * 4;
+constexpr int STAGES = 4;
+constexpr int LOADERS = 2;                      // warps that load K and V, each its rows of a tile
+constexpr int LOADER_EIGHTS = KEYS / LOADERS / 8;      // those rows, in eights
+constexpr int FIRST_SOFTMAX = 4;                // then one that issues the products (and one that does nothing), then two warpgroups of softmax
+constexpr int THREADS = 32 * (FIRST_SOFTMAX + 8);
+constexpr int FEW_REGS = 88, MANY_REGS = 208;   // of a thread of the first four warps and of the others: 128 * 88 + 256 * 208 = 384 * 168, the launch's
+constexpr int SEQ_CACHE = 512;                  // sequences whose lengths are kept there
+constexpr int SMEM_BYTES = (2 + STAGES) * TILE_BYTES + 1024 + 512 + 2 * 2 * ROWS * 8 + SEQ_CACHE * 16;
 constexpr float GROWTH = 8.0f;                  // the maximum that weights are relative to may lag by this, in log2 units
-static_assert(ROWS * JOIN_STRIDE * 4 + ROWS * 8 <= STAGES * TILE_BYTES, "the joined rows lie in the ring");
-
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void load_page(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+// Copies, barriers and arrivals by one elected lane of a whole warp with the same operands in every lane: as with the products (tcgen05.cuh),
+// from inside a branch each copy would take 60 cycles and more.
+__device__ __forceinline__ void load_queries(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-      ::"r"(smem_u32(dst)), "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar)) : "memory");
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}"
+      ::"r"(dst), "l"((uint64_t)map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+}
+// 16 bytes to shared memory; zeros where `bytes` is 0; an arrival on the barrier when all copies of this thread before it have landed
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zeros(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive_when_copied(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+template <int N> __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory"); }
+// 32 bytes of one thread: a whole sector of the L2
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 // D (+)= A B with A (two bfloat16 of K a column) in tensor memory
 __device__ __forceinline__ void umma_from_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -49,16 +87,17 @@ __device__ __forceinline__ void umma_from_tmem(uint32_t d_tmem, uint32_t a_tmem,
       "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {      // two loads under one wait
+  uint32_t r[128];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
-      "%23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%129];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(taddr), "r"(taddr + 64) : "memory");
+#pragma unroll
+  for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
@@ -83,345 +122,567 @@ __device__ __forceinline__ float row_max(const float (&s)[N]) {        // four c
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// What the drafts' value rows that were zeroed add to 16 channels of a row: their weights anew, from the tensors.
-__device__ __noinline__ void add_not_finite(const TreeArgs& a, const Unit& u, const int* table, int from, int upto, int row, int group, int oldest,
-                                            float base, int channel, float (&v)[16]) {
-  const bf16 *k_pool = (const bf16*)a.k_pool, *v_pool = (const bf16*)a.v_pool;
-  const int token = u.first + row / group;
-  const bf16* q = (const bf16*)a.q + ((size_t)token * a.q_heads + u.head * group + row % group) * DIM;
-  const int* bits = a.tree + (size_t)token * a.tree_words;
-  for (int key = max(from, u.held); key < upto; ++key) {
-    if (!sees(a, bits, key, u.held, oldest)) continue;
-    const long at = key_row(a, table, key, u.head);
-    if (at < 0) continue;
-    bool bad = false;
-    for (int c = 0; c < DIM; c += 2) bad |= not_finite(*reinterpret_cast<const uint32_t*>(v_pool + at * DIM + c));
-    if (!bad) continue;
-    float s = 0.f;
-    for (int c = 0; c < DIM; ++c) s += __bfloat162float(q[c]) * __bfloat162float(k_pool[at * DIM + c]);
-    if (a.cap_in != 0.f) s = a.cap_out - __fdividef(2.f * a.cap_out, 1.f + fast_exp2(s * a.cap_in));
-    const float w = fast_exp2(fmaf(s, a.scale_log2, -base));
-    if (w == 0.f) continue;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] += w * __bfloat162float(v_pool[at * DIM + channel + e]);
+// A sequence's rows and keys, and how many units of work it is: a unit is a row tile of a key/value head.
+struct Sequence {
+  int first, n, held, ctx, key_lo;      // its first token, drafts, held tokens, keys, the first key that a row may see
+  int row_tiles, tile_lo, tiles;        // row tiles; the first of its key tiles and how many there are (one at least)
+};
+template <bool ROWS2>
+__device__ __forceinline__ Sequence find_sequence(const TreeArgs& a, int first, int end, int ctx) {
+  Sequence s;
+  s.first = first;
+  s.n = min(end, a.tokens) - first;
+  s.ctx = ctx;
+  s.held = s.ctx - s.n;
+  s.key_lo = a.window > 0 ? max(0, s.held - a.window + 1) : 0;
+  const int drafts = a.tile_drafts * (ROWS2 ? 2 : 1);
+  s.row_tiles = s.n <= 0 ? 0 : (min(s.n, a.max_nodes) + drafts - 1) / drafts;
+  s.tile_lo = s.key_lo / KEYS;
+  s.tiles = max(1, (s.ctx + KEYS - 1) / KEYS - s.tile_lo);
+  return s;
+}
+template <bool ROWS2>
+__device__ __forceinline__ Sequence find_sequence(const TreeArgs& a, const int4* known, int seq) {
+  if (seq < SEQ_CACHE) {
+    const int4 k = known[seq];
+    return find_sequence<ROWS2>(a, k.x, k.y, k.z);
   }
+  return find_sequence<ROWS2>(a, a.cu_q[seq], a.cu_q[seq + 1], a.ctx_len[seq]);
 }
 
-__global__ void __launch_bounds__(THREADS, 1) attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                                                                          const TreeArgs a) {
+// The blocks' shares of `total` tiles: block b begins at total * b / blocks. No more blocks than tiles: a share is empty only where
+// it stands behind the list.
+__device__ __forceinline__ int share_begin(int total, int b, int blocks) {
+  return total < 1 << 20 ? (int)((unsigned)total * (unsigned)b / (unsigned)blocks) : (int)((long)total * b / blocks);      // blocks: 1,024 at most
+}
+__device__ __forceinline__ int share_of(int total, int at, int blocks) { return (int)((((long)at + 1) * blocks - 1) / total); }
+
+// A block's walk through its share, segment by segment; every role of the block makes the same walk. A segment is the key tiles
+// [begin, begin + count) of a row tile, counted from tile_lo on.
+template <bool ROWS2>
+struct Walk {
+  const int4* known;                    // the lengths of the first sequences
+  int next_seq, offset, left;           // where the walk stands: in tiles of that sequence; tiles still to come
+  Sequence s;
+  int seq, head, row_tile, begin, count;
+  __device__ __forceinline__ void begin_at(const TreeArgs& a, const int4* known_, int seq_, int offset_, int left_) {
+    known = known_; next_seq = seq_; offset = offset_; left = left_;
+    count = 0;
+    if (left > 0) s = find_sequence<ROWS2>(a, known, next_seq);
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& a) {
+    if (left <= 0) return false;
+    while (offset >= a.kv_heads * s.row_tiles * s.tiles) { offset = 0; s = find_sequence<ROWS2>(a, known, ++next_seq); }     // sequences without drafts have no tiles
+    const int unit = offset / s.tiles;
+    seq = next_seq; head = unit / s.row_tiles; row_tile = unit - head * s.row_tiles;
+    begin = offset - unit * s.tiles;
+    count = min(s.tiles - begin, left);
+    offset += count; left -= count;
+    return true;
+  }
+};
+
+// The weight of a draft whose value row was zeroed, for a row that sees it; 0 for any other: from the tensors, which is seldom.
+// `at`: the draft's row in the pools.
+__device__ __noinline__ float zeroed_weight(const bf16* q, const bf16* k_pool, const bf16* v_pool, long at, float cap_in, float cap_out, float scale_log2, float base) {
+  bool bad = false;
+  for (int c = 0; c < DIM; c += 2) bad |= not_finite(*reinterpret_cast<const uint32_t*>(v_pool + at * DIM + c));
+  if (!bad) return 0.f;
+  float s = 0.f;
+  for (int c = 0; c < DIM; ++c) s += __bfloat162float(q[c]) * __bfloat162float(k_pool[at * DIM + c]);
+  if (cap_in != 0.f) s = cap_out - __fdividef(2.f * cap_out, 1.f + fast_exp2(s * cap_in));
+  return fast_exp2(fmaf(s, scale_log2, -base));
+}
+template <bool ROWS2>
+__global__ void __launch_bounds__(THREADS, 1)
+attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const TreeArgs a) {
   extern __shared__ uint8_t raw_smem[];
-  uint8_t* q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
-  uint8_t* ring = q_s + TILE_BYTES;
+  uint8_t* q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);      // two tiles: of two segments, or of two halves
+  uint8_t* ring = q_s + 2 * TILE_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + STAGES * TILE_BYTES);
   uint64_t* full = bars;              // [STAGES]
-  uint64_t* empty = bars + STAGES;    // [STAGES]
-  uint64_t* q_full = bars + 2 * STAGES;
-  uint64_t* s_full = q_full + 1;      // [2 warpgroups] the scores of a tile are in tensor memory
-  uint64_t* p_full = q_full + 3;      // [2] its weights are, and the output is rescaled
-  uint64_t* pv_done = q_full + 5;     // [2] its second product is finished
-  uint64_t* all_done = q_full + 7;    // every product is
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 8);
-  volatile uint32_t* flag = tmem_slot + 1;        // [0] a wait ran out, [1] a draft's values are not finite
-  int* page_cache = reinterpret_cast<int*>(bars) + 128;
+  uint64_t* empty = full + STAGES;    // [STAGES]
+  uint64_t* q_full = empty + STAGES;  // [2] a segment's queries have come (ROWS2: [0] alone)
+  uint64_t* q_empty = q_full + 2;     // [2] its last scores are made
+  uint64_t* s_full = q_empty + 2;     // [2 warpgroups] the scores of a turn are in tensor memory
+  uint64_t* p_full = s_full + 2;      // [2] its weights are, and the output is rescaled
+  uint64_t* pv_done = p_full + 2;     // [2] its second product is finished
+  uint64_t* o_full = pv_done + 2;     // a segment's products are finished
+  uint64_t* o_empty = o_full + 1;     // its outputs have been read
+  uint64_t* stats_full = o_empty + 1; // its maxima and sums are in shared memory
+  uint64_t* started = stats_full + 1; // `start` and `known` are
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(started + 1);
+  volatile uint32_t* flag = tmem_slot + 1;        // [0] a wait ran out, [1] a draft's values were not finite
+  int* start = const_cast<int*>(reinterpret_cast<volatile int*>(flag + 2));      // where the walk begins: sequence, tile of it, tiles
+  float2* stats = reinterpret_cast<float2*>(bars + 64);      // [2 segments][2 warpgroups][ROWS]
+  int4* known = reinterpret_cast<int4*>(stats + 4 * ROWS);                  // first draft, end, keys and tiles of the first sequences
 
-  pdl_launch_dependents();
-  pdl_wait();
-  const int seq = blockIdx.y / a.row_tiles;
-  const Unit u = find_unit<KEYS>(a, ROWS, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
-  if (u.rows <= 0 || (int)blockIdx.z >= u.chunks) return;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int group = a.q_heads / a.kv_heads, n_tiles = max(0, u.tile_end - u.tile_begin);
-  const int* table = a.block_table + (size_t)seq * a.table_width;
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    mbar_init(q_full, 8);
-    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1); }
-    mbar_init(all_done, 1);
+  if (threadIdx.x == 32 * LOADERS) {
+    for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 32 * LOADERS); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(o_full, 1); mbar_init(o_empty, 8); mbar_init(stats_full, 8); mbar_init(started, 1);
     flag[0] = 0; flag[1] = 0;
+    prefetch_map(&q_map);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  __syncwarp();
+  if (warp == LOADERS) tmem_alloc(tmem_slot, 512);
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem_s = *tmem_slot, tmem_o = tmem_s + 256;      // two of 128 columns each
+  const int group = a.group, drafts_tile = a.tile_drafts;      // drafts of 128 rows
   auto ran_out = [&](int code) { atomicCAS(&g_tree_error, 0, code); flag[0] = 1; return false; };
-
-  float m_ref = -INFINITY, l_sum = 0.f;
-  const int wg = (warp - 2) >> 2, quarter = warp & 3, row_local = quarter * 32 + lane;
-  const int row = u.row0 + row_local, token = u.first + min(row, u.n * group - 1) / group;
-  const int* bits = a.tree + (size_t)token * a.tree_words;
-  const int oldest = a.window > 0 ? max(a.positions[token], u.held) - a.window + 1 : 0;
-  const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
   bool ok = true;
+  pdl_launch_dependents();
 
-  if (warp == 0) {
-    // ---------------- K and V, page by page; pages that are not there lie behind the pool's last and read as zeros
-    const int per_tile = KEYS / a.page_tokens, first_page = u.tile_begin * per_tile, last_page = min(a.table_width, (u.ctx + a.page_tokens - 1) / a.page_tokens);
-    const int cached = min(n_tiles * per_tile, PAGE_CACHE);
-    auto page_at = [&](int i) {
-      const int page = i < last_page ? table[i] : -1;
-      return (unsigned)page < (unsigned)a.n_pages ? page : a.n_pages;
-    };
-    for (int i = lane; i < cached; i += 32) page_cache[i] = page_at(first_page + i);
+  if (warp < FIRST_SOFTMAX) give_registers<FEW_REGS>(); else take_registers<MANY_REGS>();
+  if (warp < LOADERS) {
+    pdl_wait();
+    if (warp == 0) {
+    // ---------------- the list's length, then the sequence in which this block's share begins
+    int total = 0;
+    for (int base = 0; base < a.n_seqs; base += 32) {
+      int tiles = 0;
+      if (base + lane < a.n_seqs) {
+        const int i = base + lane, first = a.cu_q[i], end = a.cu_q[i + 1], ctx = a.ctx_len[i];
+        const Sequence s = find_sequence<ROWS2>(a, first, end, ctx);
+        tiles = a.kv_heads * s.row_tiles * s.tiles;
+        if (i < SEQ_CACHE) known[i] = make_int4(first, end, ctx, tiles);
+      }
+      total += __reduce_add_sync(0xffffffffu, tiles);
+    }
+    const int blocks = min((int)gridDim.x, total), b = min((int)blockIdx.x, blocks);
+    const int from = b < blocks ? share_begin(total, b, blocks) : total, upto = b < blocks ? share_begin(total, b + 1, blocks) : total;
+    if (lane == 0) { start[0] = start[1] = 0; start[2] = upto - from; }
     __syncwarp();
-    const int pg = lane >> 1, half = lane & 1;
-    int count = 0;
-    auto load = [&](int tile, const CUtensorMap* map) {
-      const int stage = count % STAGES;
-      if (!warp_wait(&empty[stage], ((count / STAGES) & 1) ^ 1)) return ran_out(1);
+    int before = 0;
+    for (int base = 0; base < a.n_seqs; base += 32) {
+      const int i = base + lane;
+      int tiles = 0;
+      if (i < a.n_seqs) {
+        if (i < SEQ_CACHE) {
+          tiles = known[i].w;
+        } else {
+          const Sequence s = find_sequence<ROWS2>(a, known, i);
+          tiles = a.kv_heads * s.row_tiles * s.tiles;
+        }
+      }
+      int sum = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += other;
+      }
+      const int mine = before + sum - tiles;
+      if (from >= mine && from < mine + tiles) { start[0] = i; start[1] = from - mine; }
+      if (blockIdx.x == 0 && i < a.n_seqs) a.list[1 + i] = mine;       // for the kernel that joins
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (blockIdx.x == 0 && lane == 0) a.list[0] = total;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(started);
+    } else {
+      ok = warp_wait(started, 0) || ran_out(1);
+    }
+    // ---------------- K and V, and the first of these warps the queries
+    const int n_tiles = ok ? start[2] : 0, row0 = warp * 8 * LOADER_EIGHTS, page_shift = __ffs(a.page_tokens) - 1;      // of a tile, this warp's rows
+    // a lane copies 16 bytes of rows 2 i + (lane >> 4) of each 8 of this warp's rows; `to` are their places in those 8, swizzled
+    const uint32_t ring_at = smem_u32(ring) + ((lane & 15) >> 3) * HALF_BYTES + row0 * 128;
+    uint32_t to[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = (2 * i + (lane >> 4)) * 128 + (((lane & 7) ^ (2 * i + (lane >> 4))) << 4);
+    const long lane_from = (lane >> 4) * DIM + (lane & 15) * 8;
+    int taken = 0;
+    // what a tile's copies need: the place in a pool of the first of rows 8 i .. (lane i of LOADER_EIGHTS; -1: its page is not there), its first key,
+    // which keys may be seen, and whether all of them are there
+    struct Tile { int row, key0, key_lo, ctx; bool whole; } tiles[2], coming;
+    auto load = [&](const bf16* pool, const Tile& t) {
+      const int stage = taken % STAGES;
+      if (!warp_wait(&empty[stage], ((taken / STAGES) & 1) ^ 1)) return ran_out(1);
       if (flag[0]) return false;
-      if (lane == 0) mbar_expect_tx(&full[stage], TILE_BYTES);
-      __syncwarp();
-      if (pg < per_tile) {
-        const int local = tile * per_tile + pg, page = local < PAGE_CACHE ? page_cache[local] : page_at(first_page + local);
-        load_page(ring + stage * TILE_BYTES + half * HALF_BYTES + pg * a.page_tokens * 128, map, &full[stage], half * 64, 0, u.head, page);
+      const uint32_t at = ring_at + stage * TILE_BYTES;
+      if (t.whole) {
+#pragma unroll
+        for (int g = 0; g < LOADER_EIGHTS; ++g) {
+          const bf16* from = pool + (long)__shfl_sync(0xffffffffu, t.row, g) * DIM + lane_from;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) copy16(at + to[i] + g * 1024, from + 2 * i * DIM);
+        }
+      } else {
+#pragma unroll 1
+        for (int g = 0; g < LOADER_EIGHTS; ++g) {
+          const int row = __shfl_sync(0xffffffffu, t.row, g);
+          const bf16* from = pool + (row < 0 ? 0 : (long)row * DIM + lane_from);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = t.key0 + row0 + g * 8 + 2 * i + (lane >> 4);
+            const bool wanted = row >= 0 && key < t.ctx && key >= t.key_lo;
+            copy16_or_zeros(at + to[i] + g * 1024, wanted ? from + 2 * i * DIM : pool, wanted ? 16 : 0);
+          }
+        }
       }
-      ++count;
+      arrive_when_copied(smem_u32(&full[stage]));
+      ++taken;
       return true;
     };
-    if (n_tiles > 0) ok = load(0, &k_map);
-    if (ok && n_tiles > 1) ok = load(1, &k_map);
-    for (int i = 0; i < n_tiles && ok; ++i) {
-      ok = load(i, &v_map);
-      if (ok && i + 2 < n_tiles) ok = load(i + 2, &k_map);
-    }
-  } else if (warp == 1) {
-    // ---------------- the products, in the order of the ring
-    const int tiles = warp_uniform(n_tiles);
-    int count = 0;
-    auto scores = [&](int i) {
-      const int stage = count % STAGES, w = i & 1;
-      if (!warp_wait(&full[stage], (count / STAGES) & 1)) return ran_out(3);
-      fence_after_sync();
-      const uint32_t q_addr = smem_u32(q_s), k_addr = smem_u32(ring + stage * TILE_BYTES);
-#pragma unroll
-      for (int ks = 0; ks < DIM / 16; ++ks) {
-        const uint32_t off = (ks >> 2) * HALF_BYTES + (ks & 3) * 32;
-        umma_bf16(tmem_s + w * 128, desc_k_major(q_addr + off), desc_k_major(k_addr + off), IDESC_S, ks > 0 ? 1u : 0u);
+    // K is loaded two turns ahead of V: its walk is `ahead`, its next tile `coming`, whose page is on its way; V's tiles are K's before
+    Walk<ROWS2> ahead;
+    ahead.begin_at(a, known, start[0], start[1], n_tiles);
+    int tile = 0, segments = 0, page = -1;
+    auto fetch = [&]() {                                     // the next tile of the walk, if there is one
+      if (tile == ahead.count) {
+        if (!ahead.next(a)) return;
+        tile = 0;
       }
-      umma_commit(&s_full[w]);
-      umma_commit(&empty[stage]);
-      ++count;
+      coming.key0 = (ahead.s.tile_lo + ahead.begin + tile) * KEYS; coming.key_lo = ahead.s.key_lo; coming.ctx = ahead.s.ctx;
+      const int key = coming.key0 + row0 + (lane & (LOADER_EIGHTS - 1)) * 8, index = key >> page_shift;
+      page = index < a.table_width && key < ahead.s.ctx ? a.block_table[(size_t)ahead.seq * a.table_width + index] : -1;
+    };
+    auto load_k = [&](Tile& t) {
+      const bool there = (unsigned)page < (unsigned)a.n_pages;
+      t = coming;
+      t.row = there ? (page * a.kv_heads + ahead.head) * a.page_tokens + ((t.key0 + row0 + (lane & (LOADER_EIGHTS - 1)) * 8) & (a.page_tokens - 1)) : -1;
+      t.whole = __all_sync(0xffffffffu, there) && t.key0 >= t.key_lo && t.key0 + KEYS <= t.ctx;
+      if (tile == 0) {
+        if (warp == 0) {
+          const int buf = ROWS2 ? 0 : segments & 1;
+          if (!warp_wait(&q_empty[buf], ((ROWS2 ? segments : segments >> 1) & 1) ^ 1)) return ran_out(2);
+          const uint32_t bar = smem_u32(&q_full[buf]);
+          expect_bytes(bar, (uint32_t)(drafts_tile * group * 128) * (ROWS2 ? 4 : 2));
+          const int head = warp_uniform(ahead.head * group), draft = warp_uniform(ahead.s.first + ahead.row_tile * (ROWS2 ? 2 : 1) * drafts_tile);
+          for (int part = 0; part < (ROWS2 ? 2 : 1); ++part)
+            for (int h = 0; h < 2; ++h)
+              load_queries(smem_u32(q_s) + (ROWS2 ? part : buf) * TILE_BYTES + h * HALF_BYTES, &q_map, bar, h * 64, head, draft + part * drafts_tile);
+        }
+        ++segments;
+      }
+      ++tile;
+      if (!load((const bf16*)a.k_pool, t)) return false;
+      fetch();
       return true;
     };
-    if (tiles > 0) ok = (warp_wait(q_full, 0) || ran_out(2)) && scores(0);
-    if (ok && tiles > 1) ok = scores(1);
-    for (int i = 0; i < tiles && ok; ++i) {
-      const int stage = count % STAGES, w = i & 1;
-      ok = (warp_wait(&full[stage], (count / STAGES) & 1) || ran_out(4)) && (warp_wait(&p_full[w], (i >> 1) & 1) || ran_out(5));
-      if (!ok) break;
-      fence_after_sync();
-      const uint32_t v_addr = smem_u32(ring + stage * TILE_BYTES);
-#pragma unroll
-      for (int ks = 0; ks < KEYS / 16; ++ks)              // 16 keys: 8 columns of weights, 16 rows of V
-        umma_from_tmem(tmem_o + w * 128, tmem_s + w * 128 + ks * 8, desc_mn_major(v_addr + ks * 16 * 128), IDESC_O, (i > 1 || ks > 0) ? 1u : 0u);
-      umma_commit(&pv_done[w]);
-      umma_commit(&empty[stage]);
-      ++count;
-      if (i + 2 < tiles) ok = scores(i + 2);
-    }
-    if (ok) umma_commit(all_done);
-  } else {
-    // ---------------- the queries, swizzled as the products read them; rows that are not there are zeros
-    {
-      const bf16* q = (const bf16*)a.q;
-      const int t = threadIdx.x - 64;
-      uint4 w[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = (t + i * 256) >> 4, c = t & 15, at = u.row0 + r;
-        w[i] = make_uint4(0, 0, 0, 0);
-        if (r < u.rows) w[i] = *reinterpret_cast<const uint4*>(q + ((size_t)(u.first + at / group) * a.q_heads + u.head * group + at % group) * DIM + c * 8);
+    fetch();
+    if (n_tiles > 0) ok = load_k(tiles[0]);
+    if (!ROWS2) {
+      if (ok && n_tiles > 1) ok = load_k(tiles[1]);
+      for (int i = 0; i < n_tiles && ok; i += 2) {
+        ok = load((const bf16*)a.v_pool, tiles[0]);
+        if (ok && i + 2 < n_tiles) ok = load_k(tiles[0]);
+        if (ok && i + 1 < n_tiles) ok = load((const bf16*)a.v_pool, tiles[1]);
+        if (ok && i + 3 < n_tiles) ok = load_k(tiles[1]);
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = (t + i * 256) >> 4, c = t & 15;
-        *reinterpret_cast<uint4*>(q_s + (c >> 3) * HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = w[i];
+    } else {
+      for (int i = 0; i < n_tiles && ok; ++i) {
+        ok = load((const bf16*)a.v_pool, tiles[0]);
+        if (ok && i + 1 < n_tiles) ok = load_k(tiles[0]);
       }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
     }
-    // ---------------- softmax: one row a thread, every other tile a warpgroup
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == LOADERS) {
+    // ---------------- the products, turn by turn; the scores are two turns ahead
+    pdl_wait();
+    ok = warp_wait(started, 0) || ran_out(2);
+    const int n_tiles = ok ? start[2] : 0;
+    Walk<ROWS2> ahead, walk;
+    ahead.begin_at(a, known, start[0], start[1], n_tiles);
+    walk.begin_at(a, known, start[0], start[1], n_tiles);
+    const int turns = warp_uniform(n_tiles * (ROWS2 ? 2 : 1));
+    int taken = 0, k_stage = 0, v_stage = 0;
+    int a_left = 0, a_segment = -1, g_left = 0, g_turn = 0, g_segment = -1;
+    // turn -2 and -1 have scores to be made and no second product: the loop holds each kind of product once
+#pragma unroll 1
+    for (int t = -2; t < turns && ok; ++t) {
+      const int w = t & 1;
+      if (t >= 0) {
+        if (g_left == 0) {
+          walk.next(a);
+          g_left = warp_uniform(ROWS2 ? 2 * walk.count : walk.count);
+          g_turn = 0;
+          ++g_segment;
+          if (g_segment > 0) ok = warp_wait(o_empty, (g_segment - 1) & 1) || ran_out(8);
+        }
+        if (ok && (!ROWS2 || w == 0)) {
+          v_stage = taken % STAGES;
+          ok = warp_wait(&full[v_stage], (taken / STAGES) & 1) || ran_out(4);
+          ++taken;
+          fence_async_smem();                              // what cp.async wrote is read by the tensor cores
+        }
+        ok = ok && (warp_wait(&p_full[w], (t >> 1) & 1) || ran_out(5));
+        if (!ok) break;
+        fence_after_sync();
+        const uint32_t v_addr = smem_u32(ring + v_stage * TILE_BYTES);
+#pragma unroll
+        for (int ks = 0; ks < KEYS / 16; ++ks)            // 16 keys: 8 columns of weights, 16 rows of V
+          umma_from_tmem(tmem_o + w * 128, tmem_s + w * 128 + ks * 8, desc_mn_major(v_addr + ks * 16 * 128), IDESC_O, (g_turn > 1 || ks > 0) ? 1u : 0u);
+        umma_commit(&pv_done[w]);
+        if (!ROWS2 || w == 1) umma_commit(&empty[v_stage]);
+        ++g_turn;
+        if (--g_left == 0) umma_commit(o_full);
+      }
+      if (t + 2 < turns) {
+        if (a_left == 0) {
+          ahead.next(a);
+          a_left = warp_uniform(ROWS2 ? 2 * ahead.count : ahead.count);
+          ++a_segment;
+          ok = warp_wait(&q_full[ROWS2 ? 0 : a_segment & 1], (ROWS2 ? a_segment : a_segment >> 1) & 1) || ran_out(2);
+        }
+        if (ok && (!ROWS2 || w == 0)) {
+          k_stage = taken % STAGES;
+          ok = warp_wait(&full[k_stage], (taken / STAGES) & 1) || ran_out(3);
+          ++taken;
+          fence_async_smem();
+        }
+        if (!ok) break;
+        fence_after_sync();
+        const uint32_t q_addr = smem_u32(q_s + (ROWS2 ? w : a_segment & 1) * TILE_BYTES), k_addr = smem_u32(ring + k_stage * TILE_BYTES);
+#pragma unroll
+        for (int ks = 0; ks < DIM / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * HALF_BYTES + (ks & 3) * 32;
+          umma_bf16(tmem_s + w * 128, desc_k_major(q_addr + off), desc_k_major(k_addr + off), IDESC_S, ks > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[w]);
+        if (!ROWS2 || w == 1) umma_commit(&empty[k_stage]);
+        if (--a_left == 0) umma_commit(&q_empty[ROWS2 ? 0 : a_segment & 1]);
+      }
+    }
+  } else if (warp >= FIRST_SOFTMAX) {
+    // ---------------- softmax: one row a thread
+    const int wg = (warp - FIRST_SOFTMAX) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t my_s = tmem_s + wg * 128 + lane_addr, my_o = tmem_o + wg * 128 + lane_addr;
-    const bool live = quarter * 32 < u.rows;              // whether this warp has a row at all
     const float c = a.scale_log2;
-    for (int i = wg; i < n_tiles && ok; i += 2) {
-      const int j = i >> 1, key0 = (u.tile_begin + i) * KEYS;
-      // value rows of keys that are not there, or that nobody may see, may hold anything: zeroed, since 0 x NaN is NaN
-      const bool drafts = key0 + KEYS > u.held, edge = drafts || key0 < u.key_lo;
-      // a warp without rows waits as well: the tile before has been handed on by all four by then
-      ok = mbar_wait(&s_full[wg], j & 1) || ran_out(6);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      fence_after_sync();
-      if (live) {
-        float s[KEYS];
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {
-          uint32_t raw[32];
-          tmem_ld32(my_s + part * 32, raw);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) s[part * 32 + e] = __uint_as_float(raw[e]);
-        }
-        if (a.cap_in != 0.f) {
-#pragma unroll
-          for (int e = 0; e < KEYS; ++e) s[e] = a.cap_out - __fdividef(2.f * a.cap_out, 1.f + fast_exp2(s[e] * a.cap_in));
-        }
-        if (edge || a.window > 0) {
-#pragma unroll
-          for (int part = 0; part < 4; ++part) {
-            const uint32_t word = seen_word(a, bits, key0 + part * 32, u.held, u.ctx, oldest);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(word >> e & 1u)) s[part * 32 + e] = -INFINITY;
-          }
-        }
-        const float top = row_max(s);
-        const bool grow = (top - m_ref) * c > GROWTH || (m_ref == -INFINITY && top > -INFINITY);
-        const bool any_grow = __any_sync(0xffffffffu, grow);
-        const float m_new = grow ? top : m_ref;
-        const float factor = m_ref == -INFINITY ? 0.f : fast_exp2((m_ref - m_new) * c);
-        const float neg_base = m_new == -INFINITY ? 0.f : -m_new * c;
-        float sums[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t w[KEYS / 2];
-#pragma unroll
-        for (int e = 0; e < KEYS / 2; ++e) {
-          const float x = fast_exp2(fmaf(s[2 * e], c, neg_base)), y = fast_exp2(fmaf(s[2 * e + 1], c, neg_base));
-          sums[e & 3] += x + y;
-          w[e] = pack_bf16(x, y);
-        }
-        l_sum = l_sum * factor + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
-        m_ref = m_new;
-#pragma unroll
-        for (int part = 0; part < 4; ++part) {
-          uint32_t piece[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) piece[e] = w[part * 16 + e];
-          tmem_st16(my_s + part * 16, piece);
-        }
-        if (any_grow && j > 0) {
-          ok = mbar_wait(&pv_done[wg], (j - 1) & 1) || ran_out(7);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          fence_after_sync();
-#pragma unroll
-          for (int ch = 0; ch < DIM / 16; ++ch) {
-            float v[16];
-            uint32_t r[16];
-            tmem_ld16(my_o + ch * 16, v);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(v[e] * factor);
-            tmem_st16(my_o + ch * 16, r);
-          }
-        }
-        tmem_wait_st();
-      }
-      if (edge) {
-        const int at = min(n_tiles, 2) + i + min(i, max(0, n_tiles - 2)), stage = at % STAGES;      // V(i)'s place in the ring's order
-        ok = mbar_wait(&full[stage], (at / STAGES) & 1) || ran_out(4);
+    // Segment -1 is a turn on nothing, of which every warp goes through a part (masks and maximum, weights, rescaling and values, the
+    // segment's end) and whose result nobody takes: their instructions are fetched side by side while the first loads are under way.
+    Walk<ROWS2> g;
+    g.begin_at(a, known, 0, 0, 0);
+    g.begin = g.row_tile = g.head = g.seq = 0; g.s = Sequence{};
+    int turn0 = 0, n_tiles = 0;                            // the segment's first turn; the block's tiles
+    for (int k = -1; ok; ++k) {
+      const bool dry = k < 0;
+      if (k == 0) {
+        pdl_wait();
+        ok = mbar_wait(started, 0) || ran_out(6);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        const int key = key0 + row_local;
-        uint8_t* v_row = ring + stage * TILE_BYTES + row_local * 128;
-        bool zero = key >= u.ctx || key < u.key_lo;
-        if (!zero && key >= u.held) {
-          bool bad = false;
+        n_tiles = start[2];
+        g.begin_at(a, known, start[0], start[1], n_tiles);
+      }
+      if (!dry && !g.next(a)) break;
+      const int turns = dry ? 2 : ROWS2 ? 2 * g.count : g.count, held = dry ? 1 : g.s.held, ctx = dry ? KEYS - 1 : g.s.ctx, key_lo = dry ? 0 : g.s.key_lo;
+      const int first_key = dry ? 0 : (g.s.tile_lo + g.begin) * KEYS, tree_words = dry ? 0 : a.tree_words;
+      const int draft0 = dry ? 0 : (g.row_tile * (ROWS2 ? 2 : 1) + (ROWS2 ? wg : 0)) * drafts_tile;
+      const int rows = dry ? ROWS : max(0, min(drafts_tile, min(g.s.n, a.max_nodes) - draft0)) * group;       // of this warpgroup
+      const bool live = quarter * 32 < rows, valid = !dry && lane_row < rows;
+      const int draft = lane_row / group, row_head = dry ? 0 : g.head * group + lane_row - draft * group;
+      const int token = dry ? 0 : g.s.first + (valid ? draft0 + draft : 0);
+      const int* bits = a.tree + (size_t)token * a.tree_words;
+      const int oldest = a.window > 0 && !dry ? max(a.positions[token], held) - a.window + 1 : 0;
+      float m_ref = -INFINITY, l_sum = 0.f;
+      const int t_first = turn0 + ((turn0 ^ wg) & 1);      // this warpgroup's first turn
+      for (int t = t_first; t < turn0 + turns && ok; t += 2) {
+        const int tile = ROWS2 ? (t - turn0) >> 1 : t - turn0, key0 = first_key + tile * KEYS, j = t >> 1;
+        // the keys that this row sees, while the scores are made
+        const bool masked = (key0 + KEYS > held || key0 < key_lo || a.window > 0) && (!dry || quarter == 0);
+        uint32_t words[4];
+        if (masked) {
 #pragma unroll
-          for (int piece = 0; piece < 8; ++piece)
+          for (int i = 0; i < 4; ++i) words[i] = seen_word(tree_words, bits, key0 + 32 * i, held, ctx, oldest);
+        }
+        // a warp without rows waits as well: the turn before has been handed on by all four by then
+        ok = dry || mbar_wait(&s_full[wg], j & 1) || ran_out(6);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        fence_after_sync();
+        if (live) {
+          float s[KEYS];
+          float top = -INFINITY;
+          tmem_ld128(my_s, s);
+          if (!dry || quarter == 0) {
+            if (a.cap_in != 0.f) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint4 x = *reinterpret_cast<const uint4*>(v_row + half * HALF_BYTES + piece * 16);
+              for (int e = 0; e < KEYS; ++e) s[e] = a.cap_out - __fdividef(2.f * a.cap_out, 1.f + fast_exp2(s[e] * a.cap_in));
+            }
+            if (masked) {
+#pragma unroll
+              for (int e = 0; e < KEYS; ++e)
+                if (!(words[e >> 5] >> (e & 31) & 1u)) s[e] = -INFINITY;
+            }
+            top = row_max(s);
+          }
+          const bool grow = (top - m_ref) * c > GROWTH || (m_ref == -INFINITY && top > -INFINITY);
+          const bool any_grow = __any_sync(0xffffffffu, grow);
+          const float m_new = grow ? top : m_ref;
+          const float factor = m_ref == -INFINITY ? 0.f : fast_exp2((m_ref - m_new) * c);
+          const float neg_base = m_new == -INFINITY ? 0.f : -m_new * c;
+          m_ref = m_new;
+          if (!dry || quarter == 1) {
+            float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int part = 0; part < 4; ++part) {
+              uint32_t w[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float x = fast_exp2(fmaf(s[part * 32 + 2 * e], c, neg_base)), y = fast_exp2(fmaf(s[part * 32 + 2 * e + 1], c, neg_base));
+                sums[e & 3] += x + y;
+                w[e] = pack_bf16(x, y);
+              }
+              if (!dry) tmem_st16(my_s + part * 16, w);
+            }
+            l_sum = l_sum * factor + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+          }
+          if ((any_grow && t > t_first) || (dry && quarter == 2)) {
+            ok = dry || mbar_wait(&pv_done[wg], (j - 1) & 1) || ran_out(7);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            fence_after_sync();
+#pragma unroll 2
+            for (int ch = 0; ch < DIM / 16; ++ch) {
+              float v[16];
+              uint32_t r[16];
+              tmem_ld16(my_o + ch * 16, v);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(v[e] * factor);
+              tmem_st16(my_o + ch * 16, r);
+            }
+          }
+          tmem_wait_st();
+        }
+        if (key0 + KEYS > held && (!dry || quarter == 2)) {
+          // a draft's value row that is not finite is zeroed: 0 x NaN would be NaN for rows that do not see it. V's place in the ring's order:
+          // K0 K1 V0 K2 V1 ..., or K0 V0 K1 V1 ... with ROWS2
+          const int at = ROWS2 ? t | 1 : min(n_tiles, 2) + t + min(t, max(0, n_tiles - 2)), stage = at % STAGES;
+          ok = dry || mbar_wait(&full[stage], (at / STAGES) & 1) || ran_out(4);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          const int key = key0 + lane_row;
+          uint8_t* v_row = ring + stage * TILE_BYTES + lane_row * 128;
+          if (key >= held && key < ctx) {
+            bool bad = false;
+#pragma unroll 4
+            for (int piece = 0; piece < 16; ++piece) {
+              const uint4 x = *reinterpret_cast<const uint4*>(v_row + (piece >> 3) * HALF_BYTES + (piece & 7) * 16);
               bad |= not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w);
             }
-          if (bad) { zero = true; flag[1] = 1; }
+            if (bad && !dry) {
+              flag[1] = 1;
+#pragma unroll 1
+              for (int piece = 0; piece < 16; ++piece) *reinterpret_cast<uint4*>(v_row + (piece >> 3) * HALF_BYTES + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_async_smem();
         }
-        if (zero) {
-#pragma unroll
-          for (int piece = 0; piece < 8; ++piece)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) *reinterpret_cast<uint4*>(v_row + half * HALF_BYTES + piece * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_async_smem();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0 && !dry) mbar_arrive(&p_full[wg]);
       }
+      if (!ok) break;
+      if (dry && quarter != 3) continue;
+
+      // ---- the segment's result: with turns of both warpgroups each takes half the channels of both accumulators
+      float2* pair = stats + (k & 1) * 2 * ROWS;
+      const bool both = !ROWS2 && turns > 1;
+      if (!dry) {
+        pair[wg * ROWS + lane_row] = make_float2(m_ref, l_sum);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(stats_full);
+        ok = (mbar_wait(stats_full, k & 1) || ran_out(7)) && (mbar_wait(o_full, k & 1) || ran_out(8));
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      }
+      fence_after_sync();
+      // relative to one maximum: this warpgroup's accumulator by `mine`, the other's by `other`
+      float mine = 1.f, other = 0.f;
+      if (!ROWS2) {
+        const float2 ml = pair[(wg ^ 1) * ROWS + lane_row];
+        const float top = fmaxf(m_ref, ml.x), base = top == -INFINITY ? 0.f : top;
+        mine = fast_exp2((m_ref - base) * c);
+        other = fast_exp2((ml.x - base) * c);
+        l_sum = l_sum * mine + ml.y * other;
+        m_ref = top;
+      }
+      const bool split = g.count < g.s.tiles;
+      const float m_log2 = m_ref * c;
+      if (live) {
+        float inv = 1.f;
+        if (!split) {
+          float total = l_sum, factor = 1.f;
+          if (a.sinks && valid) {
+            const float sink = a.sinks[row_head] * LOG2E, top = fmaxf(m_log2, sink);
+            factor = fast_exp2(m_log2 - top);
+            total = total * factor + fast_exp2(sink - top);
+          }
+          inv = total == 0.f ? 0.f : __fdividef(factor, total);
+        }
+        // the channels: all, or half with the other warpgroup taking the rest; `first_acc`: the accumulator of the segment's first turn
+        const uint32_t first_acc = tmem_o + (ROWS2 ? wg : turn0 & 1) * 128 + lane_addr, second_acc = tmem_o + (~turn0 & 1) * 128 + lane_addr;
+        const float by_first = (ROWS2 || (turn0 & 1) == wg ? mine : other) * inv, by_second = ((turn0 & 1) == wg ? other : mine) * inv;
+        const long at = ((long)2 * blockIdx.x + (g.begin == 0 ? 1 : 0)) * (ROWS2 ? 2 * ROWS : ROWS) + (ROWS2 ? wg * ROWS : 0) + lane_row;
+        float* part = a.partials + at * DIM;
+        bf16* out = (bf16*)a.out + ((size_t)token * a.q_heads + row_head) * DIM;
+        const int ch_begin = ROWS2 ? 0 : wg * 4, ch_end = ROWS2 ? 8 : ch_begin + 4;
+        const bool bad = flag[1];
+        auto store = [&](int ch, const float (&v)[16]) {
+          uint32_t w[8];
+          if (split) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[e]);
+            store32(part + ch * 16, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[8 + e]);
+            store32(part + ch * 16 + 8, w);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+            store32(out + ch * 16, w);
+          }
+        };
+        auto read = [&](int ch, float (&v)[16]) {
+          if (both) {
+            float x[16];
+            tmem_ld16_two(first_acc + ch * 16, second_acc + ch * 16, v, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = v[e] * by_first + x[e] * by_second;
+          } else {
+            tmem_ld16(first_acc + ch * 16, v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] *= by_first;
+          }
+        };
+        if (!__any_sync(0xffffffffu, bad)) {
+#pragma unroll 2
+          for (int ch = ch_begin; ch < ch_end; ++ch) {
+            float v[16];
+            read(ch, v);
+            if (valid) store(ch, v);
+          }
+        } else {
+#pragma unroll 1
+          for (int ch = ch_begin; ch < ch_end; ++ch) {
+            float v[16];
+            __syncwarp();                                  // lanes with drafts to add come back together
+            read(ch, v);
+            if (!valid) continue;
+            for (int key = max(first_key, held); key < min(ctx, first_key + g.count * KEYS); ++key) {
+              if (!sees(a, bits, key, held, oldest)) continue;
+              const long from = key_row(a, a.block_table + (size_t)g.seq * a.table_width, key, g.head);
+              if (from < 0) continue;
+              const float w = inv * zeroed_weight((const bf16*)a.q + ((size_t)token * a.q_heads + row_head) * DIM, (const bf16*)a.k_pool, (const bf16*)a.v_pool,
+                                                  from, a.cap_in, a.cap_out, c, m_ref == -INFINITY ? 0.f : m_log2);
+              if (w == 0.f) continue;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) v[e] += w * __bfloat162float(((const bf16*)a.v_pool)[from * DIM + ch * 16 + e]);
+            }
+            store(ch, v);
+          }
+        }
+        if (valid && split && (ROWS2 || wg == 0)) *reinterpret_cast<float2*>(a.partials + a.partial_stats + at * 2) = make_float2(m_log2, l_sum);
+      }
+      if (dry) continue;
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[wg]);
+      if (lane == 0) mbar_arrive(o_empty);
+      turn0 += turns;
     }
-    if (n_tiles > 0 && ok) {
-      ok = mbar_wait(all_done, 0) || ran_out(8);
-      ok = __all_sync(0xffffffffu, ok);
-      fence_after_sync();
-    }
-  }
-
-  // ---------------- the second warpgroup hands its accumulator over
-  float* joined = reinterpret_cast<float*>(ring);
-  float2* joined_stats = reinterpret_cast<float2*>(ring + ROWS * JOIN_STRIDE * 4);
-  const bool softmax_warp = warp >= 2 && quarter * 32 < u.rows;
-  if (softmax_warp && wg == 1 && n_tiles > 1 && ok) {
-#pragma unroll
-    for (int ch = 0; ch < DIM / 16; ++ch) {
-      float v[16];
-      tmem_ld16(tmem_o + 128 + lane_addr + ch * 16, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<float4*>(joined + row_local * JOIN_STRIDE + ch * 16 + e * 4) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-    }
-    joined_stats[row_local] = make_float2(m_ref, l_sum);
-  }
-  __syncthreads();
-  if (softmax_warp && wg == 0 && ok && !flag[0]) {
-    const float c = a.scale_log2;
-    float mine = 1.f, other = 0.f;
-    if (n_tiles > 1) {
-      const float2 ml = joined_stats[row_local];
-      const float top = fmaxf(m_ref, ml.x), base = top == -INFINITY ? 0.f : top;
-      mine = fast_exp2((m_ref - base) * c);
-      other = fast_exp2((ml.x - base) * c);
-      l_sum = l_sum * mine + ml.y * other;
-      m_ref = top;
-    }
-    const bool valid = row_local < u.rows, split = u.chunks > 1, bad = flag[1];
-    const float m_log2 = m_ref * c;
-    float inv = 1.f;
-    if (!split) {
-      float total = l_sum, factor = 1.f;
-      if (a.sinks) {
-        const float sink = a.sinks[u.head * group + row % group] * LOG2E, top = fmaxf(m_log2, sink);
-        factor = fast_exp2(m_log2 - top);
-        total = total * factor + fast_exp2(sink - top);
-      }
-      inv = total == 0.f ? 0.f : factor / total;
-    }
-    const long at = (u.index * gridDim.z + blockIdx.z) * ROWS + row_local;
-    bf16* out = (bf16*)a.out + ((size_t)token * a.q_heads + u.head * group + row % group) * DIM;
-#pragma unroll 1
-    for (int ch = 0; ch < DIM / 16; ++ch) {
-      float v[16];
-      __syncwarp();                                        // lanes without a row, or with drafts to add, come back together
-      if (n_tiles > 0) {
-        tmem_ld16(tmem_o + lane_addr + ch * 16, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = 0.f;
-      }
-      if (!valid) continue;
-      if (n_tiles > 1) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = v[e] * mine + joined[row_local * JOIN_STRIDE + ch * 16 + e] * other;
-      }
-      if (bad) add_not_finite(a, u, table, u.tile_begin * KEYS, min(u.ctx, u.tile_end * KEYS), row, group, oldest, m_ref == -INFINITY ? 0.f : m_log2, ch * 16, v);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] *= inv;
-      if (split) {
-        store_row16(a.partials + at * DIM + ch * 16, v);
-      } else {
-        store_row16(out + ch * 16, v);
-      }
-    }
-    if (valid && split) *reinterpret_cast<float2*>(a.partials + a.partial_stats + at * 2) = make_float2(m_log2, l_sum);
   }
 
   // ---------------- teardown
@@ -431,29 +692,79 @@ __global__ void __launch_bounds__(THREADS, 1) attention_tree_tcgen05_kernel(cons
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);     // let copies in flight land
     __syncthreads();
   }
-  if (warp == 1) {
+  if (warp == LOADERS) {
     fence_after_sync();
     tmem_dealloc(tmem_s, 512);
   }
 }
 
-// A pool [pages][heads][page_tokens][128] of bfloat16: copies of one page's tokens of one head, 64 channels.
-static bool pool_map(CUtensorMap* map, const void* pool, long pages, int heads, int page_tokens) {
+// The parts of a row whose keys lie in several blocks' shares, in the order of the keys; one warp a row.
+constexpr int JOIN_THREADS = 128;
+template <bool ROWS2>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const TreeArgs a, int blocks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int seq = blockIdx.y, head = blockIdx.x, group = a.group, drafts_tile = a.tile_drafts;
+  const int row = blockIdx.z * (JOIN_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;      // draft * group + head of the group
+  const Sequence s = find_sequence<ROWS2>(a, a.cu_q[seq], a.cu_q[seq + 1], a.ctx_len[seq]);
+  const int draft = row / group;
+  if (draft >= min(s.n, a.max_nodes)) return;
+  const int tile_drafts = drafts_tile * (ROWS2 ? 2 : 1), row_tile = draft / tile_drafts, in_tile = draft - row_tile * tile_drafts;
+  const int total = a.list[0], at = a.list[1 + seq] + (head * s.row_tiles + row_tile) * s.tiles;
+  const int shares = min(blocks, total), b0 = share_of(total, at, shares), b1 = share_of(total, at + s.tiles - 1, shares);
+  if (b0 == b1) return;
+  const int slot_rows = ROWS2 ? 2 * ROWS : ROWS, row_head = head * group + row - draft * group;
+  const int local = (in_tile / drafts_tile) * ROWS + (in_tile % drafts_tile) * group + row - draft * group;
+  auto place = [&](int b) { return ((long)2 * b + (b == b0 ? 1 : 0)) * slot_rows + local; };
+  const float2* stats = reinterpret_cast<const float2*>(a.partials + a.partial_stats);
+  const float sink = a.sinks ? a.sinks[row_head] * LOG2E : -INFINITY;
+  float top = sink;
+  for (int b = b0 + lane; b <= b1; b += 32) top = fmaxf(top, stats[place(b)].x);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float total_weight = a.sinks ? exp2f(sink - base) : 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int b = b0; b <= b1; ++b) {
+    const float2 ml = stats[place(b)];
+    const float4 v = *reinterpret_cast<const float4*>(a.partials + place(b) * DIM + 4 * lane);
+    const float w = exp2f(ml.x - base);
+    total_weight += w * ml.y;
+    if (w != 0.f) { sum.x += w * v.x; sum.y += w * v.y; sum.z += w * v.z; sum.w += w * v.w; }
+  }
+  const float inv = total_weight == 0.f ? 0.f : 1.f / total_weight;
+  bf16* to = (bf16*)a.out + ((size_t)(s.first + draft) * a.q_heads + row_head) * DIM + 4 * lane;
+  *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+}
+
+// The queries [tokens][q_heads][128]: 128 / group drafts with their heads of a group, 64 channels.
+static bool query_map(CUtensorMap* map, const void* q, long tokens, int q_heads, int group) {
   auto encode = encode_fn();
   if (!encode) return false;
-  cuuint64_t dims[4] = {DIM, (cuuint64_t)page_tokens, (cuuint64_t)heads, (cuuint64_t)pages};
-  cuuint64_t strides[3] = {DIM * 2, (cuuint64_t)page_tokens * DIM * 2, (cuuint64_t)heads * page_tokens * DIM * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)page_tokens, 1, 1}, elem[4] = {1, 1, 1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  cuuint64_t dims[3] = {DIM, (cuuint64_t)q_heads, (cuuint64_t)tokens}, strides[2] = {DIM * 2, (cuuint64_t)q_heads * DIM * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(ROWS / group)}, elem[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static int launch(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
-  CUtensorMap k_map, v_map;
-  if (!pool_map(&k_map, a.k_pool, a.n_pages, a.kv_heads, a.page_tokens) || !pool_map(&v_map, a.v_pool, a.n_pages, a.kv_heads, a.page_tokens)) return LB_ERR_SIZE;
+// scratch of `blocks` blocks, in floats: two places each of the partial outputs, their maxima and sums; the list
+static long scratch_floats(int blocks, bool rows2, int n_seqs) { return 2L * blocks * (rows2 ? 2 * ROWS : ROWS) * (DIM + 2) + n_seqs + 1; }
+
+template <bool ROWS2>
+int launch(TreeArgs a, int blocks, cudaStream_t stream) {
+  CUtensorMap q_map;
+  const int group = a.q_heads / a.kv_heads;
+  if (!query_map(&q_map, a.q, a.tokens, a.q_heads, group)) return LB_ERR_SIZE;
   static LbPerDeviceOnce once;
-  if (!once.run(LB_ALLOW_SMEM(attention_tree_tcgen05_kernel, SMEM_BYTES))) return lb_last_error();
-  return lb_launch(attention_tree_tcgen05_kernel, grid, THREADS, SMEM_BYTES, stream, k_map, v_map, a);
+  if (!once.run(LB_ALLOW_SMEM(attention_tree_tcgen05_kernel<ROWS2>, SMEM_BYTES))) return lb_last_error();
+  const long slots = 2L * blocks * (ROWS2 ? 2 * ROWS : ROWS);
+  a.partial_stats = slots * DIM;
+  a.list = reinterpret_cast<int*>(a.partials + slots * (DIM + 2));
+  a.group = group; a.tile_drafts = ROWS / group;
+  int code = lb_launch(attention_tree_tcgen05_kernel<ROWS2>, blocks, THREADS, SMEM_BYTES, stream, q_map, a);
+  if (code || blocks == 1) return code;
+  const int rows = a.max_nodes * group;
+  return lb_launch(join_kernel<ROWS2>, dim3(a.kv_heads, a.n_seqs, (rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32)), JOIN_THREADS, 0, stream, a, blocks);
 }
 }  // namespace wide
 }  // namespace

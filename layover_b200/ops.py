@@ -1285,26 +1285,37 @@ def attention_f32(q, cache, out, block_table, batch, q_heads, kv_heads, dim, pag
 _TREE_SCRATCH_FLOATS = 64 << 20          # the most that the chunks' results may take (256 MiB)
 
 
-def attention_tree_on_tcgen05(rows: int, dim: int, page_tokens: int, dtype: torch.dtype) -> bool:
+def attention_tree_on_tcgen05(rows: int, group: int, dim: int, page_tokens: int, dtype: torch.dtype) -> bool:
     """Whether `attention_tree` takes these rows (drafts times heads of a group) to its tcgen05 kernel."""
-    return dtype == torch.bfloat16 and dim == 128 and page_tokens % 8 == 0 and 128 % page_tokens == 0 and rows > 16
+    return dtype == torch.bfloat16 and dim == 128 and page_tokens % 8 == 0 and 128 % page_tokens == 0 and 16 < rows and group <= 128
 
 
 @functools.lru_cache(maxsize=1024)      # of the sizes alone, asked for by every layer of a step
-def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, dim: int, page_tokens: int, dtype: torch.dtype,
-              sms: int) -> tuple[int, int, int, int]:
-    """(rows of a block, row tiles of a sequence, chunks, key tiles of a chunk) for `attention_tree`."""
+def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, dim: int, sms: int) -> tuple[int, int, int, int]:
+    """(rows of a block, row tiles of a sequence, chunks, key tiles of a chunk) for the FFMA and mma.sync kernels of `attention_tree`: row
+    tiles no larger than the rows ask for, and as many chunks of the keys as give every SM about four blocks."""
     rows = max_nodes * (q_heads // kv_heads)
-    wide = attention_tree_on_tcgen05(rows, dim, page_tokens, dtype)
-    tile_rows, tile_keys, blocks = (128, 128, sms) if wide else (16 if rows <= 16 else 32 if rows <= 32 else 64, 64, 4 * sms)
+    tile_rows = 16 if rows <= 16 else 32 if rows <= 32 else 64
     row_tiles = -(-rows // tile_rows)
     keys = min(max_ctx, max_nodes + window) if window else max_ctx
-    tiles = -(-keys // tile_keys) + (1 if window else 0)
+    tiles = -(-keys // 64) + (1 if window else 0)
     units = n_seqs * kv_heads * row_tiles
     most = max(1, _TREE_SCRATCH_FLOATS // (units * tile_rows * (dim + 2)))
-    chunks = max(1, min(-(-blocks // units), tiles // 2, most, 65535))
+    chunks = max(1, min(-(-4 * sms // units), tiles // 2, most, 65535))
     chunk_tiles = -(-tiles // chunks)
     return tile_rows, row_tiles, -(-tiles // chunk_tiles), chunk_tiles
+
+
+@functools.lru_cache(maxsize=1024)
+def tree_share(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, sms: int) -> tuple[int, bool, int]:
+    """(blocks, whether a row tile is two tiles of 128 rows, floats of scratch) for the tcgen05 kernel of `attention_tree`: a block an SM, or
+    one for each tile of 128 keys where there are fewer."""
+    drafts = 128 // (q_heads // kv_heads)
+    rows2 = max_nodes > drafts
+    keys = min(max_ctx, max_nodes + window) if window else max_ctx
+    tiles = (-(-keys // 128) + (1 if window else 0)) * n_seqs * kv_heads * -(-max_nodes // (2 * drafts if rows2 else drafts))
+    blocks = min(sms, tiles)
+    return blocks, rows2, 2 * blocks * (256 if rows2 else 128) * (128 + 2) + n_seqs + 1
 
 
 def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
@@ -1355,21 +1366,30 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     _here("attention_tree", q, k_pool, v_pool, out, block_table, cu_q, ctx_len, positions if window else None, tree, sinks)
     if tokens == 0 or n_seqs == 0:
         return out
-    tile_rows, row_tiles, chunks, chunk_tiles = tree_plan(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, dim, page_tokens, q.dtype,
-                                                           sm_count(q.device))
+    global LAUNCHES
+    group, sms, given_positions = q_heads // kv_heads, sm_count(q.device), _ptr(positions if window else None)
+    if attention_tree_on_tcgen05(max_nodes * group, group, dim, page_tokens, q.dtype):
+        blocks, rows2, floats = tree_share(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, sms)
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)          # of this call alone, on its own stream
+        fn = _FUNCTIONS.get("lb_attention_tree_tcgen05") or _fn("attention_tree", "lb_attention_tree_tcgen05",
+                 [c_void_p] * 5 + [c_int, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float, c_int, c_void_p, c_float] + [c_int] * 3 + [c_void_p, c_long, c_void_p])
+        _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(block_table), block_table.shape[1], k_pool.shape[0], _ptr(cu_q), _ptr(ctx_len),
+                  given_positions, _ptr(tree), tree.shape[1], tokens, int(n_seqs), q_heads, kv_heads, dim, page_tokens, float(scale), int(window),
+                  _ptr(sinks), float(softcap), int(max_nodes), blocks, int(rows2), _ptr(scratch), floats, _stream()), "attention_tree")
+        LAUNCHES += blocks > 1      # the shares' results are joined by a kernel of their own
+        return out
+    tile_rows, row_tiles, chunks, chunk_tiles = tree_plan(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, dim, sms)
     partials = None
     if chunks > 1:          # of this call alone, on its own stream
         partials = torch.empty(n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2), dtype=torch.float32, device=q.device)
     fn = _FUNCTIONS.get("lb_attention_tree") or _fn("attention_tree", "lb_attention_tree",
-             [c_int] + [c_void_p] * 5 + [c_int, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float, c_int, c_void_p, c_float] + [c_int] * 4
+             [c_int] + [c_void_p] * 5 + [c_int, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float, c_int, c_void_p, c_float] + [c_int] * 5
              + [c_void_p, c_long, c_void_p])
     _check(fn(dtype_code(q.dtype), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(block_table), block_table.shape[1], k_pool.shape[0],
-              _ptr(cu_q), _ptr(ctx_len), _ptr(positions if window else None), _ptr(tree), tree.shape[1], tokens, int(n_seqs), q_heads, kv_heads,
-              dim, page_tokens, float(scale), int(window), _ptr(sinks), float(softcap), tile_rows, row_tiles, chunks, chunk_tiles, _ptr(partials),
+              _ptr(cu_q), _ptr(ctx_len), given_positions, _ptr(tree), tree.shape[1], tokens, int(n_seqs), q_heads, kv_heads, dim, page_tokens,
+              float(scale), int(window), _ptr(sinks), float(softcap), int(max_nodes), tile_rows, row_tiles, chunks, chunk_tiles, _ptr(partials),
               partials.numel() if partials is not None else 0, _stream()), "attention_tree")
-    if chunks > 1:
-        global LAUNCHES
-        LAUNCHES += 1          # the chunks' results are joined by a kernel of their own
+    LAUNCHES += chunks > 1      # the chunks' results are joined by a kernel of their own
     return out
 
 

@@ -164,6 +164,14 @@ def test_tree_attention_splits_long_contexts(context, dtype):
     Trees([(context, 6), (5, 6), (context // 3, 2)], 8, 2, 128, dtype=dtype, seed=context).fill().check()
 
 
+@pytest.mark.parametrize("nodes", [1, 9, 33])
+@pytest.mark.parametrize("window", [0, 150])
+def test_tree_attention_of_more_sequences_than_blocks(nodes, window):
+    """Shares of several whole row tiles and of ends of two, requests without drafts among them; keys of one tile and of some."""
+    lengths = [((i * 37) % 400, (i * 5) % (nodes + 1)) for i in range(70)] + [(2500, nodes)]
+    Trees(lengths, 16, 4, 128, window=window, seed=nodes).fill().check()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("window", [1, 3, 64, 100, 5000])
 def test_tree_attention_behind_a_window(window, dtype):

@@ -581,7 +581,7 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
   if ((uintptr_t)partials & 15) return LB_ERR_ALIGN;
   TreeArgs a{q, k_pool, v_pool, out, block_table, table_width, n_pages, cu_q, ctx_len, positions, tree, tree_words, tokens, q_heads, kv_heads, dim,
              page_tokens, scale * LOG2E, 0.f, 0.f, window, sinks, row_tiles, chunk_tiles, chunks > 1 ? partials : nullptr, partial_rows * dim, n_seqs,
-             max_nodes, 0, 0, nullptr};
+             max_nodes, 0, 0, nullptr, nullptr};
   if (softcap > 0.f) { a.cap_in = 2.f * LOG2E * scale / softcap; a.cap_out = softcap / scale; }
   const dim3 grid(kv_heads, n_seqs * row_tiles, chunks);
   int code;
@@ -600,8 +600,8 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
 }
 
 // The tcgen05 kernel: bfloat16, heads of 128 channels, at most 128 query heads a key/value head, pages of 8 .. 128 tokens that divide 128. `blocks` blocks
-// share the keys; `rows2`: tiles of twice 128 / group drafts. `scratch` holds lb_attention_tree_scratch(blocks, rows2, n_seqs) floats.
-LB_EXPORT long lb_attention_tree_scratch(int blocks, int rows2, int n_seqs) { return wide::scratch_floats(blocks, rows2 != 0, n_seqs); }
+// share the keys; `rows2`: tiles of twice 128 / group drafts. `scratch` holds lb_attention_tree_scratch(blocks, rows2) floats.
+LB_EXPORT long lb_attention_tree_scratch(int blocks, int rows2) { return wide::scratch_floats(blocks, rows2 != 0); }
 LB_EXPORT int lb_attention_tree_tcgen05(const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
                                         int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words,
                                         int tokens, int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, float scale, int window,
@@ -612,11 +612,11 @@ LB_EXPORT int lb_attention_tree_tcgen05(const void* q, const void* k_pool, const
                                  window, softcap, max_nodes);
   if (refused) return refused;
   if (dim != 128 || q_heads / kv_heads > 128 || page_tokens % 8 || 128 % page_tokens || blocks <= 0 || blocks > 1024 || !scratch ||
-      floats < wide::scratch_floats(blocks, rows2 != 0, n_seqs))
+      floats < wide::scratch_floats(blocks, rows2 != 0))
     return LB_ERR_SIZE;
   if (((uintptr_t)scratch | (uintptr_t)out) & 31) return LB_ERR_ALIGN;
   TreeArgs a{q, k_pool, v_pool, out, block_table, table_width, n_pages, cu_q, ctx_len, positions, tree, tree_words, tokens, q_heads, kv_heads, dim,
-             page_tokens, scale * LOG2E, 0.f, 0.f, window, sinks, 0, 0, scratch, 0, n_seqs, max_nodes, 0, 0, nullptr};
+             page_tokens, scale * LOG2E, 0.f, 0.f, window, sinks, 0, 0, scratch, 0, n_seqs, max_nodes, 0, 0, nullptr, nullptr};
   if (softcap > 0.f) { a.cap_in = 2.f * LOG2E * scale / softcap; a.cap_out = softcap / scale; }
   const int code = rows2 ? wide::launch<true>(a, blocks, stream) : wide::launch<false>(a, blocks, stream);
   return code ? code : lb_last_error();

@@ -7,6 +7,9 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// A row tile whose keys lie in the shares of blocks `from` to `upto`; drafts 0: none.
+struct Border { int from, upto, seq, head, token, draft, drafts, unused; };
+
 struct TreeArgs {
   const void *q, *k_pool, *v_pool;
   void* out;
@@ -24,7 +27,8 @@ struct TreeArgs {
   long partial_stats;           // where the second part begins, in floats
   int n_seqs, max_nodes;
   int group, tile_drafts;       // query heads of a key/value head; drafts of a tile of 128 rows (the tcgen05 kernel's)
-  int* list;                    // the tcgen05 kernel's tiles, and how many lie before each sequence's
+  Border* borders;       // the tcgen05 kernel's, for the kernel that joins: per block
+  int* not_finite;              // whether a block met an output that is not finite
 };
 
 // What a block works on: its rows, and its share of the keys.
@@ -58,15 +62,14 @@ __device__ __forceinline__ Unit find_unit(const TreeArgs& a, int tile_rows, int 
 
 // Bit i: whether a row sees key key0 + i, 32 of them: `bits` are its drafts, `oldest` the first held key it sees.
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-__device__ __forceinline__ uint32_t seen_word(int tree_words, const int* bits, int key0, int held, int ctx, int oldest) {
-  const int j = key0 - held, w = j >> 5, shift = j & 31;          // the first key's draft; negative for held ones
-  uint32_t drafts = 0;
-  if (j > -32) {
-    const uint32_t lo = w >= 0 && w < tree_words ? (uint32_t)bits[w] : 0u, hi = w + 1 >= 0 && w + 1 < tree_words ? (uint32_t)bits[w + 1] : 0u;
-    drafts = __funnelshift_r(lo, hi, shift);
-  }
-  const uint32_t kept = below(-j);
+__device__ __forceinline__ uint32_t seen_word(uint32_t drafts, int key0, int held, int ctx, int oldest) {      // `drafts`: the tree's bits from key0 on
+  const uint32_t kept = below(held - key0);
   return ((drafts & ~kept) | (kept & ~below(oldest - key0))) & below(ctx - key0);
+}
+__device__ __forceinline__ uint32_t seen_word(int tree_words, const int* bits, int key0, int held, int ctx, int oldest) {
+  const int j = key0 - held, w = j >> 5;                  // the first key's draft; negative for held ones
+  const uint32_t lo = w >= 0 && w < tree_words ? (uint32_t)bits[w] : 0u, hi = w + 1 >= 0 && w + 1 < tree_words ? (uint32_t)bits[w + 1] : 0u;
+  return seen_word(__funnelshift_r(lo, hi, j & 31), key0, held, ctx, oldest);
 }
 
 // Where key `key` of a sequence lies in its pool, in rows of one head's channels; -1 for a page that is not there.

@@ -4,21 +4,23 @@
 // an equal, contiguous share of the list: a few segments, each a row tile and a range of its keys. Blocks stay for the whole
 // launch, one an SM, so the loads of a segment run under the arithmetic and the stores of the one before. A row tile whose keys
 // lie in several blocks' shares leaves maxima, sums and unnormalised outputs in scratch memory, two places a block (its first and its last
-// segment), for `join_kernel`.
+// segment), for
+// `join_kernel`.
 //
 // A row tile holds 128 / group drafts with all their heads of the group, or, with ROWS2, twice as many. Two warpgroups of softmax
 // have scores and an output accumulator of their own in tensor memory: they take the key tiles in turn, or, with ROWS2, a half of
 // the rows each. Either way the products go through "turns" 0, 1, 2, ... of alternate warpgroups: O += P(t) V, then S(t + 2) = Q K^T,
-// so that one warpgroup's softmax runs under the other's products. K and V come through one ring in the order in which the products
-// use them, 16 bytes a thread (cp.async of two warps; a TMA copy of a page of 16 tokens takes 70 cycles whoever issues it, 1,150 for
+// so that one warpgroup's softmax runs under the other's products. K and V come through a ring each,
+// 16 bytes a thread (cp.async, two warps for either; a TMA copy of a page of 16 tokens takes 70 cycles whoever issues it, 1,150 for
 // the 32 KB of a tile with pages of 16, and 1,430 are what a tile may take at the memory's rate). The weights overwrite their scores in tensor
 // memory and are the A operand of the second product.
 //
 // Code that runs first is slow: a turn of softmax takes four times as long until its instructions have been fetched. So the warps run
 // through parts of it each, on nothing, while the first loads are under way.
 //
-// Rows that the tree does not have cost nothing but the tensor cores' time: their warps only hand tiles on. What a draft's values
-// hold that is not finite is zeroed in the tile and added at the end to the rows that see it.
+// Rows that the tree does not have cost nothing but the tensor cores' time: their warps only hand tiles on. A draft's values may hold what
+// is not finite, and 0 x NaN is NaN also for rows that do not see the draft: a block whose outputs are not all finite says so, and `join_kernel`
+// makes its rows once more, key by key.
 #pragma once
 #include <math.h>
 
@@ -34,14 +36,13 @@ namespace wide {
 constexpr int ROWS = 128, KEYS = 128, DIM = 128;
 constexpr int HALF_BYTES = 128 * 128;           // 64 channels of 128 rows
 constexpr int TILE_BYTES = 2 * HALF_BYTES;
-constexpr int STAGES = 4;
-constexpr int LOADERS = 2;                      // warps that load K and V, each its rows of a tile
-constexpr int LOADER_EIGHTS = KEYS / LOADERS / 8;      // those rows, in eights
-constexpr int FIRST_SOFTMAX = 4;                // then one that issues the products (and one that does nothing), then two warpgroups of softmax
+constexpr int STAGES = 2;                       // tiles of either ring
+constexpr int LOADERS = 4;                      // warps that load: two K, two V, each 64 rows of a tile
+constexpr int FIRST_SOFTMAX = 8;                // then one that issues the products (and three that do nothing), then two warpgroups of softmax
 constexpr int THREADS = 32 * (FIRST_SOFTMAX + 8);
-constexpr int FEW_REGS = 88, MANY_REGS = 208;   // of a thread of the first four warps and of the others: 128 * 88 + 256 * 208 = 384 * 168, the launch's
+constexpr int FEW_REGS = 72, MANY_REGS = 184;   // of a thread of the first eight warps and of the others: 256 * (72 + 184) = 512 * 128, the launch's
 constexpr int SEQ_CACHE = 512;                  // sequences whose lengths are kept there
-constexpr int SMEM_BYTES = (2 + STAGES) * TILE_BYTES + 1024 + 512 + 2 * 2 * ROWS * 8 + SEQ_CACHE * 16;
+constexpr int SMEM_BYTES = (2 + 2 * STAGES) * TILE_BYTES + 1024 + 512 + 2 * 2 * ROWS * 8 + SEQ_CACHE * 16;
 constexpr float GROWTH = 8.0f;                  // the maximum that weights are relative to may lag by this, in log2 units
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -98,6 +99,16 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {   
 #pragma unroll
   for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
@@ -136,7 +147,7 @@ __device__ __forceinline__ Sequence find_sequence(const TreeArgs& a, int first, 
   s.held = s.ctx - s.n;
   s.key_lo = a.window > 0 ? max(0, s.held - a.window + 1) : 0;
   const int drafts = a.tile_drafts * (ROWS2 ? 2 : 1);
-  s.row_tiles = s.n <= 0 ? 0 : (min(s.n, a.max_nodes) + drafts - 1) / drafts;
+  s.row_tiles = s.n <= 0 ? 0 : ROWS2 ? (min(s.n, a.max_nodes) + drafts - 1) / drafts : 1;      // one tile holds all drafts, but for ROWS2
   s.tile_lo = s.key_lo / KEYS;
   s.tiles = max(1, (s.ctx + KEYS - 1) / KEYS - s.tile_lo);
   return s;
@@ -182,27 +193,16 @@ struct Walk {
   }
 };
 
-// The weight of a draft whose value row was zeroed, for a row that sees it; 0 for any other: from the tensors, which is seldom.
-// `at`: the draft's row in the pools.
-__device__ __noinline__ float zeroed_weight(const bf16* q, const bf16* k_pool, const bf16* v_pool, long at, float cap_in, float cap_out, float scale_log2, float base) {
-  bool bad = false;
-  for (int c = 0; c < DIM; c += 2) bad |= not_finite(*reinterpret_cast<const uint32_t*>(v_pool + at * DIM + c));
-  if (!bad) return 0.f;
-  float s = 0.f;
-  for (int c = 0; c < DIM; ++c) s += __bfloat162float(q[c]) * __bfloat162float(k_pool[at * DIM + c]);
-  if (cap_in != 0.f) s = cap_out - __fdividef(2.f * cap_out, 1.f + fast_exp2(s * cap_in));
-  return fast_exp2(fmaf(s, scale_log2, -base));
-}
 template <bool ROWS2>
 __global__ void __launch_bounds__(THREADS, 1)
-attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const TreeArgs a) {
+attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ TreeArgs a) {
   extern __shared__ uint8_t raw_smem[];
   uint8_t* q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);      // two tiles: of two segments, or of two halves
   uint8_t* ring = q_s + 2 * TILE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + STAGES * TILE_BYTES);
-  uint64_t* full = bars;              // [STAGES]
-  uint64_t* empty = full + STAGES;    // [STAGES]
-  uint64_t* q_full = empty + STAGES;  // [2] a segment's queries have come (ROWS2: [0] alone)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + 2 * STAGES * TILE_BYTES);
+  uint64_t* full = bars;              // [K, V][STAGES]
+  uint64_t* empty = full + 2 * STAGES;    // [K, V][STAGES]
+  uint64_t* q_full = empty + 2 * STAGES;  // [2] a segment's queries have come (ROWS2: [0] alone)
   uint64_t* q_empty = q_full + 2;     // [2] its last scores are made
   uint64_t* s_full = q_empty + 2;     // [2 warpgroups] the scores of a turn are in tensor memory
   uint64_t* p_full = s_full + 2;      // [2] its weights are, and the output is rescaled
@@ -212,14 +212,14 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
   uint64_t* stats_full = o_empty + 1; // its maxima and sums are in shared memory
   uint64_t* started = stats_full + 1; // `start` and `known` are
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(started + 1);
-  volatile uint32_t* flag = tmem_slot + 1;        // [0] a wait ran out, [1] a draft's values were not finite
+  volatile uint32_t* flag = tmem_slot + 1;        // [0] a wait ran out, [1] an output is not finite
   int* start = const_cast<int*>(reinterpret_cast<volatile int*>(flag + 2));      // where the walk begins: sequence, tile of it, tiles
   float2* stats = reinterpret_cast<float2*>(bars + 64);      // [2 segments][2 warpgroups][ROWS]
   int4* known = reinterpret_cast<int4*>(stats + 4 * ROWS);                  // first draft, end, keys and tiles of the first sequences
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 32 * LOADERS) {
-    for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 32 * LOADERS); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2 * STAGES; ++i) { mbar_init(&full[i], 32 * LOADERS / 2); mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
     }
@@ -240,19 +240,30 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
   bool ok = true;
   pdl_launch_dependents();
 
-  if (warp < FIRST_SOFTMAX) give_registers<FEW_REGS>(); else take_registers<MANY_REGS>();
+  if (warp < FIRST_SOFTMAX) {
+  give_registers<FEW_REGS>();
   if (warp < LOADERS) {
     pdl_wait();
     if (warp == 0) {
     // ---------------- the list's length, then the sequence in which this block's share begins
     int total = 0;
-    for (int base = 0; base < a.n_seqs; base += 32) {
+    for (int base = 0; base < a.n_seqs; base += 64) {
+      int first[2], end[2], ctx[2];                        // on their way at once
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int seq = min(base + 32 * i + lane, a.n_seqs - 1);
+        first[i] = a.cu_q[seq]; end[i] = a.cu_q[seq + 1]; ctx[i] = a.ctx_len[seq];
+      }
       int tiles = 0;
-      if (base + lane < a.n_seqs) {
-        const int i = base + lane, first = a.cu_q[i], end = a.cu_q[i + 1], ctx = a.ctx_len[i];
-        const Sequence s = find_sequence<ROWS2>(a, first, end, ctx);
-        tiles = a.kv_heads * s.row_tiles * s.tiles;
-        if (i < SEQ_CACHE) known[i] = make_int4(first, end, ctx, tiles);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int seq = base + 32 * i + lane;
+        if (seq < a.n_seqs) {
+          const Sequence s = find_sequence<ROWS2>(a, first[i], end[i], ctx[i]);
+          const int mine = a.kv_heads * s.row_tiles * s.tiles;
+          if (seq < SEQ_CACHE) known[seq] = make_int4(first[i], end[i], ctx[i], mine);
+          tiles += mine;
+        }
       }
       total += __reduce_add_sync(0xffffffffu, tiles);
     }
@@ -280,107 +291,90 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
       }
       const int mine = before + sum - tiles;
       if (from >= mine && from < mine + tiles) { start[0] = i; start[1] = from - mine; }
-      if (blockIdx.x == 0 && i < a.n_seqs) a.list[1 + i] = mine;       // for the kernel that joins
       before += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (blockIdx.x == 0 && lane == 0) a.list[0] = total;
+    if (lane == 0) start[3] = total;
     __syncwarp();
     if (lane == 0) mbar_arrive(started);
     } else {
       ok = warp_wait(started, 0) || ran_out(1);
     }
-    // ---------------- K and V, and the first of these warps the queries
-    const int n_tiles = ok ? start[2] : 0, row0 = warp * 8 * LOADER_EIGHTS, page_shift = __ffs(a.page_tokens) - 1;      // of a tile, this warp's rows
+    // ---------------- K or V, and the first of these warps the queries
+    const int n_tiles = ok ? start[2] : 0, values = warp >> 1, row0 = (warp & 1) * 64, page_shift = __ffs(a.page_tokens) - 1;
+    const bf16* pool = (const bf16*)(values ? a.v_pool : a.k_pool);
     // a lane copies 16 bytes of rows 2 i + (lane >> 4) of each 8 of this warp's rows; `to` are their places in those 8, swizzled
-    const uint32_t ring_at = smem_u32(ring) + ((lane & 15) >> 3) * HALF_BYTES + row0 * 128;
+    const uint32_t ring_at = smem_u32(ring) + values * STAGES * TILE_BYTES + ((lane & 15) >> 3) * HALF_BYTES + row0 * 128;
     uint32_t to[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) to[i] = (2 * i + (lane >> 4)) * 128 + (((lane & 7) ^ (2 * i + (lane >> 4))) << 4);
     const long lane_from = (lane >> 4) * DIM + (lane & 15) * 8;
-    int taken = 0;
-    // what a tile's copies need: the place in a pool of the first of rows 8 i .. (lane i of LOADER_EIGHTS; -1: its page is not there), its first key,
-    // which keys may be seen, and whether all of them are there
-    struct Tile { int row, key0, key_lo, ctx; bool whole; } tiles[2], coming;
-    auto load = [&](const bf16* pool, const Tile& t) {
-      const int stage = taken % STAGES;
-      if (!warp_wait(&empty[stage], ((taken / STAGES) & 1) ^ 1)) return ran_out(1);
-      if (flag[0]) return false;
-      const uint32_t at = ring_at + stage * TILE_BYTES;
-      if (t.whole) {
-#pragma unroll
-        for (int g = 0; g < LOADER_EIGHTS; ++g) {
-          const bf16* from = pool + (long)__shfl_sync(0xffffffffu, t.row, g) * DIM + lane_from;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) copy16(at + to[i] + g * 1024, from + 2 * i * DIM);
-        }
-      } else {
-#pragma unroll 1
-        for (int g = 0; g < LOADER_EIGHTS; ++g) {
-          const int row = __shfl_sync(0xffffffffu, t.row, g);
-          const bf16* from = pool + (row < 0 ? 0 : (long)row * DIM + lane_from);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = t.key0 + row0 + g * 8 + 2 * i + (lane >> 4);
-            const bool wanted = row >= 0 && key < t.ctx && key >= t.key_lo;
-            copy16_or_zeros(at + to[i] + g * 1024, wanted ? from + 2 * i * DIM : pool, wanted ? 16 : 0);
-          }
-        }
-      }
-      arrive_when_copied(smem_u32(&full[stage]));
-      ++taken;
-      return true;
-    };
-    // K is loaded two turns ahead of V: its walk is `ahead`, its next tile `coming`, whose page is on its way; V's tiles are K's before
+    // Up to four tiles of a segment, whose pages are looked up together, four tiles ahead (a read from memory waits behind all copies
+    // in flight): lane 8 j + i has the page of rows 8 i .. of tile j.
+    struct Group { int page, key0, count, head, key_lo, ctx, draft; } now, soon;
     Walk<ROWS2> ahead;
     ahead.begin_at(a, known, start[0], start[1], n_tiles);
-    int tile = 0, segments = 0, page = -1;
-    auto fetch = [&]() {                                     // the next tile of the walk, if there is one
+    int tile = 0, segments = 0, taken = 0;
+    auto next_group = [&](Group& g) {
+      g.count = 0; g.draft = -1;
       if (tile == ahead.count) {
         if (!ahead.next(a)) return;
         tile = 0;
+        g.draft = ahead.s.first + ahead.row_tile * (ROWS2 ? 2 : 1) * drafts_tile;      // a segment begins: its queries
       }
-      coming.key0 = (ahead.s.tile_lo + ahead.begin + tile) * KEYS; coming.key_lo = ahead.s.key_lo; coming.ctx = ahead.s.ctx;
-      const int key = coming.key0 + row0 + (lane & (LOADER_EIGHTS - 1)) * 8, index = key >> page_shift;
-      page = index < a.table_width && key < ahead.s.ctx ? a.block_table[(size_t)ahead.seq * a.table_width + index] : -1;
+      g.count = min(4, ahead.count - tile); g.head = ahead.head; g.key0 = (ahead.s.tile_lo + ahead.begin + tile) * KEYS;
+      g.key_lo = ahead.s.key_lo; g.ctx = ahead.s.ctx;
+      const int key = g.key0 + (lane >> 3) * KEYS + row0 + (lane & 7) * 8, index = key >> page_shift;
+      g.page = index < a.table_width && key < g.ctx ? a.block_table[(size_t)ahead.seq * a.table_width + index] : -1;
+      tile += g.count;
     };
-    auto load_k = [&](Tile& t) {
-      const bool there = (unsigned)page < (unsigned)a.n_pages;
-      t = coming;
-      t.row = there ? (page * a.kv_heads + ahead.head) * a.page_tokens + ((t.key0 + row0 + (lane & (LOADER_EIGHTS - 1)) * 8) & (a.page_tokens - 1)) : -1;
-      t.whole = __all_sync(0xffffffffu, there) && t.key0 >= t.key_lo && t.key0 + KEYS <= t.ctx;
-      if (tile == 0) {
-        if (warp == 0) {
-          const int buf = ROWS2 ? 0 : segments & 1;
-          if (!warp_wait(&q_empty[buf], ((ROWS2 ? segments : segments >> 1) & 1) ^ 1)) return ran_out(2);
-          const uint32_t bar = smem_u32(&q_full[buf]);
-          expect_bytes(bar, (uint32_t)(drafts_tile * group * 128) * (ROWS2 ? 4 : 2));
-          const int head = warp_uniform(ahead.head * group), draft = warp_uniform(ahead.s.first + ahead.row_tile * (ROWS2 ? 2 : 1) * drafts_tile);
-          for (int part = 0; part < (ROWS2 ? 2 : 1); ++part)
-            for (int h = 0; h < 2; ++h)
-              load_queries(smem_u32(q_s) + (ROWS2 ? part : buf) * TILE_BYTES + h * HALF_BYTES, &q_map, bar, h * 64, head, draft + part * drafts_tile);
-        }
+    next_group(now);
+    while (ok && now.count > 0) {
+      next_group(soon);
+      if (warp == 0 && now.draft >= 0) {
+        const int buf = ROWS2 ? 0 : segments & 1;
+        ok = warp_wait(&q_empty[buf], ((ROWS2 ? segments : segments >> 1) & 1) ^ 1) || ran_out(2);
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&q_full[buf]);
+        expect_bytes(bar, (uint32_t)(drafts_tile * group * 128) * (ROWS2 ? 4 : 2));
+        const int head = warp_uniform(now.head * group), draft = warp_uniform(now.draft);
+        for (int part = 0; part < (ROWS2 ? 2 : 1); ++part)
+          for (int h = 0; h < 2; ++h)
+            load_queries(smem_u32(q_s) + (ROWS2 ? part : buf) * TILE_BYTES + h * HALF_BYTES, &q_map, bar, h * 64, head, draft + part * drafts_tile);
         ++segments;
       }
-      ++tile;
-      if (!load((const bf16*)a.k_pool, t)) return false;
-      fetch();
-      return true;
-    };
-    fetch();
-    if (n_tiles > 0) ok = load_k(tiles[0]);
-    if (!ROWS2) {
-      if (ok && n_tiles > 1) ok = load_k(tiles[1]);
-      for (int i = 0; i < n_tiles && ok; i += 2) {
-        ok = load((const bf16*)a.v_pool, tiles[0]);
-        if (ok && i + 2 < n_tiles) ok = load_k(tiles[0]);
-        if (ok && i + 1 < n_tiles) ok = load((const bf16*)a.v_pool, tiles[1]);
-        if (ok && i + 3 < n_tiles) ok = load_k(tiles[1]);
+      // the places in the pool of the rows that begin the eights; -1: the page is not there
+      const int first = (unsigned)now.page < (unsigned)a.n_pages
+                            ? (now.page * a.kv_heads + now.head) * a.page_tokens + ((row0 + (lane & 7) * 8) & (a.page_tokens - 1)) : -1;
+      const unsigned there = __ballot_sync(0xffffffffu, first >= 0);
+      for (int j = 0; j < now.count; ++j) {
+        const int stage = taken % STAGES, key0 = now.key0 + j * KEYS;
+        ok = warp_wait(&empty[values * STAGES + stage], ((taken / STAGES) & 1) ^ 1) || ran_out(1);
+        if (!ok || flag[0]) { ok = false; break; }
+        const uint32_t at = ring_at + stage * TILE_BYTES;
+        if ((there >> (8 * j) & 0xFFu) == 0xFFu && key0 >= now.key_lo && key0 + KEYS <= now.ctx) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const bf16* from = pool + (long)__shfl_sync(0xffffffffu, first, 8 * j + g) * DIM + lane_from;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) copy16(at + to[i] + g * 1024, from + 2 * i * DIM);
+          }
+        } else {
+#pragma unroll 1
+          for (int g = 0; g < 8; ++g) {
+            const int row = __shfl_sync(0xffffffffu, first, 8 * j + g);
+            const bf16* from = pool + (row < 0 ? 0 : (long)row * DIM + lane_from);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = key0 + row0 + g * 8 + 2 * i + (lane >> 4);
+              const bool wanted = row >= 0 && key < now.ctx && key >= now.key_lo;
+              copy16_or_zeros(at + to[i] + g * 1024, wanted ? from + 2 * i * DIM : pool, wanted ? 16 : 0);
+            }
+          }
+        }
+        arrive_when_copied(smem_u32(&full[values * STAGES + stage]));
+        ++taken;
       }
-    } else {
-      for (int i = 0; i < n_tiles && ok; ++i) {
-        ok = load((const bf16*)a.v_pool, tiles[0]);
-        if (ok && i + 1 < n_tiles) ok = load_k(tiles[0]);
-      }
+      now = soon;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == LOADERS) {
@@ -392,7 +386,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
     ahead.begin_at(a, known, start[0], start[1], n_tiles);
     walk.begin_at(a, known, start[0], start[1], n_tiles);
     const int turns = warp_uniform(n_tiles * (ROWS2 ? 2 : 1));
-    int taken = 0, k_stage = 0, v_stage = 0;
+    int k_taken = 0, v_taken = 0, k_stage = 0, v_stage = 0;
     int a_left = 0, a_segment = -1, g_left = 0, g_turn = 0, g_segment = -1;
     // turn -2 and -1 have scores to be made and no second product: the loop holds each kind of product once
 #pragma unroll 1
@@ -407,9 +401,9 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
           if (g_segment > 0) ok = warp_wait(o_empty, (g_segment - 1) & 1) || ran_out(8);
         }
         if (ok && (!ROWS2 || w == 0)) {
-          v_stage = taken % STAGES;
-          ok = warp_wait(&full[v_stage], (taken / STAGES) & 1) || ran_out(4);
-          ++taken;
+          v_stage = STAGES + v_taken % STAGES;
+          ok = warp_wait(&full[v_stage], (v_taken / STAGES) & 1) || ran_out(4);
+          ++v_taken;
           fence_async_smem();                              // what cp.async wrote is read by the tensor cores
         }
         ok = ok && (warp_wait(&p_full[w], (t >> 1) & 1) || ran_out(5));
@@ -432,9 +426,9 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
           ok = warp_wait(&q_full[ROWS2 ? 0 : a_segment & 1], (ROWS2 ? a_segment : a_segment >> 1) & 1) || ran_out(2);
         }
         if (ok && (!ROWS2 || w == 0)) {
-          k_stage = taken % STAGES;
-          ok = warp_wait(&full[k_stage], (taken / STAGES) & 1) || ran_out(3);
-          ++taken;
+          k_stage = k_taken % STAGES;
+          ok = warp_wait(&full[k_stage], (k_taken / STAGES) & 1) || ran_out(3);
+          ++k_taken;
           fence_async_smem();
         }
         if (!ok) break;
@@ -450,7 +444,27 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
         if (--a_left == 0) umma_commit(&q_empty[ROWS2 ? 0 : a_segment & 1]);
       }
     }
-  } else if (warp >= FIRST_SOFTMAX) {
+  } else if (warp == LOADERS + 1) {
+    // ---------------- for the kernel that joins: the row tile inside which this block's share begins, if it is the first that does
+    pdl_wait();
+    ok = warp_wait(started, 0) || ran_out(2);
+    Walk<ROWS2> walk;
+    walk.begin_at(a, known, start[0], start[1], ok ? start[2] : 0);
+    Border border = {};
+    if (walk.next(a) && walk.begin > 0) {
+      const int total = start[3], shares = min((int)gridDim.x, total), unit = share_begin(total, blockIdx.x, shares) - walk.begin;
+      border.from = share_of(total, unit, shares);
+      border.upto = share_of(total, unit + walk.s.tiles - 1, shares);
+      if (border.from + 1 == (int)blockIdx.x) {
+        border.draft = walk.row_tile * (ROWS2 ? 2 : 1) * drafts_tile;
+        border.drafts = min(min(walk.s.n, a.max_nodes) - border.draft, (ROWS2 ? 2 : 1) * drafts_tile);
+        border.seq = walk.seq; border.head = walk.head; border.token = walk.s.first + border.draft;
+      }
+    }
+    if (lane == 0) a.borders[blockIdx.x] = border;
+  }
+  } else {
+    take_registers<MANY_REGS>();
     // ---------------- softmax: one row a thread
     const int wg = (warp - FIRST_SOFTMAX) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
@@ -481,16 +495,25 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
       const int token = dry ? 0 : g.s.first + (valid ? draft0 + draft : 0);
       const int* bits = a.tree + (size_t)token * a.tree_words;
       const int oldest = a.window > 0 && !dry ? max(a.positions[token], held) - a.window + 1 : 0;
+      // the words of the tree that the segment's last tile needs are under way until then
+      const int last_key = first_key + (dry ? 0 : g.count - 1) * KEYS, last_draft = last_key - held, last_word = last_draft >> 5;
+      uint32_t tree_bits[5];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) {
+        const int w = last_word + i;
+        tree_bits[i] = w >= 0 && w < tree_words ? (uint32_t)bits[w] : 0u;
+      }
       float m_ref = -INFINITY, l_sum = 0.f;
       const int t_first = turn0 + ((turn0 ^ wg) & 1);      // this warpgroup's first turn
       for (int t = t_first; t < turn0 + turns && ok; t += 2) {
         const int tile = ROWS2 ? (t - turn0) >> 1 : t - turn0, key0 = first_key + tile * KEYS, j = t >> 1;
-        // the keys that this row sees, while the scores are made
         const bool masked = (key0 + KEYS > held || key0 < key_lo || a.window > 0) && (!dry || quarter == 0);
         uint32_t words[4];
         if (masked) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) words[i] = seen_word(tree_words, bits, key0 + 32 * i, held, ctx, oldest);
+          for (int i = 0; i < 4; ++i)
+            words[i] = key0 == last_key ? seen_word(__funnelshift_r(tree_bits[i], tree_bits[i + 1], last_draft & 31), key0 + 32 * i, held, ctx, oldest)
+                                        : seen_word(tree_words, bits, key0 + 32 * i, held, ctx, oldest);
         }
         // a warp without rows waits as well: the turn before has been handed on by all four by then
         ok = dry || mbar_wait(&s_full[wg], j & 1) || ran_out(6);
@@ -549,29 +572,6 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
           }
           tmem_wait_st();
         }
-        if (key0 + KEYS > held && (!dry || quarter == 2)) {
-          // a draft's value row that is not finite is zeroed: 0 x NaN would be NaN for rows that do not see it. V's place in the ring's order:
-          // K0 K1 V0 K2 V1 ..., or K0 V0 K1 V1 ... with ROWS2
-          const int at = ROWS2 ? t | 1 : min(n_tiles, 2) + t + min(t, max(0, n_tiles - 2)), stage = at % STAGES;
-          ok = dry || mbar_wait(&full[stage], (at / STAGES) & 1) || ran_out(4);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          const int key = key0 + lane_row;
-          uint8_t* v_row = ring + stage * TILE_BYTES + lane_row * 128;
-          if (key >= held && key < ctx) {
-            bool bad = false;
-#pragma unroll 4
-            for (int piece = 0; piece < 16; ++piece) {
-              const uint4 x = *reinterpret_cast<const uint4*>(v_row + (piece >> 3) * HALF_BYTES + (piece & 7) * 16);
-              bad |= not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w);
-            }
-            if (bad && !dry) {
-              flag[1] = 1;
-#pragma unroll 1
-              for (int piece = 0; piece < 16; ++piece) *reinterpret_cast<uint4*>(v_row + (piece >> 3) * HALF_BYTES + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          fence_async_smem();
-        }
         fence_before_sync();
         __syncwarp();
         if (lane == 0 && !dry) mbar_arrive(&p_full[wg]);
@@ -590,6 +590,11 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       }
       fence_after_sync();
+      auto release = [&]() {                               // the accumulators may be written again
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0 && !dry) mbar_arrive(o_empty);
+      };
       // relative to one maximum: this warpgroup's accumulator by `mine`, the other's by `other`
       float mine = 1.f, other = 0.f;
       if (!ROWS2) {
@@ -613,81 +618,68 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
           }
           inv = total == 0.f ? 0.f : __fdividef(factor, total);
         }
-        // the channels: all, or half with the other warpgroup taking the rest; `first_acc`: the accumulator of the segment's first turn
+        // 64 channels at a time: all of its own rows, or, where the rows are both warpgroups', half; `first_acc`: the accumulator of the
+        // segment's first turn. The accumulators are free as soon as they lie in registers.
         const uint32_t first_acc = tmem_o + (ROWS2 ? wg : turn0 & 1) * 128 + lane_addr, second_acc = tmem_o + (~turn0 & 1) * 128 + lane_addr;
         const float by_first = (ROWS2 || (turn0 & 1) == wg ? mine : other) * inv, by_second = ((turn0 & 1) == wg ? other : mine) * inv;
         const long at = ((long)2 * blockIdx.x + (g.begin == 0 ? 1 : 0)) * (ROWS2 ? 2 * ROWS : ROWS) + (ROWS2 ? wg * ROWS : 0) + lane_row;
         float* part = a.partials + at * DIM;
         bf16* out = (bf16*)a.out + ((size_t)token * a.q_heads + row_head) * DIM;
-        const int ch_begin = ROWS2 ? 0 : wg * 4, ch_end = ROWS2 ? 8 : ch_begin + 4;
-        const bool bad = flag[1];
-        auto store = [&](int ch, const float (&v)[16]) {
-          uint32_t w[8];
-          if (split) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[e]);
-            store32(part + ch * 16, w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[8 + e]);
-            store32(part + ch * 16 + 8, w);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
-            store32(out + ch * 16, w);
-          }
-        };
-        auto read = [&](int ch, float (&v)[16]) {
-          if (both) {
-            float x[16];
-            tmem_ld16_two(first_acc + ch * 16, second_acc + ch * 16, v, x);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = v[e] * by_first + x[e] * by_second;
-          } else {
-            tmem_ld16(first_acc + ch * 16, v);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] *= by_first;
-          }
-        };
-        if (!__any_sync(0xffffffffu, bad)) {
-#pragma unroll 2
-          for (int ch = ch_begin; ch < ch_end; ++ch) {
-            float v[16];
-            read(ch, v);
-            if (valid) store(ch, v);
-          }
-        } else {
 #pragma unroll 1
-          for (int ch = ch_begin; ch < ch_end; ++ch) {
-            float v[16];
-            __syncwarp();                                  // lanes with drafts to add come back together
-            read(ch, v);
-            if (!valid) continue;
-            for (int key = max(first_key, held); key < min(ctx, first_key + g.count * KEYS); ++key) {
-              if (!sees(a, bits, key, held, oldest)) continue;
-              const long from = key_row(a, a.block_table + (size_t)g.seq * a.table_width, key, g.head);
-              if (from < 0) continue;
-              const float w = inv * zeroed_weight((const bf16*)a.q + ((size_t)token * a.q_heads + row_head) * DIM, (const bf16*)a.k_pool, (const bf16*)a.v_pool,
-                                                  from, a.cap_in, a.cap_out, c, m_ref == -INFINITY ? 0.f : m_log2);
-              if (w == 0.f) continue;
+        for (int half = ROWS2 ? 0 : wg; half < (ROWS2 ? 2 : wg + 1); ++half) {
+          float v[64];
+          tmem_ld64(first_acc + half * 64, v);
+          if (both) {
+            float x[64];
+            tmem_ld64(second_acc + half * 64, x);
+            if (!ROWS2) release();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) v[e] += w * __bfloat162float(((const bf16*)a.v_pool)[from * DIM + ch * 16 + e]);
-            }
-            store(ch, v);
+            for (int e = 0; e < 64; ++e) v[e] = v[e] * by_first + x[e] * by_second;
+          } else {
+            if (!ROWS2 || half == 1) release();
+#pragma unroll
+            for (int e = 0; e < 64; ++e) v[e] *= by_first;
           }
+          bool bad = false;                                // x - x is 0 for what is finite
+          {
+            float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 64; ++e) zero[e & 3] += v[e] - v[e];
+            bad = valid && !((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.f);
+          }
+          if (valid) {
+            if (split) {
+#pragma unroll
+              for (int piece = 0; piece < 8; ++piece) {
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[piece * 8 + e]);
+                store32(part + half * 64 + piece * 8, w);
+              }
+            } else {
+#pragma unroll
+              for (int piece = 0; piece < 4; ++piece) {
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = pack_bf16(v[piece * 16 + 2 * e], v[piece * 16 + 2 * e + 1]);
+                store32(out + half * 64 + piece * 16, w);
+              }
+            }
+          }
+          if (bad) flag[1] = 1;
         }
         if (valid && split && (ROWS2 || wg == 0)) *reinterpret_cast<float2*>(a.partials + a.partial_stats + at * 2) = make_float2(m_log2, l_sum);
+      } else {
+        release();
       }
-      if (dry) continue;
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(o_empty);
-      turn0 += turns;
+      if (!dry) turn0 += turns;
     }
   }
 
   // ---------------- teardown
   fence_before_sync();
   __syncthreads();
+  if (threadIdx.x == 0) a.not_finite[blockIdx.x] = flag[1];
   if (flag[0]) {
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);     // let copies in flight land
     __syncthreads();
@@ -698,43 +690,119 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const T
   }
 }
 
-// The parts of a row whose keys lie in several blocks' shares, in the order of the keys; one warp a row.
-constexpr int JOIN_THREADS = 128;
+// A row of the output by a warp, key by key: what the products cannot give where values are not finite. Seldom.
+__device__ __noinline__ void row_key_by_key(const TreeArgs& a, const Sequence& s, int seq, int head, int token, int row_head) {
+  const int lane = threadIdx.x & 31, oldest = a.window > 0 ? max(a.positions[token], s.held) - a.window + 1 : 0;
+  const int* table = a.block_table + (size_t)seq * a.table_width;
+  const int* bits = a.tree + (size_t)token * a.tree_words;
+  auto four = [&](const void* pool, long row) {
+    const uint2 w = *reinterpret_cast<const uint2*>((const bf16*)pool + row * DIM + 4 * lane);
+    const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x)), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
+    return make_float4(x.x, x.y, y.x, y.y);
+  };
+  const float4 q = four(a.q, (long)token * a.q_heads + row_head);
+  float top = a.sinks ? a.sinks[row_head] * LOG2E : -INFINITY, total = a.sinks ? 1.f : 0.f;      // in log2 units
+  float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int key = s.key_lo; key < s.ctx; ++key) {
+    if (!sees(a, bits, key, s.held, oldest)) continue;
+    const long at = key_row(a, table, key, head);
+    const float4 k = at < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : four(a.k_pool, at), v = at < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : four(a.v_pool, at);
+    float z = warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w);
+    if (a.cap_in != 0.f) z = a.cap_out - __fdividef(2.f * a.cap_out, 1.f + fast_exp2(z * a.cap_in));
+    z *= a.scale_log2;
+    const float m = fmaxf(top, z), base = m == -INFINITY ? 0.f : m, keep = exp2f(top - base), w = exp2f(z - base);
+    total = total * keep + w;
+    if (keep != 1.f) { out.x *= keep; out.y *= keep; out.z *= keep; out.w *= keep; }
+    if (w != 0.f) { out.x += w * v.x; out.y += w * v.y; out.z += w * v.z; out.w += w * v.w; }
+    top = m;
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  *reinterpret_cast<uint2*>((bf16*)a.out + ((size_t)token * a.q_heads + row_head) * DIM + 4 * lane) =
+      make_uint2(pack_bf16(out.x * inv, out.y * inv), pack_bf16(out.z * inv, out.w * inv));
+}
+// The rows of all row tiles that lie wholly in block b's share, one warp of the column of blocks after the other.
 template <bool ROWS2>
-__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const TreeArgs a, int blocks) {
+__device__ __noinline__ void share_key_by_key(const TreeArgs& a, int b, int blocks, int warp, int warps) {
+  int total = 0;
+  for (int seq = 0; seq < a.n_seqs; ++seq) {
+    const Sequence s = find_sequence<ROWS2>(a, a.cu_q[seq], a.cu_q[seq + 1], a.ctx_len[seq]);
+    total += a.kv_heads * s.row_tiles * s.tiles;
+  }
+  const int shares = min(blocks, total);
+  if (b >= shares) return;
+  const int from = share_begin(total, b, shares), upto = share_begin(total, b + 1, shares);
+  int at = 0;                                              // where the row tile begins in the list
+  for (int seq = 0; seq < a.n_seqs; ++seq) {
+    const Sequence s = find_sequence<ROWS2>(a, a.cu_q[seq], a.cu_q[seq + 1], a.ctx_len[seq]);
+    for (int unit = 0; unit < a.kv_heads * s.row_tiles; ++unit, at += s.tiles) {
+      if (at < from || at + s.tiles > upto) continue;
+      const int head = unit / s.row_tiles, draft0 = (unit - head * s.row_tiles) * (ROWS2 ? 2 : 1) * a.tile_drafts;
+      const int rows = min(min(s.n, a.max_nodes) - draft0, (ROWS2 ? 2 : 1) * a.tile_drafts) * a.group;
+      for (int row = warp; row < rows; row += warps)
+        row_key_by_key(a, s, seq, head, s.first + draft0 + row / a.group, head * a.group + row % a.group);
+    }
+  }
+}
+
+// The parts of the rows whose keys lie in several blocks' shares, in the order of the keys: eight lanes a row, 16 channels each.
+constexpr int JOIN_THREADS = 256, JOIN_ROWS = JOIN_THREADS / 8;
+template <bool ROWS2>
+__global__ void __launch_bounds__(JOIN_THREADS, 4) join_kernel(const __grid_constant__ TreeArgs a, int blocks) {
   pdl_launch_dependents();
   pdl_wait();
-  const int seq = blockIdx.y, head = blockIdx.x, group = a.group, drafts_tile = a.tile_drafts;
-  const int row = blockIdx.z * (JOIN_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;      // draft * group + head of the group
-  const Sequence s = find_sequence<ROWS2>(a, a.cu_q[seq], a.cu_q[seq + 1], a.ctx_len[seq]);
-  const int draft = row / group;
-  if (draft >= min(s.n, a.max_nodes)) return;
-  const int tile_drafts = drafts_tile * (ROWS2 ? 2 : 1), row_tile = draft / tile_drafts, in_tile = draft - row_tile * tile_drafts;
-  const int total = a.list[0], at = a.list[1 + seq] + (head * s.row_tiles + row_tile) * s.tiles;
-  const int shares = min(blocks, total), b0 = share_of(total, at, shares), b1 = share_of(total, at + s.tiles - 1, shares);
-  if (b0 == b1) return;
-  const int slot_rows = ROWS2 ? 2 * ROWS : ROWS, row_head = head * group + row - draft * group;
-  const int local = (in_tile / drafts_tile) * ROWS + (in_tile % drafts_tile) * group + row - draft * group;
-  auto place = [&](int b) { return ((long)2 * b + (b == b0 ? 1 : 0)) * slot_rows + local; };
-  const float2* stats = reinterpret_cast<const float2*>(a.partials + a.partial_stats);
-  const float sink = a.sinks ? a.sinks[row_head] * LOG2E : -INFINITY;
-  float top = sink;
-  for (int b = b0 + lane; b <= b1; b += 32) top = fmaxf(top, stats[place(b)].x);
-  top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  float total_weight = a.sinks ? exp2f(sink - base) : 0.f;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int b = b0; b <= b1; ++b) {
-    const float2 ml = stats[place(b)];
-    const float4 v = *reinterpret_cast<const float4*>(a.partials + place(b) * DIM + 4 * lane);
-    const float w = exp2f(ml.x - base);
-    total_weight += w * ml.y;
-    if (w != 0.f) { sum.x += w * v.x; sum.y += w * v.y; sum.z += w * v.z; sum.w += w * v.w; }
+  const Border border = a.borders[blockIdx.x];
+  const int lane = threadIdx.x & 31, warp = blockIdx.y * (JOIN_THREADS / 32) + (threadIdx.x >> 5), warps = gridDim.y * (JOIN_THREADS / 32);
+  const int row = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 3), rows = border.drafts * a.group;
+  if (rows > blockIdx.y * JOIN_ROWS) {
+    bool odd = false;
+    for (int p = border.from + lane; p <= border.upto; p += 32) odd |= a.not_finite[p] != 0;
+    const int draft = row / a.group, member = row - draft * a.group, row_head = border.head * a.group + member;
+    const int local = min(ROWS2 && draft >= a.tile_drafts ? ROWS + (draft - a.tile_drafts) * a.group + member : row, (ROWS2 ? 2 * ROWS : ROWS) - 1);
+    const int channel = 4 * (lane & 7);                    // and 32, 64, 96 behind it
+    auto place = [&](int p) { return ((long)2 * p + (p == border.from ? 1 : 0)) * (ROWS2 ? 2 * ROWS : ROWS) + local; };
+    const float2* stats = reinterpret_cast<const float2*>(a.partials + a.partial_stats);
+    float top = a.sinks && row < rows ? a.sinks[row_head] * LOG2E : -INFINITY, total = a.sinks ? 1.f : 0.f;
+    float4 sum[4] = {};
+    for (int p0 = border.from; p0 <= border.upto; p0 += 2) {        // two parts on their way at once
+      float2 ml[2];
+      float4 v[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const long at = place(min(p0 + j, border.upto));
+        ml[j] = stats[at];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = *reinterpret_cast<const float4*>(a.partials + at * DIM + channel + 32 * i);
+        if (p0 + j > border.upto) ml[j].x = -INFINITY;
+      }
+      const float m = fmaxf(fmaxf(ml[0].x, ml[1].x), top), base = m == -INFINITY ? 0.f : m, keep = exp2f(top - base);
+      total *= keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { sum[i].x *= keep; sum[i].y *= keep; sum[i].z *= keep; sum[i].w *= keep; }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float w = exp2f(ml[j].x - base);
+        if (w == 0.f) continue;
+        total += w * ml[j].y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { sum[i].x += w * v[j][i].x; sum[i].y += w * v[j][i].y; sum[i].z += w * v[j][i].z; sum[i].w += w * v[j][i].w; }
+      }
+      top = m;
+    }
+    if (__any_sync(0xffffffffu, odd)) {
+      const Sequence s = find_sequence<ROWS2>(a, a.cu_q[border.seq], a.cu_q[border.seq + 1], a.ctx_len[border.seq]);
+      for (int r = warp; r < rows; r += warps) {
+        const int d = r / a.group;
+        row_key_by_key(a, s, border.seq, border.head, border.token + d, border.head * a.group + r - d * a.group);
+      }
+    } else if (row < rows) {
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      bf16* to = (bf16*)a.out + ((size_t)(border.token + draft) * a.q_heads + row_head) * DIM + channel;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint2*>(to + 32 * i) = make_uint2(pack_bf16(sum[i].x * inv, sum[i].y * inv), pack_bf16(sum[i].z * inv, sum[i].w * inv));
+    }
   }
-  const float inv = total_weight == 0.f ? 0.f : 1.f / total_weight;
-  bf16* to = (bf16*)a.out + ((size_t)(s.first + draft) * a.q_heads + row_head) * DIM + 4 * lane;
-  *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(sum.x * inv, sum.y * inv), pack_bf16(sum.z * inv, sum.w * inv));
+  if (a.not_finite[blockIdx.x]) share_key_by_key<ROWS2>(a, blockIdx.x, blocks, warp, warps);
 }
 
 // The queries [tokens][q_heads][128]: 128 / group drafts with their heads of a group, 64 channels.
@@ -747,8 +815,8 @@ static bool query_map(CUtensorMap* map, const void* q, long tokens, int q_heads,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// scratch of `blocks` blocks, in floats: two places each of the partial outputs, their maxima and sums; the list
-static long scratch_floats(int blocks, bool rows2, int n_seqs) { return 2L * blocks * (rows2 ? 2 * ROWS : ROWS) * (DIM + 2) + n_seqs + 1; }
+// scratch of `blocks` blocks, in floats: two places each of the partial outputs, their maxima and sums; the borders, and whose outputs are not finite
+static long scratch_floats(int blocks, bool rows2) { return 2L * blocks * (rows2 ? 2 * ROWS : ROWS) * (DIM + 2) + 9L * blocks; }
 
 template <bool ROWS2>
 int launch(TreeArgs a, int blocks, cudaStream_t stream) {
@@ -759,12 +827,13 @@ int launch(TreeArgs a, int blocks, cudaStream_t stream) {
   if (!once.run(LB_ALLOW_SMEM(attention_tree_tcgen05_kernel<ROWS2>, SMEM_BYTES))) return lb_last_error();
   const long slots = 2L * blocks * (ROWS2 ? 2 * ROWS : ROWS);
   a.partial_stats = slots * DIM;
-  a.list = reinterpret_cast<int*>(a.partials + slots * (DIM + 2));
+  a.borders = reinterpret_cast<Border*>(a.partials + slots * (DIM + 2));
+  a.not_finite = reinterpret_cast<int*>(a.borders + blocks);
   a.group = group; a.tile_drafts = ROWS / group;
   int code = lb_launch(attention_tree_tcgen05_kernel<ROWS2>, blocks, THREADS, SMEM_BYTES, stream, q_map, a);
-  if (code || blocks == 1) return code;
-  const int rows = a.max_nodes * group;
-  return lb_launch(join_kernel<ROWS2>, dim3(a.kv_heads, a.n_seqs, (rows + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32)), JOIN_THREADS, 0, stream, a, blocks);
+  if (code) return code;
+  const int rows = min(a.max_nodes, a.tile_drafts * (ROWS2 ? 2 : 1)) * group;
+  return lb_launch(join_kernel<ROWS2>, dim3(blocks, (rows + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_THREADS, 0, stream, a, blocks);
 }
 }  // namespace wide
 }  // namespace

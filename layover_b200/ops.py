@@ -1315,7 +1315,7 @@ def tree_share(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: 
     keys = min(max_ctx, max_nodes + window) if window else max_ctx
     tiles = (-(-keys // 128) + (1 if window else 0)) * n_seqs * kv_heads * -(-max_nodes // (2 * drafts if rows2 else drafts))
     blocks = min(sms, tiles)
-    return blocks, rows2, 2 * blocks * (256 if rows2 else 128) * (128 + 2) + n_seqs + 1
+    return blocks, rows2, 2 * blocks * (256 if rows2 else 128) * (128 + 2) + 9 * blocks
 
 
 def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
@@ -1376,7 +1376,7 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(block_table), block_table.shape[1], k_pool.shape[0], _ptr(cu_q), _ptr(ctx_len),
                   given_positions, _ptr(tree), tree.shape[1], tokens, int(n_seqs), q_heads, kv_heads, dim, page_tokens, float(scale), int(window),
                   _ptr(sinks), float(softcap), int(max_nodes), blocks, int(rows2), _ptr(scratch), floats, _stream()), "attention_tree")
-        LAUNCHES += blocks > 1      # the shares' results are joined by a kernel of their own
+        LAUNCHES += 1               # the shares' results are joined by a kernel of their own
         return out
     tile_rows, row_tiles, chunks, chunk_tiles = tree_plan(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, dim, sms)
     partials = None

@@ -102,4 +102,4 @@ def test_tree_plan_covers_rows_and_keys(n_seqs, nodes, ctx, window, heads):
     assert chunks * chunk_tiles * 64 >= keys and (chunks - 1) * chunk_tiles * 64 < keys + 128
     assert chunks == 1 or n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) <= 64 << 20
     blocks, rows2, floats = ops.tree_share(n_seqs, nodes, ctx, window, q_heads, kv_heads, 148)
-    assert 1 <= blocks <= 148 and rows2 == (nodes > 128 // (q_heads // kv_heads)) and floats > 2 * blocks * 128 * 130 + n_seqs
+    assert 1 <= blocks <= 148 and rows2 == (nodes > 128 // (q_heads // kv_heads)) and floats > 2 * blocks * 128 * 130

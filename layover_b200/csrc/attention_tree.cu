@@ -24,6 +24,8 @@
 // one to the rows that see them.
 #include <math.h>
 
+#include <type_traits>
+
 #include "attention_tree.cuh"
 #include "attention_tree_tcgen05.cuh"
 #include "common.cuh"
@@ -54,10 +56,21 @@ template <typename T>
 __device__ __forceinline__ void load_tile(T* to, const T* __restrict__ pool, const TreeArgs& a, const Unit& u, const int* table, int tile, int stride) {
   constexpr int PER = 16 / (int)sizeof(T);
   const int pieces = a.dim / PER;
+  int r = threadIdx.x / pieces, c = threadIdx.x - r * pieces;
+  const int r_step = THREADS / pieces, c_step = THREADS - r_step * pieces;
+  const int shift = (a.page_tokens & (a.page_tokens - 1)) == 0 ? __ffs(a.page_tokens) - 1 : -1;
+#pragma unroll 4
   for (int i = threadIdx.x; i < KEYS * pieces; i += THREADS) {
-    const int r = i / pieces, c = i - r * pieces, key = tile * KEYS + r;
-    const long row = key >= u.key_lo && key < u.ctx ? key_row(a, table, key, u.head) : -1;
+    const int key = tile * KEYS + r;
+    long row = -1;
+    if (key >= u.key_lo && key < u.ctx) {
+      const int index = shift >= 0 ? key >> shift : key / a.page_tokens;
+      const int page = index < a.table_width ? table[index] : -1;
+      if ((unsigned)page < (unsigned)a.n_pages) row = ((long)page * a.kv_heads + u.head) * a.page_tokens + (key - index * a.page_tokens);
+    }
     cp_async16(to + r * stride + c * PER, pool + (row < 0 ? 0 : row * a.dim) + c * PER, row < 0 ? 0 : 16);
+    r += r_step; c += c_step;
+    if (c >= pieces) { c -= pieces; ++r; }
   }
 }
 
@@ -316,10 +329,19 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
 }
 
 // ------------------------------------------------------------------------------- float32
-template <int RT>
-__global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeArgs a) {
+// Two products an instruction: (x, y) += (a, b) (c, d)
+__device__ __forceinline__ void fma2(float2& x, float2 a, float2 b) {
+  asm("{\n\t.reg .b64 p, q, r;\n\t"
+      "mov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%0, %1};\n\t"
+      "fma.rn.f32x2 r, p, q, r;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t}"
+      : "+f"(x.x), "+f"(x.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
+
+// MAX_C: blocks of 64 channels of a head
+template <int RT, int MAX_C>
+__global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 2 : 1) attention_tree_f32_kernel(const TreeArgs a) {
   constexpr int RPT = RT / 8;                              // rows of a thread
-  constexpr int MAX_C = 4;                                 // blocks of 64 channels: head sizes up to 256
   extern __shared__ __align__(16) float smem_f[];
   __shared__ unsigned bad_rows[4];
   const int stride = a.dim + 4;                            // rows 16 bytes apart modulo 128: eight rows' pieces lie in different banks
@@ -357,13 +379,13 @@ __global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeA
     bits[i] = a.tree + (size_t)token * a.tree_words;
     oldest[i] = a.window > 0 ? max(a.positions[token], u.held) - a.window + 1 : 0;
   }
-  float o[RPT][MAX_C][4];
+  float2 o[RPT][MAX_C][2];
   float m_run[RPT], l_run[RPT];
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
     m_run[i] = -INFINITY; l_run[i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < MAX_C; ++c) o[i][c][0] = o[i][c][1] = o[i][c][2] = o[i][c][3] = 0.f;
+    for (int c = 0; c < MAX_C; ++c) o[i][c][0] = o[i][c][1] = make_float2(0.f, 0.f);
   }
   for (int tile = u.tile_begin; tile < u.tile_end; ++tile) {
     load_tile(v_s, v_pool, a, u, table, tile, stride);
@@ -372,9 +394,12 @@ __global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeA
     __syncthreads();
     const int key0 = tile * KEYS;
     const bool drafts = key0 + KEYS > u.held;
-    float s[RPT][4];
+    float2 pairs[RPT][4];                                  // sums over the even and over the odd channels
 #pragma unroll
-    for (int i = 0; i < RPT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pairs[i][j] = make_float2(0.f, 0.f);
+#pragma unroll 2
     for (int d = 0; d < a.dim; d += 4) {
       float4 kv[4];
 #pragma unroll
@@ -384,11 +409,16 @@ __global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeA
         const float4 qv = *reinterpret_cast<const float4*>(q_s + (ty + 8 * i) * stride + d);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[i][j] = fmaf(qv.x, kv[j].x, s[i][j]); s[i][j] = fmaf(qv.y, kv[j].y, s[i][j]);
-          s[i][j] = fmaf(qv.z, kv[j].z, s[i][j]); s[i][j] = fmaf(qv.w, kv[j].w, s[i][j]);
+          fma2(pairs[i][j], make_float2(qv.x, qv.y), make_float2(kv[j].x, kv[j].y));
+          fma2(pairs[i][j], make_float2(qv.z, qv.w), make_float2(kv[j].z, kv[j].w));
         }
       }
     }
+    float s[RPT][4];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = pairs[i][j].x + pairs[i][j].y;
     const bool masked = drafts || key0 < u.key_lo || a.window > 0;
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
@@ -417,7 +447,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeA
 #pragma unroll
       for (int c = 0; c < MAX_C; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][c][e] *= alpha;
+        for (int e = 0; e < 2; ++e) { o[i][c][e].x *= alpha; o[i][c][e].y *= alpha; }
     }
     cp_async_wait<0>();
     __syncthreads();                                       // values and weights are there, the keys are done with
@@ -435,27 +465,31 @@ __global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeA
       __syncthreads();
     }
     const bool any_bad = drafts && (bad_rows[0] | bad_rows[1] | bad_rows[2] | bad_rows[3]);
-    for (int key = 0; key < KEYS; key += 4) {
-      float4 w[RPT];
+    auto values = [&](auto some_bad) {
+#pragma unroll 1
+      for (int key = 0; key < KEYS; key += 4) {
+        float4 w[RPT];
 #pragma unroll
-      for (int i = 0; i < RPT; ++i) w[i] = *reinterpret_cast<const float4*>(p_s + (ty + 8 * i) * P_STRIDE + key);
+        for (int i = 0; i < RPT; ++i) w[i] = *reinterpret_cast<const float4*>(p_s + (ty + 8 * i) * P_STRIDE + key);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool bad = any_bad && (bad_rows[(key + e) >> 4] >> (2 * ((key + e) & 15)) & 3u);
+        for (int e = 0; e < 4; ++e) {
+          const bool bad = some_bad && (bad_rows[(key + e) >> 4] >> (2 * ((key + e) & 15)) & 3u);
 #pragma unroll
-        for (int c = 0; c < MAX_C; ++c) {
-          if (64 * c + 4 * tx >= a.dim) break;
-          const float4 v = *reinterpret_cast<const float4*>(v_s + (key + e) * stride + 64 * c + 4 * tx);
+          for (int c = 0; c < MAX_C; ++c) {
+            if (64 * c + 4 * tx >= a.dim) break;
+            const float4 v = *reinterpret_cast<const float4*>(v_s + (key + e) * stride + 64 * c + 4 * tx);
 #pragma unroll
-          for (int i = 0; i < RPT; ++i) {
-            const float p = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
-            if (bad && p == 0.f) continue;                 // what a row does not see does not reach it
-            o[i][c][0] = fmaf(p, v.x, o[i][c][0]); o[i][c][1] = fmaf(p, v.y, o[i][c][1]);
-            o[i][c][2] = fmaf(p, v.z, o[i][c][2]); o[i][c][3] = fmaf(p, v.w, o[i][c][3]);
+            for (int i = 0; i < RPT; ++i) {
+              const float p = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+              if (some_bad && bad && p == 0.f) continue;   // what a row does not see does not reach it
+              fma2(o[i][c][0], make_float2(p, p), make_float2(v.x, v.y));
+              fma2(o[i][c][1], make_float2(p, p), make_float2(v.z, v.w));
+            }
           }
         }
       }
-    }
+    };
+    if (any_bad) values(std::true_type{}); else values(std::false_type{});
     __syncthreads();                                       // values and weights are done with
   }
 #pragma unroll
@@ -469,7 +503,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeA
 #pragma unroll
       for (int c = 0; c < MAX_C; ++c)
         if (64 * c + 4 * tx < a.dim)
-          *reinterpret_cast<float4*>(a.partials + at * a.dim + 64 * c + 4 * tx) = make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
+          *reinterpret_cast<float4*>(a.partials + at * a.dim + 64 * c + 4 * tx) = make_float4(o[i][c][0].x, o[i][c][0].y, o[i][c][1].x, o[i][c][1].y);
       if (tx == 0) *reinterpret_cast<float2*>(a.partials + a.partial_stats + at * 2) = make_float2(m_run[i] * a.scale_log2, l_run[i]);
     } else {
       const int head = u.head * group + row % group;
@@ -484,7 +518,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_f32_kernel(const TreeA
 #pragma unroll
       for (int c = 0; c < MAX_C; ++c)
         if (64 * c + 4 * tx < a.dim)
-          *reinterpret_cast<float4*>(to + 64 * c + 4 * tx) = make_float4(o[i][c][0] * inv, o[i][c][1] * inv, o[i][c][2] * inv, o[i][c][3] * inv);
+          *reinterpret_cast<float4*>(to + 64 * c + 4 * tx) = make_float4(o[i][c][0].x * inv, o[i][c][0].y * inv, o[i][c][1].x * inv, o[i][c][1].y * inv);
     }
   }
 }
@@ -541,16 +575,18 @@ int launch_mma(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
   if (!once.run(LB_ALLOW_SMEM((attention_tree_mma_kernel<RG, MAX_DIM>), (16 * RG + 4 * KEYS) * (MAX_DIM + PAD) * sizeof(bf16)))) return lb_last_error();
   return lb_launch(attention_tree_mma_kernel<RG, MAX_DIM>, grid, THREADS, smem, stream, a);
 }
-template <int RT>
-int launch_f32(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
+template <int RT, int MAX_C>
+int launch_f32_of(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
   const size_t smem = ((size_t)(RT + 2 * KEYS) * (a.dim + 4) + RT * (KEYS + 4)) * sizeof(float);
   static LbPerDeviceOnce once;
-  if (!once.run(LB_ALLOW_SMEM(attention_tree_f32_kernel<RT>, ((RT + 2 * KEYS) * (256 + 4) + RT * (KEYS + 4)) * sizeof(float)))) return lb_last_error();
-  return lb_launch(attention_tree_f32_kernel<RT>, grid, THREADS, smem, stream, a);
+  if (!once.run(LB_ALLOW_SMEM((attention_tree_f32_kernel<RT, MAX_C>), ((RT + 2 * KEYS) * (64 * MAX_C + 4) + RT * (KEYS + 4)) * sizeof(float)))) return lb_last_error();
+  return lb_launch(attention_tree_f32_kernel<RT, MAX_C>, grid, THREADS, smem, stream, a);
 }
+template <int RT>
+int launch_f32(const TreeArgs& a, dim3 grid, cudaStream_t stream) { return a.dim <= 128 ? launch_f32_of<RT, 2>(a, grid, stream) : launch_f32_of<RT, 4>(a, grid, stream); }
 }  // namespace
 
-// What the three entries below check alike.
+// What the two entries below check alike.
 static int check_tree(int dtype, const void* q, const void* k_pool, const void* v_pool, const void* out, int table_width, int n_pages, const int* positions,
                       int tree_words, int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, int window, float softcap, int max_nodes) {
   if (dtype != LB_F32 && dtype != LB_BF16) return LB_ERR_DTYPE;
@@ -562,7 +598,7 @@ static int check_tree(int dtype, const void* q, const void* k_pool, const void* 
   return 0;
 }
 
-// `tile_rows`: rows of a block (16, 32 or 64). `chunks` blocks of `chunk_tiles` tiles of 64 keys share a row tile's keys (the last takes
+// `tile_rows`: rows of a block (16, 32 or, in bfloat16, 64). `chunks` blocks of `chunk_tiles` tiles of 64 keys share a row tile's keys (the last takes
 // what is left); with more than one, `partials` holds n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) floats.
 LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
                                 int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words, int tokens,
@@ -574,7 +610,7 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
                                  window, softcap, max_nodes);
   if (refused) return refused;
   if (row_tiles <= 0 || chunks <= 0 || chunks > 65535 || chunk_tiles <= 0 || (long)n_seqs * row_tiles > 65535 ||
-      (tile_rows != 16 && tile_rows != 32 && tile_rows != 64))
+      (tile_rows != 16 && tile_rows != 32 && (tile_rows != 64 || dtype != LB_BF16)))
     return LB_ERR_SIZE;
   const long partial_rows = (long)n_seqs * kv_heads * row_tiles * chunks * tile_rows;
   if (chunks > 1 && (!partials || partial_floats < partial_rows * (dim + 2))) return LB_ERR_SIZE;
@@ -586,7 +622,7 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
   const dim3 grid(kv_heads, n_seqs * row_tiles, chunks);
   int code;
   if (dtype == LB_F32) {
-    code = tile_rows == 16 ? launch_f32<16>(a, grid, stream) : tile_rows == 32 ? launch_f32<32>(a, grid, stream) : launch_f32<64>(a, grid, stream);
+    code = tile_rows == 16 ? launch_f32<16>(a, grid, stream) : launch_f32<32>(a, grid, stream);
   } else if (dim <= 128) {
     code = tile_rows == 16 ? launch_mma<1, 128>(a, grid, stream) : tile_rows == 32 ? launch_mma<2, 128>(a, grid, stream) : launch_mma<4, 128>(a, grid, stream);
   } else {

@@ -54,13 +54,22 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
-def _here(what: str, *tensors: torch.Tensor | None) -> None:
-    """Every tensor is on the current CUDA device, on whose current stream the kernels are launched."""
+def _pointers(what: str, *tensors: torch.Tensor | None) -> list[int | None]:
+    """The addresses of tensors that are all on the current CUDA device, on whose current stream the kernels are launched."""
+    current, found = None, []
     for t in tensors:
-        if t is not None:
-            _ptr(t)
-            if t.get_device() != torch._C._cuda_getDevice():
-                raise ValueError(f"{what}: the tensors must be on the current CUDA device")
+        if t is None:
+            found.append(None)
+            continue
+        device = t.get_device()
+        if device < 0:
+            raise KernelError("layover_b200 kernels need CUDA tensors: there is no CPU path")
+        if current is None:
+            current = torch._C._cuda_getDevice()
+        if device != current:
+            raise ValueError(f"{what}: the tensors must be on the current CUDA device")
+        found.append(t.data_ptr())
+    return found
 
 
 def _stream() -> int:
@@ -1285,23 +1294,27 @@ def attention_f32(q, cache, out, block_table, batch, q_heads, kv_heads, dim, pag
 _TREE_SCRATCH_FLOATS = 64 << 20          # the most that the chunks' results may take (256 MiB)
 
 
-def attention_tree_on_tcgen05(rows: int, group: int, dim: int, page_tokens: int, dtype: torch.dtype) -> bool:
-    """Whether `attention_tree` takes these rows (drafts times heads of a group) to its tcgen05 kernel."""
-    return dtype == torch.bfloat16 and dim == 128 and page_tokens % 8 == 0 and 128 % page_tokens == 0 and 16 < rows and group <= 128
+def attention_tree_on_tcgen05(group: int, dim: int, page_tokens: int, dtype: torch.dtype) -> bool:
+    """Whether `attention_tree` takes these heads and pages to its tcgen05 kernel: whatever it takes, however few the rows (one B200, 32 heads
+    over 8, 4 drafts; tcgen05 and mma.sync, us: 1 request of 700 keys 12.6 and 15.2, 8 of 3,000 37 and 67)."""
+    return dtype == torch.bfloat16 and dim == 128 and page_tokens % 8 == 0 and 128 % page_tokens == 0 and group <= 128
 
 
 @functools.lru_cache(maxsize=1024)      # of the sizes alone, asked for by every layer of a step
-def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, dim: int, sms: int) -> tuple[int, int, int, int]:
-    """(rows of a block, row tiles of a sequence, chunks, key tiles of a chunk) for the FFMA and mma.sync kernels of `attention_tree`: row
-    tiles no larger than the rows ask for, and as many chunks of the keys as give every SM about four blocks."""
+def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, dim: int, sms: int, wide: bool = False) -> tuple[int, int, int, int]:
+    """(rows of a block, row tiles of a sequence, chunks, key tiles of a chunk) for the FFMA and mma.sync kernels of `attention_tree`: tiles
+    of 32 rows, or 16 where there are no more (`wide`, bfloat16: of 64 where there are over 128), and as many chunks of the keys as give every SM
+    about four blocks. Measured (one B200, us): 4 requests of 900 keys, 52 rows in 32 bits with 16, 32 and 64 rows a tile 103, 74 and 91,
+    with one, two, three and five key tiles a chunk 81, 74, 95 and 84; 5 of 1,024 keys, 78 rows of 64 channels in bfloat16 16.3, 16.1 and
+    17.1, with one, two and five 16.1, 16.8 and 24.1."""
     rows = max_nodes * (q_heads // kv_heads)
-    tile_rows = 16 if rows <= 16 else 32 if rows <= 32 else 64
+    tile_rows = 16 if rows <= 16 else 64 if wide and rows > 128 else 32
     row_tiles = -(-rows // tile_rows)
     keys = min(max_ctx, max_nodes + window) if window else max_ctx
     tiles = -(-keys // 64) + (1 if window else 0)
     units = n_seqs * kv_heads * row_tiles
     most = max(1, _TREE_SCRATCH_FLOATS // (units * tile_rows * (dim + 2)))
-    chunks = max(1, min(-(-4 * sms // units), tiles // 2, most, 65535))
+    chunks = max(1, min(-(-4 * sms // units), tiles, most, 65535))
     chunk_tiles = -(-tiles // chunks)
     return tile_rows, row_tiles, -(-tiles // chunk_tiles), chunk_tiles
 
@@ -1334,26 +1347,28 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     scaled score s becomes softcap * tanh(s / softcap). No sequence has more than `max_nodes` drafts or more than `max_ctx` keys
     (what is above is not computed: rows, or not planned for: keys). Rows behind cu_q[n_seqs] stay as they are. Head sizes: multiples of
     16 (float32: of 4) up to 256. What is in a draft's keys and values reaches only the rows that see it, infinities and NaN too."""
-    _need(q, None, "q"); _need(out, q.dtype, "out"); _need(k_pool, q.dtype, "k_pool"); _need(v_pool, q.dtype, "v_pool")
+    dtype, tokens = q.dtype, q.shape[0]
+    _need(q, None, "q"); _need(out, dtype, "out"); _need(k_pool, dtype, "k_pool"); _need(v_pool, dtype, "v_pool")
     for name, t, dims in (("block_table", block_table, 2), ("cu_q", cu_q, 1), ("ctx_len", ctx_len, 1), ("tree", tree, 2)):
         _need(t, torch.int32, name)
         if t.dim() != dims:
             raise ValueError(f"attention_tree: {name} must have {dims} dimension(s)")
     if q_heads < 1 or kv_heads < 1 or q_heads % kv_heads:
         raise ValueError(f"attention_tree: q_heads ({q_heads}) must be a multiple of kv_heads ({kv_heads})")
-    tokens = q.shape[0]
-    if tuple(q.shape) != (tokens, q_heads * dim) or out.shape != q.shape or k_pool.shape != v_pool.shape \
-            or tuple(k_pool.shape[1:]) != (kv_heads, page_tokens, dim):
+    pages, table_width, words = k_pool.shape[0], block_table.shape[1], tree.shape[1]
+    if q.shape != (tokens, q_heads * dim) or out.shape != q.shape or v_pool.shape != k_pool.shape or k_pool.shape != (pages, kv_heads, page_tokens, dim):
         raise ValueError("attention_tree: q, out or the pools do not match the heads")
-    if tree.shape[0] != tokens or block_table.shape[0] < n_seqs or cu_q.numel() < n_seqs + 1 or ctx_len.numel() < n_seqs:
+    if tree.shape[0] != tokens or block_table.shape[0] < n_seqs or cu_q.shape[0] < n_seqs + 1 or ctx_len.shape[0] < n_seqs:
         raise ValueError("attention_tree: a row of tree per draft, a table row, an end and a length per sequence")
     if max_nodes < 1 or max_ctx < 1 or window < 0 or softcap < 0:
         raise ValueError("attention_tree: max_nodes and max_ctx are at least 1, window and softcap not negative")
-    if max_nodes > 32 * tree.shape[1]:
-        raise ValueError(f"attention_tree: {max_nodes} drafts need {-(-max_nodes // 32)} words a row of tree, got {tree.shape[1]}")
-    if window:
-        if positions is None:
-            raise ValueError("attention_tree: a window needs positions")
+    if max_nodes > 32 * words:
+        raise ValueError(f"attention_tree: {max_nodes} drafts need {-(-max_nodes // 32)} words a row of tree, got {words}")
+    if not window:
+        positions = None
+    elif positions is None:
+        raise ValueError("attention_tree: a window needs positions")
+    else:
         _need(positions, torch.int32, "positions")
         if positions.numel() < tokens:
             raise ValueError("attention_tree: a position per draft")
@@ -1361,34 +1376,36 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         _need(sinks, torch.float32, "sinks")
         if sinks.numel() != q_heads:
             raise ValueError("attention_tree: one sink per query head")
-    if q.dtype not in _DTYPE_CODE or dim % (16 if q.dtype == torch.bfloat16 else 4) or not 0 < dim <= 256:
-        raise ValueError(f"attention_tree: heads of {dim} channels in {q.dtype} are not supported")
-    _here("attention_tree", q, k_pool, v_pool, out, block_table, cu_q, ctx_len, positions if window else None, tree, sinks)
+    if dtype not in _DTYPE_CODE or dim % (16 if dtype == torch.bfloat16 else 4) or not 0 < dim <= 256:
+        raise ValueError(f"attention_tree: heads of {dim} channels in {dtype} are not supported")
+    q_ptr, k_ptr, v_ptr, out_ptr, table_ptr, cu_ptr, ctx_ptr, positions_ptr, tree_ptr, sinks_ptr = _pointers(
+        "attention_tree", q, k_pool, v_pool, out, block_table, cu_q, ctx_len, positions, tree, sinks)
     if tokens == 0 or n_seqs == 0:
         return out
     global LAUNCHES
-    group, sms, given_positions = q_heads // kv_heads, sm_count(q.device), _ptr(positions if window else None)
-    if attention_tree_on_tcgen05(max_nodes * group, group, dim, page_tokens, q.dtype):
+    device = q.device
+    sms = sm_count(device)
+    if attention_tree_on_tcgen05(q_heads // kv_heads, dim, page_tokens, dtype):
         blocks, rows2, floats = tree_share(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, sms)
-        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)          # of this call alone, on its own stream
+        scratch = torch.empty(floats, dtype=torch.float32, device=device)          # of this call alone, on its own stream
         fn = _FUNCTIONS.get("lb_attention_tree_tcgen05") or _fn("attention_tree", "lb_attention_tree_tcgen05",
                  [c_void_p] * 5 + [c_int, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float, c_int, c_void_p, c_float] + [c_int] * 3 + [c_void_p, c_long, c_void_p])
-        _check(fn(_ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(block_table), block_table.shape[1], k_pool.shape[0], _ptr(cu_q), _ptr(ctx_len),
-                  given_positions, _ptr(tree), tree.shape[1], tokens, int(n_seqs), q_heads, kv_heads, dim, page_tokens, float(scale), int(window),
-                  _ptr(sinks), float(softcap), int(max_nodes), blocks, int(rows2), _ptr(scratch), floats, _stream()), "attention_tree")
+        _check(fn(q_ptr, k_ptr, v_ptr, out_ptr, table_ptr, table_width, pages, cu_ptr, ctx_ptr, positions_ptr, tree_ptr, words, tokens, n_seqs, q_heads,
+                  kv_heads, dim, page_tokens, scale, window, sinks_ptr, softcap, max_nodes, blocks, rows2, scratch.data_ptr(), floats, _stream()),
+               "attention_tree")
         LAUNCHES += 1               # the shares' results are joined by a kernel of their own
         return out
-    tile_rows, row_tiles, chunks, chunk_tiles = tree_plan(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, dim, sms)
-    partials = None
+    tile_rows, row_tiles, chunks, chunk_tiles = tree_plan(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, dim, sms, dtype == torch.bfloat16)
+    partials, floats = None, 0
     if chunks > 1:          # of this call alone, on its own stream
-        partials = torch.empty(n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2), dtype=torch.float32, device=q.device)
+        floats = n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2)
+        partials = torch.empty(floats, dtype=torch.float32, device=device)
     fn = _FUNCTIONS.get("lb_attention_tree") or _fn("attention_tree", "lb_attention_tree",
              [c_int] + [c_void_p] * 5 + [c_int, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float, c_int, c_void_p, c_float] + [c_int] * 5
              + [c_void_p, c_long, c_void_p])
-    _check(fn(dtype_code(q.dtype), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(out), _ptr(block_table), block_table.shape[1], k_pool.shape[0],
-              _ptr(cu_q), _ptr(ctx_len), given_positions, _ptr(tree), tree.shape[1], tokens, int(n_seqs), q_heads, kv_heads, dim, page_tokens,
-              float(scale), int(window), _ptr(sinks), float(softcap), int(max_nodes), tile_rows, row_tiles, chunks, chunk_tiles, _ptr(partials),
-              partials.numel() if partials is not None else 0, _stream()), "attention_tree")
+    _check(fn(dtype_code(dtype), q_ptr, k_ptr, v_ptr, out_ptr, table_ptr, table_width, pages, cu_ptr, ctx_ptr, positions_ptr, tree_ptr, words, tokens,
+              n_seqs, q_heads, kv_heads, dim, page_tokens, scale, window, sinks_ptr, softcap, max_nodes, tile_rows, row_tiles, chunks, chunk_tiles,
+              None if partials is None else partials.data_ptr(), floats, _stream()), "attention_tree")
     LAUNCHES += chunks > 1      # the chunks' results are joined by a kernel of their own
     return out
 
@@ -1408,12 +1425,12 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torc
     _need(pool, None, "pool"); _need(src, torch.int32, "src"); _need(dst, torch.int32, "dst")
     if pool.dim() < 2 or src.dim() != 1 or src.shape != dst.shape:
         raise ValueError("copy_pages: pool [planes, pages, ...], src and dst one index per copy")
-    _here("copy_pages", pool, src, dst)
+    pool_ptr, src_ptr, dst_ptr = _pointers("copy_pages", pool, src, dst)
     planes, pages = pool.shape[:2]
     if pool.numel() == 0 or src.numel() == 0:
         return pool
     fn = _FUNCTIONS.get("lb_copy_pages") or _fn("cache_moves", "lb_copy_pages", [c_void_p] * 3 + [c_int] * 3 + [c_long, c_void_p])
-    _check(fn(_ptr(pool), _ptr(src), _ptr(dst), src.numel(), planes, pages, pool.numel() // (planes * pages) * pool.element_size(), _stream()), "copy_pages")
+    _check(fn(pool_ptr, src_ptr, dst_ptr, src.numel(), planes, pages, pool.numel() // (planes * pages) * pool.element_size(), _stream()), "copy_pages")
     return pool
 
 
@@ -1429,13 +1446,13 @@ def compact_tokens(pool: torch.Tensor, block_table: torch.Tensor, first: torch.T
     n_seqs = first.numel()
     if pool.dim() != 5 or block_table.dim() != 2 or block_table.shape[0] < n_seqs or cu_picked.numel() != n_seqs + 1:
         raise ValueError("compact_tokens: pool [planes, pages, heads, page_tokens, channels], a table row and an end per sequence")
-    _here("compact_tokens", pool, block_table, first, picked, cu_picked)
+    pool_ptr, table_ptr, first_ptr, picked_ptr, cu_ptr = _pointers("compact_tokens", pool, block_table, first, picked, cu_picked)
     planes, pages, heads, page_tokens, channels = pool.shape
     if pool.numel() == 0 or picked.numel() == 0 or block_table.shape[1] == 0:
         return pool
     fn = _FUNCTIONS.get("lb_compact_tokens") or _fn("cache_moves", "lb_compact_tokens",
              [c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_long, c_void_p])
-    _check(fn(_ptr(pool), _ptr(block_table), block_table.shape[1], _ptr(first), _ptr(picked), _ptr(cu_picked), n_seqs, planes, pages, heads,
+    _check(fn(pool_ptr, table_ptr, block_table.shape[1], first_ptr, picked_ptr, cu_ptr, n_seqs, planes, pages, heads,
               page_tokens, channels * pool.element_size(), _stream()), "compact_tokens")
     return pool
 
@@ -1444,10 +1461,15 @@ BEAM_MAX_KEEP = 32      # the most continuations that `beam_select` chooses
 BEAM_MAX_BEAMS = 64     # the most beams of a request
 
 
-def _beam_chunk(rows: int, vocab: int, sms: int) -> int:
-    """Values of a row that a block of the first kernel reads: about three blocks an SM, at least 2,048 values each."""
-    chunks = max(1, min(-(-vocab // 2048), 3 * sms // rows))
-    return -(-vocab // chunks)
+_BEAM_PIECE = 4096      # values of a row that a block of the first kernel looks at together (csrc/beam.cu)
+
+
+def _beam_pieces(rows: int, vocab: int, sms: int) -> int:
+    """Pieces of a row that one block takes: 2 to 5, by the pieces there are for the SMs. The first costs the block most, but what is left
+    over runs alone. Measured (one B200, us; 1, 2, 4, 5 and 8 pieces): 128 rows of 151,936 67, 47, 39.6, 37.5 and 41.5 (5 are taken), 64 rows
+    22, 18, 17.6, 16.4 and 19.5 (5), 16 rows 11.6, 11.2, 11.5, 12.3 and 14.9 (2), 4 rows 8.7, 8.3, 10.4, 11.5 and 14.4 (2), 32 rows of 32,768
+    with 32 kept 37, 20, 22, 27 and 36 (2)."""
+    return min(5, max(2, -(-10 * rows * -(-vocab // _BEAM_PIECE) // (34 * sms))))
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, next_scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor,
@@ -1475,15 +1497,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, next_scores: torch.T
         _need(ended, torch.int32, "ended")
         if ended.shape != scores.shape:
             raise ValueError("beam_select: ended must have scores' shape")
-    _here("beam_select", logits, scores, next_scores, parents, tokens, ended)
+    logits_ptr, scores_ptr, next_ptr, parents_ptr, tokens_ptr, ended_ptr = _pointers("beam_select", logits, scores, next_scores, parents, tokens, ended)
     if requests == 0:
         return
-    chunk = _beam_chunk(requests * beams, vocab, sm_count(logits.device))
-    scratch = torch.empty(requests * beams * -(-vocab // chunk) * (2 + 2 * keep), dtype=torch.int32, device=logits.device)     # of this call alone
+    pieces = _beam_pieces(requests * beams, vocab, sm_count(logits.device))
+    scratch = torch.empty(requests * beams * -(-vocab // (_BEAM_PIECE * pieces)) * (2 + 2 * keep), dtype=torch.int32, device=logits.device)     # of this call alone
     fn = _FUNCTIONS.get("lb_beam_select") or _fn("beam", "lb_beam_select",
              [c_void_p, c_long, c_void_p, c_void_p] + [c_int] * 6 + [c_void_p, c_long] + [c_void_p] * 4)
-    _check(fn(_ptr(logits), logits.stride(0), _ptr(scores), _ptr(ended), requests, beams, vocab, keep, int(pad), chunk, _ptr(scratch), scratch.numel(),
-              _ptr(next_scores), _ptr(parents), _ptr(tokens), _stream()), "beam_select")
+    _check(fn(logits_ptr, logits.stride(0), scores_ptr, ended_ptr, requests, beams, vocab, keep, pad, pieces, scratch.data_ptr(), scratch.numel(),
+              next_ptr, parents_ptr, tokens_ptr, _stream()), "beam_select")
     global LAUNCHES
     LAUNCHES += 1              # the chunks' lists are joined by a kernel of their own
 

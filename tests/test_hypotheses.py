@@ -96,10 +96,11 @@ def test_beam_selection_refuses(over, message):
                                                              (5, 13, 1544, 1024, (12, 2, 64)), (3, 700, 900, 16, (16, 1, 128)), (64, 64, 131072, 0, (64, 8, 256))])
 def test_tree_plan_covers_rows_and_keys(n_seqs, nodes, ctx, window, heads):
     q_heads, kv_heads, dim = heads
-    tile_rows, row_tiles, chunks, chunk_tiles = ops.tree_plan(n_seqs, nodes, ctx, window, *heads, 148)
-    rows, keys = nodes * q_heads // kv_heads, min(ctx, nodes + window) if window else ctx
-    assert (row_tiles - 1) * tile_rows < rows <= row_tiles * tile_rows
-    assert chunks * chunk_tiles * 64 >= keys and (chunks - 1) * chunk_tiles * 64 < keys + 128
-    assert chunks == 1 or n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) <= 64 << 20
+    for wide in (False, True):
+        tile_rows, row_tiles, chunks, chunk_tiles = ops.tree_plan(n_seqs, nodes, ctx, window, *heads, 148, wide)
+        rows, keys = nodes * q_heads // kv_heads, min(ctx, nodes + window) if window else ctx
+        assert (row_tiles - 1) * tile_rows < rows <= row_tiles * tile_rows
+        assert chunks * chunk_tiles * 64 >= keys and (chunks - 1) * chunk_tiles * 64 < keys + 128
+        assert chunks == 1 or n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) <= 64 << 20
     blocks, rows2, floats = ops.tree_share(n_seqs, nodes, ctx, window, q_heads, kv_heads, 148)
     assert 1 <= blocks <= 148 and rows2 == (nodes > 128 // (q_heads // kv_heads)) and floats > 2 * blocks * 128 * 130

@@ -21,6 +21,8 @@ import torch
 from .cache import CacheManager, OutOfBlocks
 from .config import FimilixConfig, KirenexConfig, LimazenConfig, MimitarConfig, Qwen3Config, TopidraConfig, VopozenConfig, load_config, preset, register_architecture, supported_architectures
 from .engine import DEVICE_TOKEN, Engine, EngineConfig, Request, RequestTooLarge, State, StepEntry
+from .engine.beams import beam_search
+from .engine.drafts import LookupDrafts, generate_with_drafts
 from .models import load_model, random_model
 from .parts.base import PagedKVNeed
 from .sampling import SamplingParams
@@ -73,5 +75,5 @@ __all__ = [
     "CacheManager", "OutOfBlocks", "FimilixConfig", "KirenexConfig", "LimazenConfig", "MimitarConfig", "Qwen3Config", "TopidraConfig", "VopozenConfig", "load_config", "preset", "register_architecture",
     "supported_architectures", "DEVICE_TOKEN", "Engine", "EngineConfig", "Request", "RequestTooLarge", "State", "StepEntry",
     "load_model", "random_model", "SamplingParams", "write_model_folder", "PagedKVCache", "blocks_for_pool",
-    "generate",
+    "generate", "beam_search", "generate_with_drafts", "LookupDrafts",
 ]

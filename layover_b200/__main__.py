@@ -7,7 +7,8 @@ Option names and meanings follow the reference's server where it has them
 (layover/server.py:415-434): --model, --device, --dtype {bf16,fp32}, --pool-gib, --block-tokens,
 --max-batch, --prefill-chunk (also the per-step prompt budget, as server.py:461), --cuda-graphs.
 --ignore-eos is the request option of that name (server.py:183,195). --max-batched-tokens is this
-engine's own: one budget for a whole step, decoded tokens first. The HTTP server itself and the
+engine's own: one budget for a whole step, decoded tokens first; so are --beams N (the N most likely continuations of each prompt
+instead of one) and --drafts N (greedy, N guessed tokens a branch checked in every step). The HTTP server itself and the
 agent options are not part of this engine. The result is one JSON object on standard output.
 """
 
@@ -41,6 +42,8 @@ def parse_args(argv=None):
     p.add_argument("--prompt-lens", default=None, help="comma-separated lengths of seeded random prompts")
     p.add_argument("--max-new-tokens", type=int, default=16)
     p.add_argument("--temperature", type=float, default=0.0)
+    p.add_argument("--beams", type=int, default=0, help="follow this many beams of each prompt and print all of them")
+    p.add_argument("--drafts", type=int, default=0, help="check guesses of up to this many tokens in every step (greedy)")
     p.add_argument("--write-model", default=None, help="write the --preset's random model to this folder and exit")
     return p.parse_args(argv)
 
@@ -74,6 +77,20 @@ def main(argv=None) -> int:
             prompts.append(torch.randint(0, model.spec.vocab_size, (length,), generator=gen).tolist())
     if not prompts:
         raise SystemExit("no prompts: give --prompt-ids or --prompt-lens")
+    stop = frozenset() if args.ignore_eos or getattr(model.cfg, "eos_token_id", None) is None else frozenset({model.cfg.eos_token_id})
+    if args.beams or args.drafts:
+        if (args.beams and args.drafts) or args.temperature:
+            raise SystemExit("--beams and --drafts exclude one another and a temperature")
+        began, options = time.perf_counter(), dict(stop_tokens=stop, num_blocks=args.num_blocks, block_tokens=args.block_tokens, prefill_chunk=args.prefill_chunk)
+        if args.beams:
+            found = lb.beam_search(model, prompts, args.beams, args.max_new_tokens, **options)
+            result = {"generated": [[tokens for _, tokens in beams] for beams in found], "scores": [[round(score, 4) for score, _ in beams] for beams in found]}
+        else:
+            generated, counts = lb.generate_with_drafts(model, prompts, args.max_new_tokens, lb.LookupDrafts(depth=args.drafts), **options)
+            result = {"generated": generated, "stats": counts}
+        torch.cuda.synchronize()
+        print(json.dumps({**result, "seconds": round(time.perf_counter() - began, 4)}))
+        return 0
     blocks = args.num_blocks or lb.blocks_for_pool(model, args.pool_gib, args.block_tokens)
     cache = lb.PagedKVCache(model, blocks, block_tokens=args.block_tokens, max_requests=max(args.max_batch, 1))
     engine = lb.Engine(model, cache, lb.EngineConfig(args.max_batch, args.prefill_chunk, args.prefill_chunk,

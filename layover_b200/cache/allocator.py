@@ -2,8 +2,8 @@
 
 What the reference's allocator does and this one keeps (layover/kv/allocator.py:15-60): a request
 for several pages is served whole or not at all, and the page given back last is handed out
-first. What it drops: reference counts. No two requests share a page in this engine, so a page
-is either free or out to exactly one table, and giving back a page that is not out (a second
+first. A page that is out belongs to one table, or, once it has been `share`d (a request was forked), to
+several, and returns when the last of them gives it back; giving back a page that is not out (a second
 time, or one that never left) is an error rather than a no-op.
 """
 
@@ -19,7 +19,7 @@ OutOfPages = OutOfBlocks
 
 class BlockAllocator:
     """Pages 0 .. num_blocks - 1. `_stack` holds the free ones, the next to go out at its end;
-    `_out[page]` says whether a page is with a caller."""
+    `_out[page]` says whether a page is with a caller, `_more[page]` with how many more than one."""
 
     def __init__(self, num_blocks: int):
         if num_blocks < 1:
@@ -27,6 +27,7 @@ class BlockAllocator:
         self.num_blocks = int(num_blocks)
         self._stack = list(reversed(range(self.num_blocks)))    # page 0 leaves first
         self._out = bytearray(self.num_blocks)
+        self._more: dict[int, int] = {}
 
     @property
     def num_free(self) -> int:
@@ -54,11 +55,25 @@ class BlockAllocator:
     def is_held(self, block: int) -> bool:
         return 0 <= block < self.num_blocks and bool(self._out[block])
 
+    def holders(self, block: int) -> int:
+        return 1 + self._more.get(block, 0) if self.is_held(block) else 0
+
+    def share(self, block: int) -> None:
+        """One more table holds the page."""
+        if not self.is_held(block):
+            raise ValueError(f"block {block} is not allocated: it cannot be shared")
+        self._more[block] = self._more.get(block, 0) + 1
+
     def free(self, block: int) -> None:
         if not 0 <= block < self.num_blocks:
             raise ValueError(f"block {block} is outside a pool of {self.num_blocks}")
         if not self._out[block]:
             raise ValueError(f"block {block} is not allocated (freed twice?)")
+        if block in self._more:                  # others still hold it
+            self._more[block] -= 1
+            if not self._more[block]:
+                del self._more[block]
+            return
         self._out[block] = 0
         self._stack.append(block)
 

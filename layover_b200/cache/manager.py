@@ -20,6 +20,10 @@ State groups own `[slots + 1, *shape]`; a request's slot is zeroed when it is op
 A group whose values are the leading channels of its keys (`values_in_keys`) has one store, not two.
 A mixer made of several mixers names several needs (a tuple); its view is a composite of their views.
 
+A request can be *forked* (`fork`): its full pages are shared, which nobody writes any more, and the page that is
+still being written, the state and the record are copied on the device. After a step over drafted tokens `accept`
+moves the rows of those that are kept to the places behind what the request holds and gives back the pages behind them.
+
 Beside the mixers' state every request has one *record* of `record_words` int32 words on the
 device, `records[slot]`, written whole when the request is opened and never touched by the host
 again: kernels index it by the request's slot, so a captured CUDA graph sees a fixed address.
@@ -345,6 +349,105 @@ class CacheManager:
 
     release = close
 
+    # ------------------------------------------------------------------ several hypotheses of a request
+    def _need_kernels(self) -> None:
+        if self.device is not None and self.device.type != "cuda":
+            from .. import ops
+            raise ops.KernelError("rows of a cache are moved on a CUDA device: there is no CPU path")
+
+    def _paged_pools(self, group: PagedGroup) -> list[torch.Tensor]:
+        """A group's pools as [planes, pages, kv_heads, page_tokens, channels]."""
+        return [p.flatten(0, 1) if p.dim() == 6 else p for p in (group.pool, group.k_store, group.v_store) if p is not None]
+
+    def fork(self, forks: list[tuple[SequenceCache, str]]) -> list[SequenceCache]:
+        """A new request for each (live request, new request id), holding the same tokens: all of them, or (OutOfBlocks) none. Pages
+        that hold nothing but those tokens are shared; the page that is still being written, the state slot and the record are
+        copied, in one launch a pool whatever the number of forks. Pages behind the held tokens are not taken over."""
+        from .. import ops
+
+        self._need_kernels()
+        ids = [request_id for _, request_id in forks]
+        if len(set(ids)) != len(ids) or any(i in self.live for i in ids):
+            raise ValueError("a forked request needs an id of its own")
+        for seq, _ in forks:
+            if seq.closed or self.live.get(seq.request_id) is not seq:
+                raise ValueError(f"request {seq.request_id!r} is closed or does not belong to this cache")
+        open_page = [seq.num_tokens // self.block_tokens if seq.num_tokens % self.block_tokens else None for seq, _ in forks]
+        for g, group in enumerate(self.paged):
+            wanted = sum(at is not None and seq.tables[g].blocks[at] != group.scratch_page for (seq, _), at in zip(forks, open_page))
+            if wanted > group.allocator.num_free:
+                raise OutOfBlocks(f"forking needs {wanted} blocks, {group.allocator.num_free} free")
+        if len(forks) > self._slots.num_free:
+            raise OutOfBlocks(f"forking needs {len(forks)} request slots, {self._slots.num_free} free")
+        made, copies = [], [[] for _ in self.paged]
+        for (seq, request_id), at in zip(forks, open_page):
+            child = SequenceCache(request_id, self._slots.alloc(1)[0], [], seq.num_tokens)
+            for g, group in enumerate(self.paged):
+                source = seq.tables[g]
+                blocks = source.blocks[: self.blocks_for(seq.num_tokens)]
+                for index, block in enumerate(blocks):
+                    if block == group.scratch_page:
+                        continue
+                    if index == at:
+                        blocks[index] = group.allocator.alloc(1)[0]
+                        copies[g].append((block, blocks[index]))
+                    else:
+                        group.allocator.share(block)
+                child.tables.append(BlockTable(blocks, min(source.first_live, len(blocks)), sum(b == group.scratch_page for b in blocks)))
+            self.live[request_id] = child
+            made.append(child)
+        if self.device is not None and forks:
+            for group, pairs in zip(self.paged, copies):
+                if pairs:
+                    src, dst = torch.tensor(pairs, dtype=torch.int32).T.contiguous().to(self.device)
+                    for pool in self._paged_pools(group):
+                        ops.copy_pages(pool, src, dst)
+            src, dst = torch.tensor([[seq.slot, child.slot] for (seq, _), child in zip(forks, made)], dtype=torch.int32).T.contiguous().to(self.device)
+            for group in self.states:
+                ops.copy_pages(group.pool, src, dst)
+            ops.copy_pages(self.records.unsqueeze(0), src, dst)
+        return made
+
+    def accept(self, accepted: list[tuple[SequenceCache, list[int]]]) -> None:
+        """After a step over drafted tokens: each request keeps the drafts listed (rising places among its drafts, a path down their
+        tree). Their rows move to the places right behind what the request holds, in all layers; they are counted, and the pages
+        behind them given back."""
+        from .. import ops
+
+        self._need_kernels()
+        seen = set()
+        for seq, path in accepted:
+            if seq.closed or self.live.get(seq.request_id) is not seq or seq.request_id in seen:
+                raise ValueError(f"request {seq.request_id!r} is closed, listed twice or does not belong to this cache")
+            seen.add(seq.request_id)
+            room = min((len(t.blocks) for t in seq.tables), default=0) * self.block_tokens - seq.num_tokens
+            if any(b <= a for a, b in zip([-1, *path], path)) or (path and path[-1] >= room):
+                raise ValueError(f"request {seq.request_id!r}: accepted drafts rise and lie in its pages, got {path} with room for {room}")
+        if self.device is not None and any(place != node for _, path in accepted for place, node in enumerate(path)):
+            cu = [0]
+            for _, path in accepted:
+                cu.append(cu[-1] + len(path))
+            lists = [[seq.num_tokens for seq, _ in accepted], [node for _, path in accepted for node in path], cu]
+            for g, group in enumerate(self.paged):
+                width = max(len(seq.tables[g].blocks) for seq, _ in accepted)
+                rows = [seq.tables[g].blocks + [group.scratch_page] * (width - len(seq.tables[g].blocks)) for seq, _ in accepted]
+                sizes = [len(accepted) * width, *(len(x) for x in lists)]
+                flat = torch.tensor([b for row in rows for b in row] + [x for part in lists for x in part], dtype=torch.int32).to(self.device)
+                table, first, picked, ends = flat.split(sizes)
+                for pool in self._paged_pools(group):
+                    ops.compact_tokens(pool, table.view(len(accepted), width), first, picked, ends)
+        for seq, path in accepted:
+            self.commit(seq, seq.num_tokens + len(path))
+            keep = self.blocks_for(seq.num_tokens)
+            for group, table in zip(self.paged, seq.tables):
+                for block in table.blocks[keep:]:
+                    if block != group.scratch_page:
+                        group.allocator.free(block)
+                    else:
+                        table.given_back -= 1
+                del table.blocks[keep:]
+                table.first_live = min(table.first_live, len(table.blocks))
+
     # ------------------------------------------------------------------ checks
     def check_tables(self, seq: SequenceCache, tokens: int | None = None) -> None:
         """What a kernel cannot check for itself, before every launch (layover/kv/paged_cache.py:160-165):
@@ -387,10 +490,11 @@ class CacheManager:
         for index, group in enumerate(self.paged):
             group.allocator.check()
             held = [b for seq in self.live.values() for b in seq.tables[index].blocks if b != group.scratch_page]
-            if len(held) != len(set(held)):
-                raise AssertionError("a page is held by two tables")
-            if len(held) != group.allocator.num_used:
-                raise AssertionError(f"{group.allocator.num_used} pages are out, {len(held)} are in tables")
+            for block in set(held):
+                if held.count(block) != max(1, group.allocator.holders(block)):
+                    raise AssertionError("a page is held by two tables")
+            if len(set(held)) != group.allocator.num_used:
+                raise AssertionError(f"{group.allocator.num_used} pages are out, {len(set(held))} are in tables")
             for block in held:
                 if not group.allocator.is_held(block):
                     raise AssertionError(f"page {block} is in a table and on the free list")

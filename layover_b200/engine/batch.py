@@ -11,6 +11,8 @@ side; the tokens of all entries are laid end to end:
   logit_rows [R]                      flat rows whose logits are returned, in entry / want order
   row_slots [R]                       the state slot of the request that each of those rows belongs to
   token_src [T]                       state slot whose record holds the token (still on the device), or -1
+  tree [T, words]                     only where an entry brings drafts (`StepEntry.parents`): bit j of a row says whether the
+                                      token sees token j of its own entry; positions are then those of the tree's levels
   per paged cache group:
     block_table [S, W]                page ids, padded with the group's scratch page
     slot_map [T]                      page * page_tokens + slot where the token's K and V go
@@ -45,6 +47,20 @@ class StepEntry:
     seq: SequenceCache
     tokens: list[int]
     want: list[int] = field(default_factory=list)
+    # drafted tokens that form a tree: the place of each token's parent among them, before its own (-1: the request's last held
+    # token). The step computes them and does not count them: `CacheManager.accept` does, for those that are kept
+    parents: list[int] | None = None
+
+
+def tree_rows(parents: list[int]) -> tuple[list[int], list[int]]:
+    """(what each token of a tree sees of it, as the bits of an integer; its level) from the tokens' parents."""
+    seen, level = [], []
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"token {i} of a tree has parent {p}: it must come before it, or be -1")
+        seen.append((seen[p] if p >= 0 else 0) | 1 << i)
+        level.append(level[p] + 1 if p >= 0 else 0)
+    return seen, level
 
 
 @dataclass
@@ -98,6 +114,7 @@ class StepBatch:
     # is to plan for them (a captured step: of the class of steps it is captured for)
     plan_max_ctx: int = 0
     plan_mean_ctx: int = 0
+    tree: torch.Tensor | None = None     # int32 [T, words]: what each token sees of its own entry (drafts), or None: all before it
     shared: dict = field(default_factory=dict)   # what parts make once per step and share (rotary tables)
 
 
@@ -193,6 +210,16 @@ class BatchBuilder:
             tiles = [(s, q0) for s, n in enumerate(q_lens) for q0 in range(0, n, size)]
             tile_lists[size] = tiles
             layout.add(f"tile_seq{size}", len(tiles)); layout.add(f"tile_q0{size}", len(tiles))
+        drafts, words = any(e.parents is not None for e in entries), 0
+        if drafts:
+            if capacity:
+                raise ValueError("drafted tokens do not fit a batch of fixed capacity")
+            for e in entries:
+                if e.parents is not None and len(e.parents) != len(e.tokens):
+                    raise ValueError(f"request {e.seq.request_id!r}: a parent per drafted token")
+            trees = [tree_rows(e.parents if e.parents is not None else list(range(-1, len(e.tokens) - 1))) for e in entries]
+            words = -(-max(q_lens) // 32)
+            layout.add("tree", n_tokens, words)
         singles = [s for s, n in enumerate(q_lens) if n == 1]
         mixed = 0 < len(singles) < n_seqs
         portion_lists = {}
@@ -224,6 +251,12 @@ class BatchBuilder:
             view[ids_at + at: ids_at + at + n] = entry.tokens
             view[pos_at + at: pos_at + at + n] = np.arange(starts[index], starts[index] + n, dtype=np.int32)
             view[src_at + at: src_at + at + n] = -1
+            if drafts:
+                seen, level = trees[index]
+                view[pos_at + at: pos_at + at + n] = np.array(level, dtype=np.int32) + starts[index]
+                where = layout.fields["tree"][0] + at * words
+                rows_of = np.frombuffer(b"".join(s.to_bytes(4 * words, "little") for s in seen), dtype=np.int32)
+                view[where: where + n * words] = rows_of
             if n == 1 and entry.tokens[0] < 0:          # the request's newest token is in its record on the device
                 view[ids_at + at] = 0
                 view[src_at + at] = entry.seq.slot
@@ -311,6 +344,7 @@ class BatchBuilder:
             all_decode=max(q_lens) == 1, real_seqs=real,
             plan_max_ctx=plan_ctx[0] if plan_ctx else max((ctx_lens[s] for s in singles), default=0),
             plan_mean_ctx=plan_ctx[1] if plan_ctx else (sum(ctx_lens[s] for s in singles) // len(singles) if singles else 0),
+            tree=get("tree") if drafts else None,
         )
 
     @staticmethod

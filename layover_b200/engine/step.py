@@ -16,6 +16,10 @@ captures batch 1, 2, 4, 8 the same way, layover/decode_graphs.py:25-100). The wi
 request's pages rounded up to a power of two, so the attention's split count is planned for about
 the context that is really there, not for the longest a request could ever get.
 
+An entry may bring drafted tokens that form a tree (`StepEntry.parents`): the step computes the logits wanted of
+them, each seeing what the request holds and its own ancestors, and leaves it to `CacheManager.accept` which of them
+the request keeps (the reference has no drafts).
+
 A step that is one prompt portion of a size named in `portion_graph_tokens` (the scheduler's
 prefill chunk) replays a graph too, one per (size, width bucket, last token's logits wanted or
 not): a portion is a few hundred launches, and the first short ones (embedding, norms, rotation)
@@ -119,6 +123,8 @@ class StepFunction:
                 raise ValueError(f"request {seq.request_id!r}: state slot {seq.slot} is outside the cache")
             if seq.num_tokens + len(entry.tokens) > self.max_position:
                 raise ValueError(f"request {seq.request_id!r} would exceed {self.max_position} positions")
+            if entry.parents is not None and not self.model.takes_drafts:
+                raise ValueError(f"request {seq.request_id!r}: this model's mixers have no form for a tree of drafts")
             low, high = min(entry.tokens), max(entry.tokens)
             if low == DEVICE_TOKEN and len(entry.tokens) == 1:
                 continue
@@ -155,9 +161,12 @@ class StepFunction:
 
     def _step(self, entries: list[StepEntry], sampled: bool):
         self._check(entries)
+        drafts = any(e.parents is not None for e in entries)
+        if drafts and sampled:
+            raise ValueError("drafted tokens are checked against their logits, not sampled")
         self._reserve(entries)
         with profiling.nvtx_range("step"):
-            graph = self._graph_for(entries, sampled)
+            graph = None if drafts else self._graph_for(entries, sampled)
             if graph is not None:
                 batch = self.builder.build(entries, graph.capacity, graph.buffer, graph.plan_ctx)
                 if self.replay_graphs:
@@ -182,7 +191,8 @@ class StepFunction:
                 if sampled:
                     out = self.sampler.launch(out, batch)
         for entry in entries:
-            self.cache.commit(entry.seq, entry.seq.num_tokens + len(entry.tokens))
+            if entry.parents is None:       # drafts are counted when they are accepted
+                self.cache.commit(entry.seq, entry.seq.num_tokens + len(entry.tokens))
         self.steps += 1
         return out
 

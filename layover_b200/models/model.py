@@ -102,6 +102,13 @@ class Model:
             names += part.kernel_libraries(dtype)
         return tuple(dict.fromkeys(names))
 
+    @property
+    def takes_drafts(self) -> bool:
+        """Whether a step may bring drafted tokens that form a tree: every mixer attends, without further options."""
+        from ..parts.attention import Attention
+
+        return all(isinstance(getattr(block, "mixer", None), Attention) and not block.mixer.general for block in self.blocks)
+
     def tile_sizes(self) -> tuple[int, ...]:
         """Query-tile sizes that the parts want listed in every batch."""
         sizes = [size for part in self.all_parts() for size in part.tile_sizes(self.runtime.dtype)]

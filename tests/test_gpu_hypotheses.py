@@ -428,3 +428,158 @@ def test_captured_and_on_another_stream():
 def test_the_same_call_gives_the_same_bits():
     case = Trees([(2000, 9), (77, 3)], 8, 2, 128, seed=2).fill()
     assert torch.equal(case.run(), case.run())
+
+
+# ------------------------------------------------------------------------------- as they are used
+@pytest.fixture(scope="module", params=["fp32", "bf16"])
+def served(request, tiny_folders):
+    """A model with the head size of the served ones (tcgen05) and one of small heads, in either precision."""
+    import layover_b200 as lb
+    return {name: lb.load_model(str(tiny_folders[name][0]), device="cuda", dtype=request.param) for name in ("a", "c")}
+
+
+def fresh(model, blocks=200, page=8):
+    import layover_b200 as lb
+    from layover_b200.engine.step import StepFunction
+    cache = lb.PagedKVCache(model, blocks, block_tokens=page, max_requests=24)
+    return cache, StepFunction(model, cache)
+
+
+def feed(cache, step, name, tokens):
+    """A request that holds `tokens`, fed as one portion; the logits of its last."""
+    import layover_b200 as lb
+    seq = cache.open(name)
+    return seq, step([lb.StepEntry(seq, list(tokens), [len(tokens) - 1])]).clone()[0]
+
+
+@pytest.mark.parametrize("name", ["a", "c"])
+def test_a_step_over_drafts_and_what_follows_it(served, name):
+    """Every draft's logits are those of its own branch fed as a request of its own; after some are accepted the request goes on as if it
+    had been fed them; a second request's portion shares the step."""
+    import layover_b200 as lb
+    from conftest import random_prompt, tolerance
+    model = served[name]
+    cache, step = fresh(model)
+    vocab = model.spec.vocab_size
+    prompt, tokens = random_prompt(vocab, 45, 1), random_prompt(vocab, 9, 2)
+    parents, other = [-1, 0, 0, 1, 1, 2, -1, 4, 7], random_prompt(vocab, 13, 3)
+    seq, _ = feed(cache, step, "x", prompt)
+    beside = cache.open("y")
+    logits = step([lb.StepEntry(seq, tokens, list(range(9)), parents), lb.StepEntry(beside, other, [12])]).clone()
+    assert seq.num_tokens == 45 and beside.num_tokens == 13
+    branch = [[t] if p < 0 else None for t, p in zip(tokens, parents)]
+    for i, p in enumerate(parents):
+        branch[i] = branch[i] or branch[p] + [tokens[i]]
+    for i in range(9):
+        one, want = feed(cache, step, f"branch {i}", prompt + branch[i])
+        assert (logits[i] - want).abs().max().item() <= tolerance(want, model.dtype)
+        cache.close(one)
+    _, want = feed(cache, step, "alone", other)
+    assert (logits[9] - want).abs().max().item() <= tolerance(want, model.dtype)
+    path = [0, 1, 4, 7, 8]
+    cache.accept([(seq, path)])
+    cache.check()
+    assert seq.num_tokens == 50
+    got = step([lb.StepEntry(seq, [3], [0])])[0].clone()
+    _, want = feed(cache, step, "path", prompt + [tokens[i] for i in path] + [3])
+    assert (got - want).abs().max().item() <= tolerance(want, model.dtype)
+    assert ops().attention_tree_status() == 0
+
+
+@pytest.mark.parametrize("name", ["a", "c"])
+def test_forked_requests_go_their_own_ways(served, name):
+    import layover_b200 as lb
+    from conftest import random_prompt, tolerance
+    model = served[name]
+    cache, step = fresh(model)
+    prompt = random_prompt(model.spec.vocab_size, 43, 5)
+    seq, _ = feed(cache, step, "x", prompt)
+    children = cache.fork([(seq, "b"), (seq, "c")])
+    logits = step([lb.StepEntry(s, [t], [0]) for s, t in zip((seq, *children), (1, 2, 3))]).clone()
+    cache.close(seq)
+    for row, child, token in zip(logits[1:], children, (2, 3)):
+        _, want = feed(cache, step, f"plain {token}", prompt + [token])
+        assert (row - want).abs().max().item() <= tolerance(want, model.dtype)
+        got = step([lb.StepEntry(child, [9, 8, 7], [2])])[0].clone()
+        _, want = feed(cache, step, f"longer {token}", prompt + [token, 9, 8, 7])
+        assert (got - want).abs().max().item() <= tolerance(want, model.dtype)
+    cache.check()
+
+
+def test_forks_copy_states_and_records(tmp_path):
+    import layover_b200 as lb
+    from layover_b200.engine.step import StepFunction
+    model = lb.random_model(lb.preset("topidra-tiny"), seed=0, device="cuda", dtype="fp32")
+    cache = lb.PagedKVCache(model, 100, block_tokens=8, max_requests=6)
+    step = StepFunction(model, cache)
+    prompt = [int(t) for t in torch.randint(0, model.spec.vocab_size, (29,), generator=torch.Generator().manual_seed(1))]
+    seq, _ = feed(cache, step, "x", prompt)
+    cache.records[seq.slot] = torch.arange(cache.record_words, dtype=torch.int32, device="cuda")
+    (child,) = cache.fork([(seq, "y")])
+    assert torch.equal(cache.records[child.slot], cache.records[seq.slot])
+    for group in cache.states:
+        assert torch.equal(group.pool[:, child.slot], group.pool[:, seq.slot])
+    first, second = step([lb.StepEntry(seq, [4], [0]), lb.StepEntry(child, [4], [0])])
+    assert torch.equal(first, second)
+    with pytest.raises(ValueError, match="no form for a tree"):
+        step([lb.StepEntry(seq, [1, 2], [0], [-1, -1])])
+    cache.check()
+
+
+@pytest.mark.parametrize("name", ["a", "c"])
+def test_generation_with_drafts_is_greedy_generation(served, name):
+    """Each token is the greedy choice after those before it, within the logits' tolerance; a text that repeats itself takes fewer steps."""
+    import layover_b200 as lb
+    from conftest import tolerance
+    model = served[name]
+    prompts = [[7, 8, 9, 10, 7, 8, 9, 10, 7, 8], [5, 6], [3]]
+    out, counts = lb.generate_with_drafts(model, prompts, 40, lb.LookupDrafts(2, 5, 1), block_tokens=8, prefill_chunk=4)
+    assert [len(o) for o in out] == [40, 40, 40] and counts["drafted"] >= counts["accepted"]
+    cache, step = fresh(model)
+    for i, (prompt, tokens) in enumerate(zip(prompts, out)):
+        text = prompt + tokens
+        seq = cache.open(f"{i}")
+        logits = step([lb.StepEntry(seq, text, list(range(len(prompt) - 1, len(text) - 1)))])
+        chosen = logits.gather(1, torch.tensor(tokens, device="cuda")[:, None])[:, 0]
+        assert (logits.amax(1) - chosen).max().item() <= 2 * tolerance(logits, model.dtype)
+    stop = out[0][5]
+    again, _ = lb.generate_with_drafts(model, prompts[:1], 40, lb.LookupDrafts(2, 5, 1), stop_tokens={stop}, block_tokens=8, prefill_chunk=4)
+    assert again[0] == out[0][: out[0].index(stop) + 1]
+
+
+def test_beam_search_finds_the_best_beams(tiny_folders):
+    """Against a search that feeds every beam's whole text anew: the same texts where their sums are apart, the same sums."""
+    import layover_b200 as lb
+    from conftest import random_prompt
+    model = lb.load_model(str(tiny_folders["a"][0]), device="cuda", dtype="fp32")
+    prompts, beams, new = [random_prompt(256, 11, 1), random_prompt(256, 1, 2), random_prompt(256, 24, 3)], 3, 7
+    found = lb.beam_search(model, prompts, beams, new, block_tokens=4, prefill_chunk=8)
+    cache, step = fresh(model, 800, 4)
+    for r, prompt in enumerate(prompts):
+        held = [(0.0, [])]
+        for _ in range(new):
+            rows = []
+            for score, tokens in held:
+                seq, logits = feed(cache, step, "t", prompt + tokens)
+                cache.close(seq)
+                rows += [(score + float(p), tokens + [t]) for t, p in enumerate(torch.log_softmax(logits.double(), 0).tolist())]
+            held = sorted(rows, key=lambda x: -x[0])[:beams]
+        assert [round(s, 3) for s, _ in found[r]] == pytest.approx([round(s, 3) for s, _ in held], abs=2e-3)
+        for (score, tokens), (want, text) in zip(found[r], held):
+            assert tokens == text or min(abs(want - s) for s, t in held if t != text) < 1e-3
+    stop = found[0][0][1][2]
+    stopped = lb.beam_search(model, prompts[:1], beams, new, stop_tokens={stop}, block_tokens=4)
+    assert any(tokens[-1] == stop for _, tokens in stopped[0]) and all(stop not in tokens[:-1] for _, tokens in stopped[0])
+
+
+def test_command_line_follows_beams_and_checks_drafts(capsys):
+    import json
+    from layover_b200.__main__ import main
+    base = ["--preset", "tiny-b", "--random-weights", "--dtype", "fp32", "--prompt-lens", "9,20", "--max-new-tokens", "6"]
+    assert main(base + ["--beams", "3"]) == 0
+    beams = json.loads(capsys.readouterr().out)
+    assert [len(b) for b in beams["generated"]] == [3, 3] and all(len(t) == 6 for b in beams["generated"] for t in b)
+    assert main(base + ["--drafts", "4"]) == 0
+    assert [len(t) for t in json.loads(capsys.readouterr().out)["generated"]] == [6, 6]
+    with pytest.raises(SystemExit):
+        main(base + ["--drafts", "4", "--beams", "2"])

@@ -17,7 +17,7 @@
 // than one chunk each leaves its maxima, sums and unnormalised outputs in scratch memory of this call, and a second kernel joins them.
 //
 //   attention_tree_mma_kernel   bfloat16, mma.sync m16n8k16: RG groups of 16 rows, the four warps share a tile's 64 keys
-//   attention_tree_f32_kernel   float32, FFMA: 8 x 16 threads, RT / 8 rows and 4 keys (dim / 16 channels) each
+//   attention_tree_f32_kernel   float32, FFMA: 8 x 16 threads, RT / 8 rows and 2 keys (dim / 16 channels) each
 //
 // The values of a draft may be anything (a draft whose arithmetic overflowed): what a row does not see must not reach it, and
 // 0 x NaN is NaN. So in tiles that hold drafts, value rows that are not finite are taken out of the product and added one by
@@ -51,8 +51,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Keys [tile * 64, + 64) of one head into rows of `stride` elements of T; what lies outside [key_lo, ctx) becomes zeros.
-template <typename T>
+// Keys [tile * KEYS, + KEYS) of one head into rows of `stride` elements of T; what lies outside [key_lo, ctx) becomes zeros.
+template <int KEYS, typename T>
 __device__ __forceinline__ void load_tile(T* to, const T* __restrict__ pool, const TreeArgs& a, const Unit& u, const int* table, int tile, int stride) {
   constexpr int PER = 16 / (int)sizeof(T);
   const int pieces = a.dim / PER;
@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
     }
   }
   if (u.tile_begin < u.tile_end) {
-    load_tile(k_s, k_pool, a, u, table, u.tile_begin, stride);
-    load_tile(v_s, v_pool, a, u, table, u.tile_begin, stride);
+    load_tile<KEYS>(k_s, k_pool, a, u, table, u.tile_begin, stride);
+    load_tile<KEYS>(v_s, v_pool, a, u, table, u.tile_begin, stride);
   }
   cp_async_commit();
 
@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
   for (int tile = u.tile_begin; tile < u.tile_end; ++tile) {
     const int buf = (tile - u.tile_begin) & 1;
     if (tile + 1 < u.tile_end) {
-      load_tile(k_s + (buf ^ 1) * KEYS * stride, k_pool, a, u, table, tile + 1, stride);
-      load_tile(v_s + (buf ^ 1) * KEYS * stride, v_pool, a, u, table, tile + 1, stride);
+      load_tile<KEYS>(k_s + (buf ^ 1) * KEYS * stride, k_pool, a, u, table, tile + 1, stride);
+      load_tile<KEYS>(v_s + (buf ^ 1) * KEYS * stride, v_pool, a, u, table, tile + 1, stride);
       cp_async_commit();
       cp_async_wait<1>();
     } else {
@@ -338,10 +338,13 @@ __device__ __forceinline__ void fma2(float2& x, float2 a, float2 b) {
       : "+f"(x.x), "+f"(x.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
 }
 
+constexpr int F32_KEYS = 32;    // keys per tile: four blocks an SM have room for theirs
+static_assert(F32_KEYS * 4 == THREADS, "four threads a value row");
+
 // MAX_C: blocks of 64 channels of a head
 template <int RT, int MAX_C>
-__global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 2 : 1) attention_tree_f32_kernel(const TreeArgs a) {
-  constexpr int RPT = RT / 8;                              // rows of a thread
+__global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f32_kernel(const TreeArgs a) {
+  constexpr int RPT = RT / 8, KEYS = F32_KEYS, KPT = KEYS / 16;      // rows and keys of a thread
   extern __shared__ __align__(16) float smem_f[];
   __shared__ unsigned bad_rows[4];
   const int stride = a.dim + 4;                            // rows 16 bytes apart modulo 128: eight rows' pieces lie in different banks
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 2 : 1) attention_tree_f3
       cp_async16(q_s + r * stride + c * 4, q + at, live ? 16 : 0);
     }
   }
-  if (u.tile_begin < u.tile_end) load_tile(k_s, k_pool, a, u, table, u.tile_begin, stride);
+  if (u.tile_begin < u.tile_end) load_tile<KEYS>(k_s, k_pool, a, u, table, u.tile_begin, stride);
   cp_async_commit();
 
   const int* bits[RPT];
@@ -388,43 +391,45 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 2 : 1) attention_tree_f3
     for (int c = 0; c < MAX_C; ++c) o[i][c][0] = o[i][c][1] = make_float2(0.f, 0.f);
   }
   for (int tile = u.tile_begin; tile < u.tile_end; ++tile) {
-    load_tile(v_s, v_pool, a, u, table, tile, stride);
+    load_tile<KEYS>(v_s, v_pool, a, u, table, tile, stride);
     cp_async_commit();
     cp_async_wait<1>();                                    // the keys; the values come under the first product
     __syncthreads();
     const int key0 = tile * KEYS;
     const bool drafts = key0 + KEYS > u.held;
-    float2 pairs[RPT][4];                                  // sums over the even and over the odd channels
+    float2 pairs[RPT][KPT];                                  // sums over the even and over the odd channels
 #pragma unroll
     for (int i = 0; i < RPT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) pairs[i][j] = make_float2(0.f, 0.f);
+      for (int j = 0; j < KPT; ++j) pairs[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
     for (int d = 0; d < a.dim; d += 4) {
-      float4 kv[4];
+      float4 kv[KPT];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kv[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * stride + d);
+      for (int j = 0; j < KPT; ++j) kv[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * stride + d);
+      float4 qv[RPT];
 #pragma unroll
-      for (int i = 0; i < RPT; ++i) {
-        const float4 qv = *reinterpret_cast<const float4*>(q_s + (ty + 8 * i) * stride + d);
+      for (int i = 0; i < RPT; ++i) qv[i] = *reinterpret_cast<const float4*>(q_s + (ty + 8 * i) * stride + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          fma2(pairs[i][j], make_float2(qv.x, qv.y), make_float2(kv[j].x, kv[j].y));
-          fma2(pairs[i][j], make_float2(qv.z, qv.w), make_float2(kv[j].z, kv[j].w));
-        }
-      }
+      for (int i = 0; i < RPT; ++i)                        // a sum's two products stand apart: one waits for the other
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) fma2(pairs[i][j], make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y));
+#pragma unroll
+      for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) fma2(pairs[i][j], make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w));
     }
-    float s[RPT][4];
+    float s[RPT][KPT];
 #pragma unroll
     for (int i = 0; i < RPT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = pairs[i][j].x + pairs[i][j].y;
+      for (int j = 0; j < KPT; ++j) s[i][j] = pairs[i][j].x + pairs[i][j].y;
     const bool masked = drafts || key0 < u.key_lo || a.window > 0;
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < KPT; ++j) {
         const int key = key0 + tx + 16 * j;
         if (a.cap_in != 0.f) s[i][j] = a.cap_out * tanhf(s[i][j] / a.cap_out);
         if (masked && (key >= u.ctx || !sees(a, bits[i], key, u.held, oldest[i]))) s[i][j] = -INFINITY;
@@ -438,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 2 : 1) attention_tree_f3
       m_run[i] = top;
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < KPT; ++j) {
         const float w = exp2f((s[i][j] - shift) * a.scale_log2);      // the difference first: a product of the maximum would round with its size
         p_s[(ty + 8 * i) * P_STRIDE + tx + 16 * j] = w;
         sum += w;
@@ -451,12 +456,12 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 2 : 1) attention_tree_f3
     }
     cp_async_wait<0>();
     __syncthreads();                                       // values and weights are there, the keys are done with
-    if (tile + 1 < u.tile_end) load_tile(k_s, k_pool, a, u, table, tile + 1, stride);
+    if (tile + 1 < u.tile_end) load_tile<KEYS>(k_s, k_pool, a, u, table, tile + 1, stride);
     cp_async_commit();
     if (drafts) {
-      const float* row = v_s + (threadIdx.x >> 1) * stride;
+      const float* row = v_s + (threadIdx.x >> 2) * stride;                  // four threads look at a value row
       bool bad = false;
-      for (int c = threadIdx.x & 1; c < a.dim >> 2; c += 2) {
+      for (int c = threadIdx.x & 3; c < a.dim >> 2; c += 4) {
         const float4 w = *reinterpret_cast<const float4*>(row + c * 4);
         bad |= !isfinite(w.x) || !isfinite(w.y) || !isfinite(w.z) || !isfinite(w.w);
       }
@@ -473,10 +478,10 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 2 : 1) attention_tree_f3
         for (int i = 0; i < RPT; ++i) w[i] = *reinterpret_cast<const float4*>(p_s + (ty + 8 * i) * P_STRIDE + key);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool bad = some_bad && (bad_rows[(key + e) >> 4] >> (2 * ((key + e) & 15)) & 3u);
+          const bool bad = some_bad && (bad_rows[(key + e) >> 3] >> (4 * ((key + e) & 7)) & 15u);
 #pragma unroll
           for (int c = 0; c < MAX_C; ++c) {
-            if (64 * c + 4 * tx >= a.dim) break;
+            if (64 * c >= a.dim) break;                    // sums behind the last channel are of what lies there, and are not stored
             const float4 v = *reinterpret_cast<const float4*>(v_s + (key + e) * stride + 64 * c + 4 * tx);
 #pragma unroll
             for (int i = 0; i < RPT; ++i) {
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_join_kernel(const Tree
   pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.y / a.row_tiles, row_tile = blockIdx.y - seq * a.row_tiles;
-  const Unit u = find_unit<KEYS>(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks);
+  const Unit u = find_unit<sizeof(T) == 4 ? F32_KEYS : KEYS>(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks);
   const int local = blockIdx.z * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (local >= u.rows || u.chunks <= 1) return;
   const int group = a.q_heads / a.kv_heads, row = u.row0 + local, head = u.head * group + row % group;
@@ -577,6 +582,7 @@ int launch_mma(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
 }
 template <int RT, int MAX_C>
 int launch_f32_of(const TreeArgs& a, dim3 grid, cudaStream_t stream) {
+  constexpr int KEYS = F32_KEYS;
   const size_t smem = ((size_t)(RT + 2 * KEYS) * (a.dim + 4) + RT * (KEYS + 4)) * sizeof(float);
   static LbPerDeviceOnce once;
   if (!once.run(LB_ALLOW_SMEM((attention_tree_f32_kernel<RT, MAX_C>), ((RT + 2 * KEYS) * (64 * MAX_C + 4) + RT * (KEYS + 4)) * sizeof(float)))) return lb_last_error();
@@ -598,7 +604,7 @@ static int check_tree(int dtype, const void* q, const void* k_pool, const void* 
   return 0;
 }
 
-// `tile_rows`: rows of a block (16, 32 or, in bfloat16, 64). `chunks` blocks of `chunk_tiles` tiles of 64 keys share a row tile's keys (the last takes
+// `tile_rows`: rows of a block (16, 32 or, in bfloat16, 64). `chunks` blocks of `chunk_tiles` tiles of 64 keys (float32: of 32) share a row tile's keys (the last takes
 // what is left); with more than one, `partials` holds n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) floats.
 LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
                                 int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words, int tokens,

@@ -1304,17 +1304,17 @@ def attention_tree_on_tcgen05(group: int, dim: int, page_tokens: int, dtype: tor
 def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, dim: int, sms: int, wide: bool = False) -> tuple[int, int, int, int]:
     """(rows of a block, row tiles of a sequence, chunks, key tiles of a chunk) for the FFMA and mma.sync kernels of `attention_tree`: tiles
     of 32 rows, or 16 where there are no more (`wide`, bfloat16: of 64 where there are over 128), and as many chunks of the keys as give every SM
-    about four blocks. Measured (one B200, us): 4 requests of 900 keys, 52 rows in 32 bits with 16, 32 and 64 rows a tile 103, 74 and 91,
-    with one, two, three and five key tiles a chunk 81, 74, 95 and 84; 5 of 1,024 keys, 78 rows of 64 channels in bfloat16 16.3, 16.1 and
+    four blocks and no fifth (all run at once). Measured (one B200, us): 4 requests of 900 keys, 52 rows in 32 bits with 16 and 32 rows a tile
+    78 and 63, with two, three, four and five key tiles a chunk 64, 67, 63 and 71; 5 of 1,024 keys, 78 rows of 64 channels in bfloat16 16.3, 16.1 and
     17.1, with one, two and five 16.1, 16.8 and 24.1."""
     rows = max_nodes * (q_heads // kv_heads)
     tile_rows = 16 if rows <= 16 else 64 if wide and rows > 128 else 32
     row_tiles = -(-rows // tile_rows)
     keys = min(max_ctx, max_nodes + window) if window else max_ctx
-    tiles = -(-keys // 64) + (1 if window else 0)
+    tiles = -(-keys // (64 if wide else 32)) + (1 if window else 0)
     units = n_seqs * kv_heads * row_tiles
     most = max(1, _TREE_SCRATCH_FLOATS // (units * tile_rows * (dim + 2)))
-    chunks = max(1, min(-(-4 * sms // units), tiles, most, 65535))
+    chunks = max(1, min(4 * sms // units, tiles, most, 65535))
     chunk_tiles = -(-tiles // chunks)
     return tile_rows, row_tiles, -(-tiles // chunk_tiles), chunk_tiles
 

@@ -100,7 +100,8 @@ def test_tree_plan_covers_rows_and_keys(n_seqs, nodes, ctx, window, heads):
         tile_rows, row_tiles, chunks, chunk_tiles = ops.tree_plan(n_seqs, nodes, ctx, window, *heads, 148, wide)
         rows, keys = nodes * q_heads // kv_heads, min(ctx, nodes + window) if window else ctx
         assert (row_tiles - 1) * tile_rows < rows <= row_tiles * tile_rows
-        assert chunks * chunk_tiles * 64 >= keys and (chunks - 1) * chunk_tiles * 64 < keys + 128
+        tile = 64 if wide else 32
+        assert chunks * chunk_tiles * tile >= keys and (chunks - 1) * chunk_tiles * tile < keys + 2 * tile
         assert chunks == 1 or n_seqs * kv_heads * row_tiles * chunks * tile_rows * (dim + 2) <= 64 << 20
     blocks, rows2, floats = ops.tree_share(n_seqs, nodes, ctx, window, q_heads, kv_heads, 148)
     assert 1 <= blocks <= 148 and rows2 == (nodes > 128 // (q_heads // kv_heads)) and floats > 2 * blocks * 128 * 130

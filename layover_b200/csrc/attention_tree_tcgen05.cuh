@@ -4,8 +4,7 @@
 // an equal, contiguous share of the list: a few segments, each a row tile and a range of its keys. Blocks stay for the whole
 // launch, one an SM, so the loads of a segment run under the arithmetic and the stores of the one before. A row tile whose keys
 // lie in several blocks' shares leaves maxima, sums and unnormalised outputs in scratch memory, two places a block (its first and its last
-// segment), for
-// `join_kernel`.
+// segment), for `join_kernel`.
 //
 // A row tile holds 128 / group drafts with all their heads of the group, or, with ROWS2, twice as many. Two warpgroups of softmax
 // have scores and an output accumulator of their own in tensor memory: they take the key tiles in turn, or, with ROWS2, a half of
@@ -241,228 +240,228 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
   pdl_launch_dependents();
 
   if (warp < FIRST_SOFTMAX) {
-  give_registers<FEW_REGS>();
-  if (warp < LOADERS) {
-    pdl_wait();
-    if (warp == 0) {
-    // ---------------- the list's length, then the sequence in which this block's share begins
-    int total = 0;
-    for (int base = 0; base < a.n_seqs; base += 64) {
-      int first[2], end[2], ctx[2];                        // on their way at once
+    give_registers<FEW_REGS>();
+    if (warp < LOADERS) {
+      pdl_wait();
+      if (warp == 0) {
+        // ---------------- the list's length, then the sequence in which this block's share begins
+        int total = 0;
+        for (int base = 0; base < a.n_seqs; base += 64) {
+          int first[2], end[2], ctx[2];                        // on their way at once
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int seq = min(base + 32 * i + lane, a.n_seqs - 1);
-        first[i] = a.cu_q[seq]; end[i] = a.cu_q[seq + 1]; ctx[i] = a.ctx_len[seq];
-      }
-      int tiles = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int seq = base + 32 * i + lane;
-        if (seq < a.n_seqs) {
-          const Sequence s = find_sequence<ROWS2>(a, first[i], end[i], ctx[i]);
-          const int mine = a.kv_heads * s.row_tiles * s.tiles;
-          if (seq < SEQ_CACHE) known[seq] = make_int4(first[i], end[i], ctx[i], mine);
-          tiles += mine;
-        }
-      }
-      total += __reduce_add_sync(0xffffffffu, tiles);
-    }
-    const int blocks = min((int)gridDim.x, total), b = min((int)blockIdx.x, blocks);
-    const int from = b < blocks ? share_begin(total, b, blocks) : total, upto = b < blocks ? share_begin(total, b + 1, blocks) : total;
-    if (lane == 0) { start[0] = start[1] = 0; start[2] = upto - from; }
-    __syncwarp();
-    int before = 0;
-    for (int base = 0; base < a.n_seqs; base += 32) {
-      const int i = base + lane;
-      int tiles = 0;
-      if (i < a.n_seqs) {
-        if (i < SEQ_CACHE) {
-          tiles = known[i].w;
-        } else {
-          const Sequence s = find_sequence<ROWS2>(a, known, i);
-          tiles = a.kv_heads * s.row_tiles * s.tiles;
-        }
-      }
-      int sum = tiles;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int other = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += other;
-      }
-      const int mine = before + sum - tiles;
-      if (from >= mine && from < mine + tiles) { start[0] = i; start[1] = from - mine; }
-      before += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    if (lane == 0) start[3] = total;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(started);
-    } else {
-      ok = warp_wait(started, 0) || ran_out(1);
-    }
-    // ---------------- K or V, and the first of these warps the queries
-    const int n_tiles = ok ? start[2] : 0, values = warp >> 1, row0 = (warp & 1) * 64, page_shift = __ffs(a.page_tokens) - 1;
-    const bf16* pool = (const bf16*)(values ? a.v_pool : a.k_pool);
-    // a lane copies 16 bytes of rows 2 i + (lane >> 4) of each 8 of this warp's rows; `to` are their places in those 8, swizzled
-    const uint32_t ring_at = smem_u32(ring) + values * STAGES * TILE_BYTES + ((lane & 15) >> 3) * HALF_BYTES + row0 * 128;
-    uint32_t to[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) to[i] = (2 * i + (lane >> 4)) * 128 + (((lane & 7) ^ (2 * i + (lane >> 4))) << 4);
-    const long lane_from = (lane >> 4) * DIM + (lane & 15) * 8;
-    // Up to four tiles of a segment, whose pages are looked up together, four tiles ahead (a read from memory waits behind all copies
-    // in flight): lane 8 j + i has the page of rows 8 i .. of tile j.
-    struct Group { int page, key0, count, head, key_lo, ctx, draft; } now, soon;
-    Walk<ROWS2> ahead;
-    ahead.begin_at(a, known, start[0], start[1], n_tiles);
-    int tile = 0, segments = 0, taken = 0;
-    auto next_group = [&](Group& g) {
-      g.count = 0; g.draft = -1;
-      if (tile == ahead.count) {
-        if (!ahead.next(a)) return;
-        tile = 0;
-        g.draft = ahead.s.first + ahead.row_tile * (ROWS2 ? 2 : 1) * drafts_tile;      // a segment begins: its queries
-      }
-      g.count = min(4, ahead.count - tile); g.head = ahead.head; g.key0 = (ahead.s.tile_lo + ahead.begin + tile) * KEYS;
-      g.key_lo = ahead.s.key_lo; g.ctx = ahead.s.ctx;
-      const int key = g.key0 + (lane >> 3) * KEYS + row0 + (lane & 7) * 8, index = key >> page_shift;
-      g.page = index < a.table_width && key < g.ctx ? a.block_table[(size_t)ahead.seq * a.table_width + index] : -1;
-      tile += g.count;
-    };
-    next_group(now);
-    while (ok && now.count > 0) {
-      next_group(soon);
-      if (warp == 0 && now.draft >= 0) {
-        const int buf = ROWS2 ? 0 : segments & 1;
-        ok = warp_wait(&q_empty[buf], ((ROWS2 ? segments : segments >> 1) & 1) ^ 1) || ran_out(2);
-        if (!ok) break;
-        const uint32_t bar = smem_u32(&q_full[buf]);
-        expect_bytes(bar, (uint32_t)(drafts_tile * group * 128) * (ROWS2 ? 4 : 2));
-        const int head = warp_uniform(now.head * group), draft = warp_uniform(now.draft);
-        for (int part = 0; part < (ROWS2 ? 2 : 1); ++part)
-          for (int h = 0; h < 2; ++h)
-            load_queries(smem_u32(q_s) + (ROWS2 ? part : buf) * TILE_BYTES + h * HALF_BYTES, &q_map, bar, h * 64, head, draft + part * drafts_tile);
-        ++segments;
-      }
-      // the places in the pool of the rows that begin the eights; -1: the page is not there
-      const int first = (unsigned)now.page < (unsigned)a.n_pages
-                            ? (now.page * a.kv_heads + now.head) * a.page_tokens + ((row0 + (lane & 7) * 8) & (a.page_tokens - 1)) : -1;
-      const unsigned there = __ballot_sync(0xffffffffu, first >= 0);
-      for (int j = 0; j < now.count; ++j) {
-        const int stage = taken % STAGES, key0 = now.key0 + j * KEYS;
-        ok = warp_wait(&empty[values * STAGES + stage], ((taken / STAGES) & 1) ^ 1) || ran_out(1);
-        if (!ok || flag[0]) { ok = false; break; }
-        const uint32_t at = ring_at + stage * TILE_BYTES;
-        if ((there >> (8 * j) & 0xFFu) == 0xFFu && key0 >= now.key_lo && key0 + KEYS <= now.ctx) {
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const bf16* from = pool + (long)__shfl_sync(0xffffffffu, first, 8 * j + g) * DIM + lane_from;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) copy16(at + to[i] + g * 1024, from + 2 * i * DIM);
+          for (int i = 0; i < 2; ++i) {
+            const int seq = min(base + 32 * i + lane, a.n_seqs - 1);
+            first[i] = a.cu_q[seq]; end[i] = a.cu_q[seq + 1]; ctx[i] = a.ctx_len[seq];
           }
-        } else {
-#pragma unroll 1
-          for (int g = 0; g < 8; ++g) {
-            const int row = __shfl_sync(0xffffffffu, first, 8 * j + g);
-            const bf16* from = pool + (row < 0 ? 0 : (long)row * DIM + lane_from);
+          int tiles = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int key = key0 + row0 + g * 8 + 2 * i + (lane >> 4);
-              const bool wanted = row >= 0 && key < now.ctx && key >= now.key_lo;
-              copy16_or_zeros(at + to[i] + g * 1024, wanted ? from + 2 * i * DIM : pool, wanted ? 16 : 0);
+          for (int i = 0; i < 2; ++i) {
+            const int seq = base + 32 * i + lane;
+            if (seq < a.n_seqs) {
+              const Sequence s = find_sequence<ROWS2>(a, first[i], end[i], ctx[i]);
+              const int mine = a.kv_heads * s.row_tiles * s.tiles;
+              if (seq < SEQ_CACHE) known[seq] = make_int4(first[i], end[i], ctx[i], mine);
+              tiles += mine;
             }
           }
+          total += __reduce_add_sync(0xffffffffu, tiles);
         }
-        arrive_when_copied(smem_u32(&full[values * STAGES + stage]));
-        ++taken;
+        const int blocks = min((int)gridDim.x, total), b = min((int)blockIdx.x, blocks);
+        const int from = b < blocks ? share_begin(total, b, blocks) : total, upto = b < blocks ? share_begin(total, b + 1, blocks) : total;
+        if (lane == 0) { start[0] = start[1] = 0; start[2] = upto - from; }
+        __syncwarp();
+        int before = 0;
+        for (int base = 0; base < a.n_seqs; base += 32) {
+          const int i = base + lane;
+          int tiles = 0;
+          if (i < a.n_seqs) {
+            if (i < SEQ_CACHE) {
+              tiles = known[i].w;
+            } else {
+              const Sequence s = find_sequence<ROWS2>(a, known, i);
+              tiles = a.kv_heads * s.row_tiles * s.tiles;
+            }
+          }
+          int sum = tiles;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += other;
+          }
+          const int mine = before + sum - tiles;
+          if (from >= mine && from < mine + tiles) { start[0] = i; start[1] = from - mine; }
+          before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) start[3] = total;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(started);
+      } else {
+        ok = warp_wait(started, 0) || ran_out(1);
       }
-      now = soon;
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == LOADERS) {
-    // ---------------- the products, turn by turn; the scores are two turns ahead
-    pdl_wait();
-    ok = warp_wait(started, 0) || ran_out(2);
-    const int n_tiles = ok ? start[2] : 0;
-    Walk<ROWS2> ahead, walk;
-    ahead.begin_at(a, known, start[0], start[1], n_tiles);
-    walk.begin_at(a, known, start[0], start[1], n_tiles);
-    const int turns = warp_uniform(n_tiles * (ROWS2 ? 2 : 1));
-    int k_taken = 0, v_taken = 0, k_stage = 0, v_stage = 0;
-    int a_left = 0, a_segment = -1, g_left = 0, g_turn = 0, g_segment = -1;
-    // turn -2 and -1 have scores to be made and no second product: the loop holds each kind of product once
+      // ---------------- K or V, and the first of these warps the queries
+      const int n_tiles = ok ? start[2] : 0, values = warp >> 1, row0 = (warp & 1) * 64, page_shift = __ffs(a.page_tokens) - 1;
+      const bf16* pool = (const bf16*)(values ? a.v_pool : a.k_pool);
+      // a lane copies 16 bytes of rows 2 i + (lane >> 4) of each 8 of this warp's rows; `to` are their places in those 8, swizzled
+      const uint32_t ring_at = smem_u32(ring) + values * STAGES * TILE_BYTES + ((lane & 15) >> 3) * HALF_BYTES + row0 * 128;
+      uint32_t to[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[i] = (2 * i + (lane >> 4)) * 128 + (((lane & 7) ^ (2 * i + (lane >> 4))) << 4);
+      const long lane_from = (lane >> 4) * DIM + (lane & 15) * 8;
+      // Up to four tiles of a segment, whose pages are looked up together, four tiles ahead (a read from memory waits behind all copies
+      // in flight): lane 8 j + i has the page of rows 8 i .. of tile j.
+      struct Group { int page, key0, count, head, key_lo, ctx, draft; } now, soon;
+      Walk<ROWS2> ahead;
+      ahead.begin_at(a, known, start[0], start[1], n_tiles);
+      int tile = 0, segments = 0, taken = 0;
+      auto next_group = [&](Group& g) {
+        g.count = 0; g.draft = -1;
+        if (tile == ahead.count) {
+          if (!ahead.next(a)) return;
+          tile = 0;
+          g.draft = ahead.s.first + ahead.row_tile * (ROWS2 ? 2 : 1) * drafts_tile;      // a segment begins: its queries
+        }
+        g.count = min(4, ahead.count - tile); g.head = ahead.head; g.key0 = (ahead.s.tile_lo + ahead.begin + tile) * KEYS;
+        g.key_lo = ahead.s.key_lo; g.ctx = ahead.s.ctx;
+        const int key = g.key0 + (lane >> 3) * KEYS + row0 + (lane & 7) * 8, index = key >> page_shift;
+        g.page = index < a.table_width && key < g.ctx ? a.block_table[(size_t)ahead.seq * a.table_width + index] : -1;
+        tile += g.count;
+      };
+      next_group(now);
+      while (ok && now.count > 0) {
+        next_group(soon);
+        if (warp == 0 && now.draft >= 0) {
+          const int buf = ROWS2 ? 0 : segments & 1;
+          ok = warp_wait(&q_empty[buf], ((ROWS2 ? segments : segments >> 1) & 1) ^ 1) || ran_out(2);
+          if (!ok) break;
+          const uint32_t bar = smem_u32(&q_full[buf]);
+          expect_bytes(bar, (uint32_t)(drafts_tile * group * 128) * (ROWS2 ? 4 : 2));
+          const int head = warp_uniform(now.head * group), draft = warp_uniform(now.draft);
+          for (int part = 0; part < (ROWS2 ? 2 : 1); ++part)
+            for (int h = 0; h < 2; ++h)
+              load_queries(smem_u32(q_s) + (ROWS2 ? part : buf) * TILE_BYTES + h * HALF_BYTES, &q_map, bar, h * 64, head, draft + part * drafts_tile);
+          ++segments;
+        }
+        // the places in the pool of the rows that begin the eights; -1: the page is not there
+        const int first = (unsigned)now.page < (unsigned)a.n_pages
+                              ? (now.page * a.kv_heads + now.head) * a.page_tokens + ((row0 + (lane & 7) * 8) & (a.page_tokens - 1)) : -1;
+        const unsigned there = __ballot_sync(0xffffffffu, first >= 0);
+        for (int j = 0; j < now.count; ++j) {
+          const int stage = taken % STAGES, key0 = now.key0 + j * KEYS;
+          ok = warp_wait(&empty[values * STAGES + stage], ((taken / STAGES) & 1) ^ 1) || ran_out(1);
+          if (!ok || flag[0]) { ok = false; break; }
+          const uint32_t at = ring_at + stage * TILE_BYTES;
+          if ((there >> (8 * j) & 0xFFu) == 0xFFu && key0 >= now.key_lo && key0 + KEYS <= now.ctx) {
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              const bf16* from = pool + (long)__shfl_sync(0xffffffffu, first, 8 * j + g) * DIM + lane_from;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) copy16(at + to[i] + g * 1024, from + 2 * i * DIM);
+            }
+          } else {
 #pragma unroll 1
-    for (int t = -2; t < turns && ok; ++t) {
-      const int w = t & 1;
-      if (t >= 0) {
-        if (g_left == 0) {
-          walk.next(a);
-          g_left = warp_uniform(ROWS2 ? 2 * walk.count : walk.count);
-          g_turn = 0;
-          ++g_segment;
-          if (g_segment > 0) ok = warp_wait(o_empty, (g_segment - 1) & 1) || ran_out(8);
-        }
-        if (ok && (!ROWS2 || w == 0)) {
-          v_stage = STAGES + v_taken % STAGES;
-          ok = warp_wait(&full[v_stage], (v_taken / STAGES) & 1) || ran_out(4);
-          ++v_taken;
-          fence_async_smem();                              // what cp.async wrote is read by the tensor cores
-        }
-        ok = ok && (warp_wait(&p_full[w], (t >> 1) & 1) || ran_out(5));
-        if (!ok) break;
-        fence_after_sync();
-        const uint32_t v_addr = smem_u32(ring + v_stage * TILE_BYTES);
+            for (int g = 0; g < 8; ++g) {
+              const int row = __shfl_sync(0xffffffffu, first, 8 * j + g);
+              const bf16* from = pool + (row < 0 ? 0 : (long)row * DIM + lane_from);
 #pragma unroll
-        for (int ks = 0; ks < KEYS / 16; ++ks)            // 16 keys: 8 columns of weights, 16 rows of V
-          umma_from_tmem(tmem_o + w * 128, tmem_s + w * 128 + ks * 8, desc_mn_major(v_addr + ks * 16 * 128), IDESC_O, (g_turn > 1 || ks > 0) ? 1u : 0u);
-        umma_commit(&pv_done[w]);
-        if (!ROWS2 || w == 1) umma_commit(&empty[v_stage]);
-        ++g_turn;
-        if (--g_left == 0) umma_commit(o_full);
+              for (int i = 0; i < 4; ++i) {
+                const int key = key0 + row0 + g * 8 + 2 * i + (lane >> 4);
+                const bool wanted = row >= 0 && key < now.ctx && key >= now.key_lo;
+                copy16_or_zeros(at + to[i] + g * 1024, wanted ? from + 2 * i * DIM : pool, wanted ? 16 : 0);
+              }
+            }
+          }
+          arrive_when_copied(smem_u32(&full[values * STAGES + stage]));
+          ++taken;
+        }
+        now = soon;
       }
-      if (t + 2 < turns) {
-        if (a_left == 0) {
-          ahead.next(a);
-          a_left = warp_uniform(ROWS2 ? 2 * ahead.count : ahead.count);
-          ++a_segment;
-          ok = warp_wait(&q_full[ROWS2 ? 0 : a_segment & 1], (ROWS2 ? a_segment : a_segment >> 1) & 1) || ran_out(2);
-        }
-        if (ok && (!ROWS2 || w == 0)) {
-          k_stage = k_taken % STAGES;
-          ok = warp_wait(&full[k_stage], (k_taken / STAGES) & 1) || ran_out(3);
-          ++k_taken;
-          fence_async_smem();
-        }
-        if (!ok) break;
-        fence_after_sync();
-        const uint32_t q_addr = smem_u32(q_s + (ROWS2 ? w : a_segment & 1) * TILE_BYTES), k_addr = smem_u32(ring + k_stage * TILE_BYTES);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == LOADERS) {
+      // ---------------- the products, turn by turn; the scores are two turns ahead
+      pdl_wait();
+      ok = warp_wait(started, 0) || ran_out(2);
+      const int n_tiles = ok ? start[2] : 0;
+      Walk<ROWS2> ahead, walk;
+      ahead.begin_at(a, known, start[0], start[1], n_tiles);
+      walk.begin_at(a, known, start[0], start[1], n_tiles);
+      const int turns = warp_uniform(n_tiles * (ROWS2 ? 2 : 1));
+      int k_taken = 0, v_taken = 0, k_stage = 0, v_stage = 0;
+      int a_left = 0, a_segment = -1, g_left = 0, g_turn = 0, g_segment = -1;
+      // turn -2 and -1 have scores to be made and no second product: the loop holds each kind of product once
+#pragma unroll 1
+      for (int t = -2; t < turns && ok; ++t) {
+        const int w = t & 1;
+        if (t >= 0) {
+          if (g_left == 0) {
+            walk.next(a);
+            g_left = warp_uniform(ROWS2 ? 2 * walk.count : walk.count);
+            g_turn = 0;
+            ++g_segment;
+            if (g_segment > 0) ok = warp_wait(o_empty, (g_segment - 1) & 1) || ran_out(8);
+          }
+          if (ok && (!ROWS2 || w == 0)) {
+            v_stage = STAGES + v_taken % STAGES;
+            ok = warp_wait(&full[v_stage], (v_taken / STAGES) & 1) || ran_out(4);
+            ++v_taken;
+            fence_async_smem();                              // what cp.async wrote is read by the tensor cores
+          }
+          ok = ok && (warp_wait(&p_full[w], (t >> 1) & 1) || ran_out(5));
+          if (!ok) break;
+          fence_after_sync();
+          const uint32_t v_addr = smem_u32(ring + v_stage * TILE_BYTES);
 #pragma unroll
-        for (int ks = 0; ks < DIM / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * HALF_BYTES + (ks & 3) * 32;
-          umma_bf16(tmem_s + w * 128, desc_k_major(q_addr + off), desc_k_major(k_addr + off), IDESC_S, ks > 0 ? 1u : 0u);
+          for (int ks = 0; ks < KEYS / 16; ++ks)            // 16 keys: 8 columns of weights, 16 rows of V
+            umma_from_tmem(tmem_o + w * 128, tmem_s + w * 128 + ks * 8, desc_mn_major(v_addr + ks * 16 * 128), IDESC_O, (g_turn > 1 || ks > 0) ? 1u : 0u);
+          umma_commit(&pv_done[w]);
+          if (!ROWS2 || w == 1) umma_commit(&empty[v_stage]);
+          ++g_turn;
+          if (--g_left == 0) umma_commit(o_full);
         }
-        umma_commit(&s_full[w]);
-        if (!ROWS2 || w == 1) umma_commit(&empty[k_stage]);
-        if (--a_left == 0) umma_commit(&q_empty[ROWS2 ? 0 : a_segment & 1]);
+        if (t + 2 < turns) {
+          if (a_left == 0) {
+            ahead.next(a);
+            a_left = warp_uniform(ROWS2 ? 2 * ahead.count : ahead.count);
+            ++a_segment;
+            ok = warp_wait(&q_full[ROWS2 ? 0 : a_segment & 1], (ROWS2 ? a_segment : a_segment >> 1) & 1) || ran_out(2);
+          }
+          if (ok && (!ROWS2 || w == 0)) {
+            k_stage = k_taken % STAGES;
+            ok = warp_wait(&full[k_stage], (k_taken / STAGES) & 1) || ran_out(3);
+            ++k_taken;
+            fence_async_smem();
+          }
+          if (!ok) break;
+          fence_after_sync();
+          const uint32_t q_addr = smem_u32(q_s + (ROWS2 ? w : a_segment & 1) * TILE_BYTES), k_addr = smem_u32(ring + k_stage * TILE_BYTES);
+#pragma unroll
+          for (int ks = 0; ks < DIM / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * HALF_BYTES + (ks & 3) * 32;
+            umma_bf16(tmem_s + w * 128, desc_k_major(q_addr + off), desc_k_major(k_addr + off), IDESC_S, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[w]);
+          if (!ROWS2 || w == 1) umma_commit(&empty[k_stage]);
+          if (--a_left == 0) umma_commit(&q_empty[ROWS2 ? 0 : a_segment & 1]);
+        }
       }
-    }
-  } else if (warp == LOADERS + 1) {
-    // ---------------- for the kernel that joins: the row tile inside which this block's share begins, if it is the first that does
-    pdl_wait();
-    ok = warp_wait(started, 0) || ran_out(2);
-    Walk<ROWS2> walk;
-    walk.begin_at(a, known, start[0], start[1], ok ? start[2] : 0);
-    Border border = {};
-    if (walk.next(a) && walk.begin > 0) {
-      const int total = start[3], shares = min((int)gridDim.x, total), unit = share_begin(total, blockIdx.x, shares) - walk.begin;
-      border.from = share_of(total, unit, shares);
-      border.upto = share_of(total, unit + walk.s.tiles - 1, shares);
-      if (border.from + 1 == (int)blockIdx.x) {
-        border.draft = walk.row_tile * (ROWS2 ? 2 : 1) * drafts_tile;
-        border.drafts = min(min(walk.s.n, a.max_nodes) - border.draft, (ROWS2 ? 2 : 1) * drafts_tile);
-        border.seq = walk.seq; border.head = walk.head; border.token = walk.s.first + border.draft;
+    } else if (warp == LOADERS + 1) {
+      // ---------------- for the kernel that joins: the row tile inside which this block's share begins, if it is the first that does
+      pdl_wait();
+      ok = warp_wait(started, 0) || ran_out(2);
+      Walk<ROWS2> walk;
+      walk.begin_at(a, known, start[0], start[1], ok ? start[2] : 0);
+      Border border = {};
+      if (walk.next(a) && walk.begin > 0) {
+        const int total = start[3], shares = min((int)gridDim.x, total), unit = share_begin(total, blockIdx.x, shares) - walk.begin;
+        border.from = share_of(total, unit, shares);
+        border.upto = share_of(total, unit + walk.s.tiles - 1, shares);
+        if (border.from + 1 == (int)blockIdx.x) {
+          border.draft = walk.row_tile * (ROWS2 ? 2 : 1) * drafts_tile;
+          border.drafts = min(min(walk.s.n, a.max_nodes) - border.draft, (ROWS2 ? 2 : 1) * drafts_tile);
+          border.seq = walk.seq; border.head = walk.head; border.token = walk.s.first + border.draft;
+        }
       }
+      if (lane == 0) a.borders[blockIdx.x] = border;
     }
-    if (lane == 0) a.borders[blockIdx.x] = border;
-  }
   } else {
     take_registers<MANY_REGS>();
     // ---------------- softmax: one row a thread

@@ -8,11 +8,17 @@
 //
 // Two kernels. The first reads the logits once: a block takes a chunk of one row, piece by piece, and leaves the chunk's maximum and sum of
 // exponentials and its `keep` best. Those are found by a threshold that `keep` values reach at least and few more: the keep-th largest of 64
-// groups' own maxima in the first piece. What reaches it is collected, and ranked by counting when there is much of it (which gives
-// a higher threshold) and at the end. Within a beam the order is that of the logits themselves, so no rounding is involved. The
-// second kernel has one block a request: the beams' sums are joined in 64 bits, and of the chunks' lists the candidates are compared
-// in 64 bits behind a threshold of the same kind, where two beams' tie only where the formula's do within 1e-7.
-// Where more values reach a threshold than there is room for (many equal ones), the best are picked one by one.
+// groups' own maxima in the first piece. Every warp collects what reaches it by itself (a barrier a piece and a counter of the block cost 11 of
+// 27 us at 128 rows of 151,936), keeps the best of it when it gets much, which gives a higher threshold, and at the end a threshold
+// of the same kind, over the whole chunk, leaves a few to be ranked by counting. Within a beam the order is that of the logits
+// themselves, so no rounding is involved. The second kernel has one block a request: the beams' sums are joined in 64 bits, and of the
+// chunks' lists the candidates are compared in 64 bits behind a threshold of the same kind, where two beams' tie only where the formula's
+// do within 1e-7; where more reach it than there is room for (many equal ones), the best are picked one by one.
+//
+// The logits' bytes bound it in theory. Measured (one B200): 128 rows of 151,936, a fifth of the beams ended, 16 kept 33 us, of them 24 the
+// first kernel (3.2 TB/s of what it reads: a block's first piece, its thresholds and ranking run alone), 4 rows 8.1 us, two launches
+// of about 4 that wait for memory twice.
+#include <float.h>
 #include <math.h>
 
 #include "common.cuh"
@@ -34,22 +40,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }
 template <typename T>
 __device__ __forceinline__ bool before(T v, int i, T w, int j) { return v > w || (v == w && i < j); }
-
-// The keep-th largest (keep <= 64) of the values of threads 0 .. 63 (ties: the lower thread first): the same for all threads. Where they
-// are the largest of 64 groups of values, `keep` values reach it at least. `all` has room for them.
-template <typename T>
-__device__ __forceinline__ T kth_largest_of_64(T v, int keep, T* all, T* result) {
-  if (threadIdx.x < 64) all[threadIdx.x] = v;
-  __syncthreads();
-  if (threadIdx.x < 64) {
-    int rank = 0;
-#pragma unroll 16
-    for (int t = 0; t < 64; ++t) rank += before(all[t], t, v, (int)threadIdx.x) ? 1 : 0;
-    if (rank == keep - 1) *result = v;
-  }
-  __syncthreads();
-  return *result;
-}
 // The best of what the threads offer: the same for all threads.
 template <typename T>
 __device__ __forceinline__ void block_best(T& v, int& i, T* values, int* indices) {
@@ -67,116 +57,158 @@ __device__ __forceinline__ void block_best(T& v, int& i, T* values, int* indices
     if (before(values[w], indices[w], v, i)) { v = values[w]; i = indices[w]; }
 }
 
+// The best `keep` of the warp's `n` values (keep < n <= WARP_ROOM) are left in `found`, best first; the last of them.
+constexpr int WARP_ROOM = 128;
+__device__ __noinline__ float keep_best(const float* __restrict__ row, int* found, float* worth, int n, int keep) {
+  const int lane = threadIdx.x & 31;
+  float v[WARP_ROOM / 32];
+  int i[WARP_ROOM / 32], rank[WARP_ROOM / 32];
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < WARP_ROOM / 32; ++c) {
+    rank[c] = 0; i[c] = NONE; v[c] = -INFINITY;
+    if (lane + 32 * c < n) {
+      i[c] = found[lane + 32 * c]; v[c] = row[i[c]];
+      worth[lane + 32 * c] = v[c];
+    }
+  }
+  __syncwarp();
+  for (int o = 0; o < n; ++o) {
+    const float other = worth[o];
+    const int index = found[o];
+#pragma unroll
+    for (int c = 0; c < WARP_ROOM / 32; ++c) rank[c] += before(other, index, v[c], i[c]) ? 1 : 0;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < WARP_ROOM / 32; ++c)
+    if (lane + 32 * c < n && rank[c] < keep) { found[rank[c]] = i[c]; worth[rank[c]] = v[c]; }
+  __syncwarp();
+  return worth[keep - 1];
+}
+
+// A value that at least `keep` of the block's reach, found from the maxima of 64 groups of four threads: the keep-th largest of those, up to
+// its last six bits, which make way for the group's number so that no two are equal. Not below the lowest finite number: -inf is no candidate.
+__device__ __forceinline__ float reached_by(float top, int keep, int* keys, float* result) {
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int bits = __float_as_int(top), key = bits ^ (bits >> 31 & 0x7fffffff);      // in the order of the numbers
+  if ((threadIdx.x & 3) == 0) keys[threadIdx.x >> 2] = (key & ~63) | threadIdx.x >> 2;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    const int mine = keys[threadIdx.x], low = mine & ~63;
+    int rank = 0;
+#pragma unroll
+    for (int t = 0; t < 64; t += 4) {
+      const int4 k = *reinterpret_cast<const int4*>(keys + t);
+      rank += (k.x > mine ? 1 : 0) + (k.y > mine ? 1 : 0) + (k.z > mine ? 1 : 0) + (k.w > mine ? 1 : 0);
+    }
+    if (rank == keep - 1) *result = fmaxf(__int_as_float(low ^ (low >> 31 & 0x7fffffff)), -FLT_MAX);      // what is below -inf is NaN
+  }
+  __syncthreads();
+  return *result;
+}
+
 // stats [rows][chunks] (maximum, sum of exp(x - maximum)), lists [rows][chunks][keep] of (value, index), best first, (-inf, NONE) behind the last.
-// A chunk is `pieces` of PIECE values.
+// A chunk is `pieces` of PIECE values. Rows of beams that are not there or have ended are not read, and nothing is written for them.
 constexpr int EACH = 16, PIECE = THREADS * EACH;
-__global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const float* __restrict__ logits, long row_stride, int vocab, int keep, int pieces,
+__global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const float* __restrict__ logits, long row_stride, const float* __restrict__ scores,
+                                                                const int* __restrict__ ended, int vocab, int keep, int pieces,
                                                                 float2* __restrict__ stats, float2* __restrict__ lists) {
-  __shared__ float values[ROOM], part[WARPS], part_sum[WARPS], threshold, spread[THREADS];
-  __shared__ int indices[ROOM], count;
+  __shared__ __align__(16) int keys[64];
+  __shared__ float worth[WARPS][WARP_ROOM], part[WARPS], part_sum[WARPS], threshold, last_threshold;
+  __shared__ float2 all_best[THREADS];
+  __shared__ int found[WARPS][WARP_ROOM], total;
   pdl_launch_dependents();
   pdl_wait();
   const float* row = logits + (size_t)blockIdx.y * row_stride;
   const int begin = blockIdx.x * pieces * PIECE, end = min(vocab, begin + pieces * PIECE), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float next[EACH], m = -INFINITY, sum = 0.f, reach = -INFINITY;
+  float next[EACH], m = -INFINITY, sum = 0.f, bar = -FLT_MAX;      // what does not reach `bar` is not among the best
+  int held = 0;                                            // indices in `found` of this warp, in their order
+  const bool wanted = scores[blockIdx.y] > -INFINITY && !(ended && ended[blockIdx.y]);
 #pragma unroll
   for (int j = 0; j < EACH; ++j) next[j] = begin + (int)threadIdx.x + j * THREADS < end ? row[begin + threadIdx.x + j * THREADS] : -INFINITY;
-  if (threadIdx.x == 0) count = 0;
+  if (!wanted) return;                                     // the first piece was asked for all the same: the others would wait for this
+  if (threadIdx.x == 0) total = 0;
   for (int from = begin; from < end; from += PIECE) {
     const int lo = from + threadIdx.x;
     float x[EACH];
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {                       // the next piece is on its way while this one is looked at
-      x[j] = next[j];
-      next[j] = lo + PIECE + j * THREADS < end ? row[lo + PIECE + j * THREADS] : -INFINITY;
+    for (int j = 0; j < EACH; ++j) x[j] = next[j];
+    const float* behind = row + lo + PIECE;                // the next piece is on its way while this one is looked at
+    if (from + 2 * PIECE <= end) {
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) next[j] = behind[j * THREADS];
+    } else {
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) next[j] = lo + PIECE + j * THREADS < end ? behind[j * THREADS] : -INFINITY;
     }
     float top = -INFINITY;                                 // of numbers: NaN is no maximum, but the sum becomes it
 #pragma unroll
     for (int j = 0; j < EACH; ++j) top = fmaxf(top, x[j]);
-    if (from == begin) {
-      spread[threadIdx.x] = top;
-      __syncthreads();
-      float group = -INFINITY;
-      if (threadIdx.x < 64) group = fmaxf(fmaxf(spread[threadIdx.x], spread[threadIdx.x + 64]), fmaxf(spread[threadIdx.x + 128], spread[threadIdx.x + 192]));
-      reach = kth_largest_of_64(group, keep, values, &threshold);
-    }
+    if (from == begin) bar = reached_by(top, keep, keys, &threshold);
     const float rise = fmaxf(m, top), base = rise == -INFINITY ? 0.f : rise;
     sum *= fast_exp2((m - base) * LOG2E);
     m = rise;
 #pragma unroll
     for (int j = 0; j < EACH; ++j) sum += fast_exp2((x[j] - base) * LOG2E);
-    if (top >= reach) {
+    unsigned hits = 0, any;
+    if (top >= bar) {
 #pragma unroll
-      for (int j = 0; j < EACH; ++j)
-        if (x[j] >= reach && x[j] > -INFINITY) {
-          const int at = atomicAdd(&count, 1);
-          if (at < ROOM) { values[at] = x[j]; indices[at] = lo + j * THREADS; }
-        }
+      for (int j = 0; j < EACH; ++j) hits |= x[j] >= bar ? 1u << j : 0u;
     }
-    __syncthreads();
-    const int n = count;
-    if (n > ROOM / 2 && n <= ROOM) {                       // the best of them, and a higher threshold
-      float v[ROOM / THREADS];
-      int i[ROOM / THREADS], rank[ROOM / THREADS];
+    for (any = __reduce_or_sync(0xffffffffu, hits); any; any &= any - 1) {      // in the order of the indices
+      const int j = __ffs(any) - 1;
+      const unsigned with = __ballot_sync(0xffffffffu, hits >> j & 1u);
+      if (hits >> j & 1u) found[warp][held + __popc(with & ((1u << lane) - 1u))] = lo + j * THREADS;
+      held += __popc(with);
+      if (held > WARP_ROOM - 32) {                         // what comes behind and equals the last of the best is not among them
+        bar = nextafterf(keep_best(row, found[warp], worth[warp], held, keep), INFINITY);
+        held = keep;
+        unsigned still = 0;
 #pragma unroll
-      for (int c = 0; c < ROOM / THREADS; ++c) {
-        rank[c] = NONE;
-        if ((int)threadIdx.x + c * THREADS < n) {
-          v[c] = values[threadIdx.x + c * THREADS]; i[c] = indices[threadIdx.x + c * THREADS];
-          rank[c] = 0;
-          for (int o = 0; o < n; ++o) rank[c] += before(values[o], indices[o], v[c], i[c]) ? 1 : 0;
-        }
+        for (int e = 0; e < EACH; ++e) still |= x[e] >= bar ? 1u << e : 0u;
+        hits &= still;
+        any &= __reduce_or_sync(0xffffffffu, hits) | (1u << j);
       }
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < ROOM / THREADS; ++c)
-        if (rank[c] < keep) {
-          values[rank[c]] = v[c]; indices[rank[c]] = i[c];
-          if (rank[c] == keep - 1) threshold = v[c];
-        }
-      if (threadIdx.x == 0) count = keep;
-      __syncthreads();
-      reach = threshold;
     }
   }
-  // the maximum and the sum of all threads
-  float top = warp_max(m), base = top == -INFINITY ? 0.f : top;
+  if (held > 32) {
+    keep_best(row, found[warp], worth[warp], held, keep);
+    held = keep;
+  }
+  // the maximum and the sum of all threads, and of what the warps hold that which reaches a threshold of the whole chunk
+  int i = NONE;
+  float v = -INFINITY;
+  if (lane < held) { i = found[warp][lane]; v = row[i]; }
+  const float top = warp_max(m), base = top == -INFINITY ? 0.f : top;
   sum = warp_sum(sum * fast_exp2((m - base) * LOG2E));
   if (lane == 0) { part[warp] = top; part_sum[warp] = sum; }
+  bar = reached_by(m, keep, keys, &last_threshold);
+  const unsigned with = __ballot_sync(0xffffffffu, v >= bar);
+  int at = 0;
+  if (lane == 0 && with) at = atomicAdd(&total, __popc(with));      // any order: they are ranked
+  at = __shfl_sync(0xffffffffu, at, 0) + __popc(with & ((1u << lane) - 1u));
+  if (v >= bar) all_best[at] = make_float2(v, __int_as_float(i));
   __syncthreads();
-  const size_t at = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, part[w]);
-    base = top == -INFINITY ? 0.f : top;
-    float all = 0.f;
-    for (int w = 0; w < WARPS; ++w) all += part_sum[w] * fast_exp2((part[w] - base) * LOG2E);
-    stats[at] = make_float2(top, all);
+  const size_t chunk = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
+  float2* list = lists + chunk * keep;
+  const int n = total;                                     // 32 of each warp at most
+  if ((int)threadIdx.x < n) {
+    const float2 mine = all_best[threadIdx.x];
+    int rank = 0;
+    for (int o = 0; o < n; ++o) {
+      const float2 other = all_best[o];
+      rank += before(other.x, __float_as_int(other.y), mine.x, __float_as_int(mine.y)) ? 1 : 0;
+    }
+    if (rank < keep) list[rank] = mine;
+  } else if ((int)threadIdx.x < keep) {
+    list[threadIdx.x] = make_float2(-INFINITY, __int_as_float(NONE));
   }
-  float2* list = lists + at * keep;
-  const int n = count;
-  if (n <= ROOM) {
-    for (int c = threadIdx.x; c < n; c += THREADS) {
-      const float v = values[c];
-      const int i = indices[c];
-      int rank = 0;
-      for (int o = 0; o < n; ++o) rank += before(values[o], indices[o], v, i) ? 1 : 0;
-      if (rank < keep) list[rank] = make_float2(v, __int_as_float(i));
-    }
-    if ((int)threadIdx.x >= n && (int)threadIdx.x < keep) list[threadIdx.x] = make_float2(-INFINITY, __int_as_float(NONE));
-  } else {                                                 // one after the other: the best behind the one before
-    float last = INFINITY;
-    int last_index = -1;
-    for (int k = 0; k < keep; ++k) {
-      float v = -INFINITY;
-      int i = NONE;
-      for (int j = begin + threadIdx.x; j < end; j += THREADS) {
-        const float y = row[j];
-        if (y > -INFINITY && before(last, last_index, y, j) && before(y, j, v, i)) { v = y; i = j; }
-      }
-      block_best(v, i, part, indices);
-      if (threadIdx.x == 0) list[k] = make_float2(v, __int_as_float(i));
-      last = v; last_index = i;
-    }
+  if (warp == WARPS - 1) {
+    const float mine = lane < WARPS ? part[lane] : -INFINITY, all = warp_max(mine), from = all == -INFINITY ? 0.f : all;
+    const float sums = warp_sum(lane < WARPS ? part_sum[lane] * fast_exp2((mine - from) * LOG2E) : 0.f);
+    if (lane == 0) stats[chunk] = make_float2(all, sums);
   }
 }
 
@@ -185,8 +217,9 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const float* __restr
                                                             float* __restrict__ next_scores, int* __restrict__ parents, int* __restrict__ tokens) {
   __shared__ double offsets[MAX_BEAMS];                    // what a beam's logits are raised by; its own score where it has ended; -inf: no beam
   __shared__ bool over[MAX_BEAMS];
-  __shared__ double values[ROOM], part[WARPS], threshold;
-  __shared__ double spread[THREADS];
+  __shared__ double values[ROOM], part[WARPS];
+  __shared__ __align__(16) int keys[64];
+  __shared__ float threshold;
   __shared__ int indices[ROOM], part_index[WARPS];
   __shared__ int count;
   pdl_launch_dependents();
@@ -236,19 +269,19 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const float* __restr
     if (v > best) best = v;
   }
   // groups of threads 64 apart: what is best of a list lies in different ones
-  spread[threadIdx.x] = best;
-  __syncthreads();
-  if (threadIdx.x < 64) best = fmax(fmax(spread[threadIdx.x], spread[threadIdx.x + 64]), fmax(spread[threadIdx.x + 128], spread[threadIdx.x + 192]));
-  const double reach = kth_largest_of_64(best, keep, values, &threshold);
-  for (int c = threadIdx.x; c < n_candidates; c += THREADS) {
-    double v;
-    int i;
-    candidate(c, v, i);
-    if (v >= reach && i != NONE) {
-      const int at = atomicAdd(&count, 1);
-      if (at < ROOM) { values[at] = v; indices[at] = i; }
+  // a value that `keep` candidates reach; the lowest one stands for none
+  const float lowest = reached_by(__double2float_rd(best), keep, keys, &threshold);
+  const double reach = lowest == -FLT_MAX ? -INFINITY : (double)lowest;
+  if (best >= reach)
+    for (int c = threadIdx.x; c < n_candidates; c += THREADS) {
+      double v;
+      int i;
+      candidate(c, v, i);
+      if (v >= reach && i != NONE) {
+        const int at = atomicAdd(&count, 1);
+        if (at < ROOM) { values[at] = v; indices[at] = i; }
+      }
     }
-  }
   __syncthreads();
   const int n = count;
   auto choose = [&](int k, double v, int i) {
@@ -299,7 +332,7 @@ LB_EXPORT int lb_beam_select(const float* logits, long row_stride, const float* 
   if (scratch_words < rows * chunks * (2 + 2 * keep)) return LB_ERR_SIZE;
   if ((uintptr_t)scratch & 7) return LB_ERR_ALIGN;
   float2 *stats = (float2*)scratch, *lists = stats + rows * chunks;
-  int code = lb_launch(beam_chunk_kernel, dim3((unsigned)chunks, (unsigned)rows), THREADS, 0, stream, logits, row_stride, vocab, keep, pieces, stats, lists);
+  int code = lb_launch(beam_chunk_kernel, dim3((unsigned)chunks, (unsigned)rows), THREADS, 0, stream, logits, row_stride, scores, ended, vocab, keep, pieces, stats, lists);
   if (code) return code;
   code = lb_launch(beam_join_kernel, requests, THREADS, 0, stream, scores, ended, beams, vocab, keep, pad, (int)chunks, stats, lists, next_scores, parents, tokens);
   return code ? code : lb_last_error();

@@ -1466,9 +1466,9 @@ _BEAM_PIECE = 4096      # values of a row that a block of the first kernel looks
 
 def _beam_pieces(rows: int, vocab: int, sms: int) -> int:
     """Pieces of a row that one block takes: 2 to 5, by the pieces there are for the SMs. The first costs the block most, but what is left
-    over runs alone. Measured (one B200, us; 1, 2, 4, 5 and 8 pieces): 128 rows of 151,936 67, 47, 39.6, 37.5 and 41.5 (5 are taken), 64 rows
-    22, 18, 17.6, 16.4 and 19.5 (5), 16 rows 11.6, 11.2, 11.5, 12.3 and 14.9 (2), 4 rows 8.7, 8.3, 10.4, 11.5 and 14.4 (2), 32 rows of 32,768
-    with 32 kept 37, 20, 22, 27 and 36 (2)."""
+    over runs alone. Measured (one B200, us; 2, 4, 5, 6 and 8 pieces): 128 rows of 151,936 41.5, 33.9, 32.8, 33.1 and 32.4 (5 are taken), 64 rows
+    18.2, 17.4, 16.1, 16.9 and 18.5 (5), 16 rows 11.1, 10.4, 10.6, 11.3 and 12.1 (2), 4 rows 8.1, 9.3, 9.7, 10.2 and 11.4 (2), 32 rows of
+    32,768 with 32 kept 19.6, 19.9, 21.5, 23.2 and 24.6 (2)."""
     return min(5, max(2, -(-10 * rows * -(-vocab // _BEAM_PIECE) // (34 * sms))))
 
 

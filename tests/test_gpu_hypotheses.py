@@ -377,6 +377,18 @@ def test_beam_selection_of_masked_beams_and_tokens():
         check_beams(logits.cuda(), scores, keep, torch.tensor([[0, 1, 1], [0, 0, 1], [1, 1, 0], [1, 0, 1]], dtype=torch.int32), pad=2999)
 
 
+def test_beam_selection_does_not_read_beams_that_are_over():
+    """Neither an ended beam's logits nor those of one that is not there reach the others."""
+    gen = torch.Generator().manual_seed(10)
+    logits = torch.randn(8, 9000, generator=gen)
+    clean = logits.clone()
+    logits[1] = float("nan"); logits[6] = INF; logits[7, 100:] = float("nan")
+    scores = torch.tensor([[-1.0, -INF, -2.0, -1.5], [-1.0, -2.0, -1.5, -INF]])
+    ended = torch.tensor([[0, 0, 0, 1], [0, 0, 1, 0]], dtype=torch.int32)
+    found, expected = select(logits.cuda(), scores, 8, ended, 5), select(clean.cuda(), scores, 8, ended, 5)
+    assert all(torch.equal(x, y) for x, y in zip(found, expected)) and bool((found[2] >= 0).all())
+
+
 def test_first_step_of_a_beam_search_takes_one_beam():
     gen = torch.Generator().manual_seed(9)
     logits = torch.randn(8, 4096, generator=gen).cuda()

@@ -40,12 +40,12 @@ constexpr int ROWS = 8;
 template <typename V>
 __global__ void __launch_bounds__(THREADS) compact_tokens_kernel(V* __restrict__ pool, const int* __restrict__ block_table, int table_width,
                                                                  const int* __restrict__ first, const int* __restrict__ picked,
-                                                                 const int* __restrict__ cu, int n_pages, int heads, int page_tokens, int vecs,
-                                                                 unsigned pieces) {
+                                                                 const int* __restrict__ cu, int n_picked, int n_pages, int heads, int page_tokens,
+                                                                 int vecs, unsigned pieces) {
   __shared__ long from_s[ROWS], to_s[ROWS];
   pdl_launch_dependents();
   pdl_wait();
-  const int seq = blockIdx.y, lo = cu[seq], n = cu[seq + 1] - lo, held = first[seq];
+  const int seq = blockIdx.y, lo = max(cu[seq], 0), n = min(cu[seq + 1], n_picked) - lo, held = first[seq];
   const int* table = block_table + (size_t)seq * table_width;
   for (int i0 = 0; i0 < n; i0 += ROWS) {
     __syncthreads();
@@ -104,8 +104,8 @@ LB_EXPORT int lb_copy_pages(void* pool, const int* src, const int* dst, int n_pa
   });
 }
 
-LB_EXPORT int lb_compact_tokens(void* pool, const int* block_table, int table_width, const int* first, const int* picked, const int* cu, int n_seqs,
-                                int planes, int n_pages, int heads, int page_tokens, long row_bytes, cudaStream_t stream) {
+LB_EXPORT int lb_compact_tokens(void* pool, const int* block_table, int table_width, const int* first, const int* picked, const int* cu, int n_picked,
+                                int n_seqs, int planes, int n_pages, int heads, int page_tokens, long row_bytes, cudaStream_t stream) {
   if (n_seqs <= 0 || planes <= 0 || heads <= 0 || row_bytes <= 0) return 0;
   if (n_pages <= 0 || page_tokens <= 0 || table_width <= 0 || n_seqs > 65535) return LB_ERR_SIZE;
   return with_vector(row_bytes, pool, [&](auto vec) {
@@ -114,7 +114,7 @@ LB_EXPORT int lb_compact_tokens(void* pool, const int* block_table, int table_wi
     if (pieces > 0x7fffffffL) return (int)LB_ERR_SIZE;
     const long blocks = (pieces + THREADS - 1) / THREADS, each = (blocks * n_seqs + MOST_BLOCKS - 1) / MOST_BLOCKS;      // passes of a block
     lb_launch(compact_tokens_kernel<V>, dim3((unsigned)((blocks + each - 1) / each), n_seqs), THREADS, 0, stream, (V*)pool, block_table, table_width, first,
-              picked, cu, n_pages, heads, page_tokens, (int)vecs, (unsigned)pieces);
+              picked, cu, n_picked, n_pages, heads, page_tokens, (int)vecs, (unsigned)pieces);
     return lb_last_error();
   });
 }

@@ -56,20 +56,12 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _pointers(what: str, *tensors: torch.Tensor | None) -> list[int | None]:
     """The addresses of tensors that are all on the current CUDA device, on whose current stream the kernels are launched."""
-    current, found = None, []
-    for t in tensors:
-        if t is None:
-            found.append(None)
-            continue
-        device = t.get_device()
-        if device < 0:
-            raise KernelError("layover_b200 kernels need CUDA tensors: there is no CPU path")
-        if current is None:
-            current = torch._C._cuda_getDevice()
-        if device != current:
-            raise ValueError(f"{what}: the tensors must be on the current CUDA device")
-        found.append(t.data_ptr())
-    return found
+    devices = {t.get_device() for t in tensors if t is not None}
+    if min(devices) < 0:
+        raise KernelError("layover_b200 kernels need CUDA tensors: there is no CPU path")
+    if len(devices) > 1 or devices.pop() != torch._C._cuda_getDevice():
+        raise ValueError(f"{what}: the tensors must be on the current CUDA device")
+    return [None if t is None else t.data_ptr() for t in tensors]
 
 
 def _stream() -> int:
@@ -1349,19 +1341,19 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     16 (float32: of 4) up to 256. What is in a draft's keys and values reaches only the rows that see it, infinities and NaN too."""
     dtype, tokens = q.dtype, q.shape[0]
     _need(q, None, "q"); _need(out, dtype, "out"); _need(k_pool, dtype, "k_pool"); _need(v_pool, dtype, "v_pool")
-    for name, t, dims in (("block_table", block_table, 2), ("cu_q", cu_q, 1), ("ctx_len", ctx_len, 1), ("tree", tree, 2)):
-        _need(t, torch.int32, name)
-        if t.dim() != dims:
-            raise ValueError(f"attention_tree: {name} must have {dims} dimension(s)")
+    _need(block_table, torch.int32, "block_table"); _need(cu_q, torch.int32, "cu_q"); _need(ctx_len, torch.int32, "ctx_len"); _need(tree, torch.int32, "tree")
+    if (block_table.dim(), cu_q.dim(), ctx_len.dim(), tree.dim()) != (2, 1, 1, 2):
+        raise ValueError("attention_tree: block_table and tree must have 2 dimensions, cu_q and ctx_len 1")
     if q_heads < 1 or kv_heads < 1 or q_heads % kv_heads:
         raise ValueError(f"attention_tree: q_heads ({q_heads}) must be a multiple of kv_heads ({kv_heads})")
     pages, table_width, words = k_pool.shape[0], block_table.shape[1], tree.shape[1]
-    if q.shape != (tokens, q_heads * dim) or out.shape != q.shape or v_pool.shape != k_pool.shape or k_pool.shape != (pages, kv_heads, page_tokens, dim):
+    rows, pool = (tokens, q_heads * dim), (pages, kv_heads, page_tokens, dim)
+    if q.shape != rows or out.shape != rows or v_pool.shape != pool or k_pool.shape != pool:
         raise ValueError("attention_tree: q, out or the pools do not match the heads")
-    if tree.shape[0] != tokens or block_table.shape[0] < n_seqs or cu_q.shape[0] < n_seqs + 1 or ctx_len.shape[0] < n_seqs:
+    if tree.shape[0] != tokens or block_table.shape[0] < n_seqs or cu_q.numel() < n_seqs + 1 or ctx_len.numel() < n_seqs:
         raise ValueError("attention_tree: a row of tree per draft, a table row, an end and a length per sequence")
-    if max_nodes < 1 or max_ctx < 1 or window < 0 or softcap < 0:
-        raise ValueError("attention_tree: max_nodes and max_ctx are at least 1, window and softcap not negative")
+    if max_nodes < 1 or max_ctx < 1 or window < 0 or not softcap >= 0 or not 0 < scale < float("inf"):
+        raise ValueError("attention_tree: max_nodes and max_ctx are at least 1, window and softcap not negative, scale is positive")
     if max_nodes > 32 * words:
         raise ValueError(f"attention_tree: {max_nodes} drafts need {-(-max_nodes // 32)} words a row of tree, got {words}")
     if not window:
@@ -1385,7 +1377,7 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     global LAUNCHES
     device = q.device
     sms = sm_count(device)
-    if attention_tree_on_tcgen05(q_heads // kv_heads, dim, page_tokens, dtype):
+    if attention_tree_on_tcgen05(q_heads // kv_heads, dim, page_tokens, dtype) and out_ptr % 32 == 0:      # it stores 32 bytes a thread
         blocks, rows2, floats = tree_share(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, sms)
         scratch = torch.empty(floats, dtype=torch.float32, device=device)          # of this call alone, on its own stream
         fn = _FUNCTIONS.get("lb_attention_tree_tcgen05") or _fn("attention_tree", "lb_attention_tree_tcgen05",
@@ -1451,8 +1443,8 @@ def compact_tokens(pool: torch.Tensor, block_table: torch.Tensor, first: torch.T
     if pool.numel() == 0 or picked.numel() == 0 or block_table.shape[1] == 0:
         return pool
     fn = _FUNCTIONS.get("lb_compact_tokens") or _fn("cache_moves", "lb_compact_tokens",
-             [c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 5 + [c_long, c_void_p])
-    _check(fn(pool_ptr, table_ptr, block_table.shape[1], first_ptr, picked_ptr, cu_ptr, n_seqs, planes, pages, heads,
+             [c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 6 + [c_long, c_void_p])
+    _check(fn(pool_ptr, table_ptr, block_table.shape[1], first_ptr, picked_ptr, cu_ptr, picked.numel(), n_seqs, planes, pages, heads,
               page_tokens, channels * pool.element_size(), _stream()), "compact_tokens")
     return pool
 

@@ -76,7 +76,7 @@ class Trees:
     def run(self, **over):
         o = ops()
         d = {name: getattr(self, name).cuda() for name in ("q", "k_pool", "v_pool", "table", "cu_q", "ctx", "positions", "tree")}
-        out = torch.full_like(d["q"], 7.0)
+        out = torch.full((d["q"].numel() + over.get("shift", 0),), 7.0, dtype=d["q"].dtype, device="cuda")[over.get("shift", 0):].view_as(d["q"])
         o.attention_tree(d["q"], d["k_pool"], d["v_pool"], out, d["table"], d["cu_q"], d["ctx"], d["positions"] if self.window else None, d["tree"],
                          len(self.lengths), self.q_heads, self.kv_heads, self.dim, self.page, self.scale, over.get("max_nodes", self.max_nodes),
                          over.get("max_ctx", self.max_ctx), window=self.window, sinks=None if self.sinks is None else self.sinks.cuda(),
@@ -244,6 +244,11 @@ def test_tree_attention_bounds_may_be_larger_than_the_lengths(dtype):
     case.check(case.run(max_ctx=100))                      # planned for fewer keys: all are read all the same
 
 
+def test_tree_attention_writes_to_any_16_bytes():
+    case = Trees([(90, 4), (200, 9)], 8, 2, 128, seed=2).fill()
+    case.check(case.run(shift=8))
+
+
 # ------------------------------------------------------------------------------- moves in a cache
 @pytest.mark.parametrize("dtype, channels", [(torch.bfloat16, 128), (torch.float32, 20), (torch.bfloat16, 20), (torch.bfloat16, 7), (torch.float32, 256), (torch.int8, 3)])
 @pytest.mark.parametrize("page", [1, 5, 16])
@@ -276,6 +281,7 @@ def test_compaction_leaves_out_what_is_outside():
     before, put = pool.clone(), (lambda x: torch.tensor(x, dtype=torch.int32, device="cuda"))
     table = put([[0, 1, -1], [2, 99, 3]])
     o.compact_tokens(pool, table, put([2, 1]), put([7, 90, 100, 4, 6]), put([0, 3, 5]))      # page -1, behind the table, page 99
+    o.compact_tokens(pool, put([[0, 1, 2]]), put([0]), put([0, 1]), put([-9, 1000]))                                # ends behind the drafts that are there
     assert torch.equal(pool, before)
 
 

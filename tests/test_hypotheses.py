@@ -27,6 +27,7 @@ def tree_call(**over):
     (dict(tree=zeros(5, 2)[:, :1]), "contiguous"), (dict(q=zeros(64, 5, dtype=torch.bfloat16).T), "contiguous"), (dict(q_heads=3), "multiple of kv_heads"),
     (dict(kv_heads=0), "multiple of kv_heads"), (dict(dim=32), "do not match the heads"), (dict(page_tokens=8), "do not match the heads"),
     (dict(n_seqs=3), "a row of tree per draft"), (dict(max_nodes=33), "2 words"), (dict(max_nodes=0), "at least 1"), (dict(max_ctx=0), "at least 1"),
+    (dict(scale=0.0), "scale is positive"), (dict(scale=float("nan")), "scale is positive"),
     (dict(window=-1), "not negative"), (dict(softcap=-1.0), "not negative"), (dict(window=4, positions=None), "needs positions"),
     (dict(window=4, positions=zeros(4)), "a position per draft"), (dict(sinks=zeros(3, dtype=torch.float32)), "one sink"),
     (dict(q=zeros(5, 64, dtype=torch.float16), out=zeros(5, 64, dtype=torch.float16), k_pool=zeros(3, 2, 4, 16, dtype=torch.float16),

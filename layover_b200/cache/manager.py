@@ -38,6 +38,7 @@ which is how the scheduler and the property tests use it.
 
 from __future__ import annotations
 
+from collections import Counter
 from dataclasses import dataclass, field
 
 import torch
@@ -490,11 +491,11 @@ class CacheManager:
         for index, group in enumerate(self.paged):
             group.allocator.check()
             held = [b for seq in self.live.values() for b in seq.tables[index].blocks if b != group.scratch_page]
-            for block in set(held):
-                if held.count(block) != max(1, group.allocator.holders(block)):
-                    raise AssertionError("a page is held by two tables")
-            if len(set(held)) != group.allocator.num_used:
-                raise AssertionError(f"{group.allocator.num_used} pages are out, {len(set(held))} are in tables")
+            counts = Counter(held)
+            if any(count != max(1, group.allocator.holders(block)) for block, count in counts.items()):
+                raise AssertionError("a page is held by two tables")
+            if len(counts) != group.allocator.num_used:
+                raise AssertionError(f"{group.allocator.num_used} pages are out, {len(counts)} are in tables")
             for block in held:
                 if not group.allocator.is_held(block):
                     raise AssertionError(f"page {block} is in a table and on the free list")

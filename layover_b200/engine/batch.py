@@ -12,7 +12,8 @@ side; the tokens of all entries are laid end to end:
   row_slots [R]                       the state slot of the request that each of those rows belongs to
   token_src [T]                       state slot whose record holds the token (still on the device), or -1
   tree [T, words]                     only where an entry brings drafts (`StepEntry.parents`): bit j of a row says whether the
-                                      token sees token j of its own entry; positions are then those of the tree's levels
+                                      token sees token j of its own entry; positions are then those of the tree's levels. A group
+                                      whose window is shorter than a branch has a tree of its own
   per paged cache group:
     block_table [S, W]                page ids, padded with the group's scratch page
     slot_map [T]                      page * page_tokens + slot where the token's K and V go
@@ -63,10 +64,20 @@ def tree_rows(parents: list[int]) -> tuple[list[int], list[int]]:
     return seen, level
 
 
+def tree_rows_in_window(parents: list[int], seen: list[int], window: int) -> list[int]:
+    """What each token of a tree sees of it behind a window: itself and the `window - 1` ancestors before it."""
+    lines, rows = [], []
+    for i, p in enumerate(parents):
+        lines.append((lines[p] if p >= 0 else []) + [i])
+        rows.append(seen[i] & ~seen[lines[i][-1 - window]] if len(lines[i]) > window else seen[i])
+    return rows
+
+
 @dataclass
 class GroupBatch:
     block_table: torch.Tensor
     slot_map: torch.Tensor
+    tree: torch.Tensor | None = None     # the batch's, but for what the group's window hides
 
 
 @dataclass
@@ -217,9 +228,14 @@ class BatchBuilder:
             for e in entries:
                 if e.parents is not None and len(e.parents) != len(e.tokens):
                     raise ValueError(f"request {e.seq.request_id!r}: a parent per drafted token")
-            trees = [tree_rows(e.parents if e.parents is not None else list(range(-1, len(e.tokens) - 1))) for e in entries]
+            parents = [e.parents if e.parents is not None else list(range(-1, len(e.tokens) - 1)) for e in entries]
+            trees = [tree_rows(p) for p in parents]
             words = -(-max(q_lens) // 32)
             layout.add("tree", n_tokens, words)
+            longest = 1 + max(max(level) for _, level in trees)
+            windows = [g.need.window if g.need.window and g.need.window < longest else 0 for g in cache.paged]
+            for window in set(windows) - {0}:
+                layout.add(f"tree{window}", n_tokens, words)
         singles = [s for s, n in enumerate(q_lens) if n == 1]
         mixed = 0 < len(singles) < n_seqs
         portion_lists = {}
@@ -254,9 +270,10 @@ class BatchBuilder:
             if drafts:
                 seen, level = trees[index]
                 view[pos_at + at: pos_at + at + n] = np.array(level, dtype=np.int32) + starts[index]
-                where = layout.fields["tree"][0] + at * words
-                rows_of = np.frombuffer(b"".join(s.to_bytes(4 * words, "little") for s in seen), dtype=np.int32)
-                view[where: where + n * words] = rows_of
+                for window in {0, *windows}:
+                    where = layout.fields[f"tree{window or ''}"][0] + at * words
+                    bits = tree_rows_in_window(parents[index], seen, window) if window else seen
+                    view[where: where + n * words] = np.frombuffer(b"".join(b.to_bytes(4 * words, "little") for b in bits), dtype=np.int32)
             if n == 1 and entry.tokens[0] < 0:          # the request's newest token is in its record on the device
                 view[ids_at + at] = 0
                 view[src_at + at] = entry.seq.slot
@@ -332,7 +349,8 @@ class BatchBuilder:
             token_ids=get("token_ids"), positions=get("positions"), cu_q=get("cu_q"), ctx_len=get("ctx_len"),
             state_slots=get("state_slots"), logit_rows=get("logit_rows"), n_logit_rows=n_rows,
             row_slots=get("row_slots"), token_src=get("token_src"), device_tokens=device_tokens,
-            groups=[GroupBatch(get(f"table{g}"), get(f"slots{g}")) for g in range(len(cache.paged))],
+            groups=[GroupBatch(get(f"table{g}"), get(f"slots{g}"), get(f"tree{windows[g] or ''}") if drafts else None)
+                    for g in range(len(cache.paged))],
             tiles={size: QueryTiles(get(f"tile_seq{size}"), get(f"tile_q0{size}"), len(tiles))
                    for size, tiles in tile_lists.items()},
             decode_seqs=get("decode_seqs") if mixed else None, n_decode_seqs=len(singles) if mixed else 0,

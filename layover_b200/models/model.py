@@ -104,10 +104,14 @@ class Model:
 
     @property
     def takes_drafts(self) -> bool:
-        """Whether a step may bring drafted tokens that form a tree: every mixer attends, without further options."""
+        """Whether a step may bring drafted tokens that form a tree: every mixer attends, without further options, and behind the window
+        of the pages that it reads."""
         from ..parts.attention import Attention
 
-        return all(isinstance(getattr(block, "mixer", None), Attention) and not block.mixer.general for block in self.blocks)
+        mixers = [getattr(block, "mixer", None) for block in self.blocks]
+        schedule = self.spec.schedule
+        return all(isinstance(m, Attention) and not m.general for m in mixers) and all(
+            e.reads_cache_of is None or mixers[e.layer].window == mixers[schedule[e.reads_cache_of].layer].window for e in schedule)
 
     def tile_sizes(self) -> tuple[int, ...]:
         """Query-tile sizes that the parts want listed in every batch."""

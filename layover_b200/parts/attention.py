@@ -363,7 +363,7 @@ class Attention(Part):
 
     def attend(self, q, cache, batch, group, out) -> None:
         if batch.tree is not None:           # drafts that see their own ancestors, not all that came before them
-            ops.attention_tree(q, cache.k_pool, cache.v_pool, out, group.block_table, batch.cu_q, batch.ctx_len, batch.positions, batch.tree,
+            ops.attention_tree(q, cache.k_pool, cache.v_pool, out, group.block_table, batch.cu_q, batch.ctx_len, batch.positions, group.tree,
                                batch.n_seqs, self.q_heads, self.kv_heads, self.dim, cache.page_tokens, self.scale, batch.max_q_len, batch.max_ctx,
                                window=self.window or 0)
             return

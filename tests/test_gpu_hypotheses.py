@@ -504,6 +504,40 @@ def test_a_step_over_drafts_and_what_follows_it(served, name):
     assert ops().attention_tree_status() == 0
 
 
+@pytest.mark.parametrize("window", [1, 3, 16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_drafts_behind_a_window_shorter_than_their_branch(tiny_folders, window, dtype):
+    """As token by token: a window counts drafts too, and the tokens of a portion that shares the step."""
+    import layover_b200 as lb
+    from conftest import random_prompt, tolerance
+    from test_gpu_engine import build_toy
+    model = build_toy(tiny_folders, "a", dtype, window=window)[0]
+    assert model.takes_drafts
+    cache, step = fresh(model)
+    vocab = model.spec.vocab_size
+    prompt, other = random_prompt(vocab, 45, 1), random_prompt(vocab, 40, 3)
+    parents = [-1, 0, 0, 1, 1, 2, *range(5, 30)]
+    tokens = random_prompt(vocab, len(parents), 2)
+    seq, _ = feed(cache, step, "x", prompt)
+    beside = cache.open("y")
+    logits = step([lb.StepEntry(seq, tokens, list(range(len(tokens))), parents), lb.StepEntry(beside, other, [39])]).clone()
+    for i in (0, 2, 4, 8, 20, len(tokens) - 1):
+        branch, at = [], i
+        while at >= 0:
+            branch, at = [tokens[at], *branch], parents[at]
+        one, want = feed(cache, step, f"branch {i}", prompt + branch)
+        assert (logits[i] - want).abs().max().item() <= tolerance(want, model.dtype)
+        cache.close(one)
+    _, want = feed(cache, step, "alone", other)
+    assert (logits[-1] - want).abs().max().item() <= tolerance(want, model.dtype)
+    path = [0, 2, *range(5, 25)]
+    cache.accept([(seq, path)])
+    cache.check()
+    got = step([lb.StepEntry(seq, [3], [0])])[0].clone()
+    _, want = feed(cache, step, "after", prompt + [tokens[i] for i in path] + [3])
+    assert (got - want).abs().max().item() <= tolerance(want, model.dtype)
+
+
 @pytest.mark.parametrize("name", ["a", "c"])
 def test_forked_requests_go_their_own_ways(served, name):
     import layover_b200 as lb

@@ -288,6 +288,24 @@ def test_a_batch_carries_the_tree_of_its_drafts():
         BatchBuilder(m, torch.device("cpu")).build([StepEntry(a, [5, 6], parents=[-1])])
 
 
+def test_a_window_hides_ancestors_from_a_draft():
+    """Groups whose window is shorter than a branch have a tree of their own, also for a portion beside the drafts."""
+    from layover_b200.engine.batch import BatchBuilder, StepEntry, tree_rows, tree_rows_in_window
+
+    PagedKVNeed = __import__("layover_b200").parts.base.PagedKVNeed
+    m = manager([PagedKVNeed(2, 16, None), PagedKVNeed(2, 16, 2), PagedKVNeed(2, 16, 5)], blocks=40)
+    a, b = m.open("a"), m.open("b")
+    m.grow(a, 7); m.commit(a, 7)
+    m.grow(a, 7 + 5); m.grow(b, 4)
+    parents = [-1, 0, 0, 2, 3]
+    batch = BatchBuilder(m, torch.device("cpu")).build([StepEntry(a, [5, 6, 7, 8, 9], [0, 3], parents=parents), StepEntry(b, [1, 2, 3, 4])])
+    trees = [g.tree.flatten().tolist() for g in batch.groups]
+    assert trees[0] == trees[2] == batch.tree.flatten().tolist() == [0b1, 0b11, 0b101, 0b1101, 0b11101, 0b1, 0b11, 0b111, 0b1111]
+    assert trees[1] == [0b1, 0b11, 0b101, 0b1100, 0b11000, 0b1, 0b11, 0b110, 0b1100]
+    seen, _ = tree_rows(parents)
+    assert tree_rows_in_window(parents, seen, 1) == [1 << i for i in range(5)] and tree_rows_in_window(parents, seen, 9) == seen
+
+
 def test_lookup_drafts_and_the_walk_down_them():
     import layover_b200 as lb
     from layover_b200.engine.drafts import walk

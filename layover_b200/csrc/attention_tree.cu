@@ -22,6 +22,13 @@
 // The values of a draft may be anything (a draft whose arithmetic overflowed): what a row does not see must not reach it, and
 // 0 x NaN is NaN. So in tiles that hold drafts, value rows that are not finite are taken out of the product and added one by
 // one to the rows that see them.
+//
+// Bounds. bfloat16: the keys' and values' bytes and, with few keys, the time to start two launches and to reach a page through its
+// table; 5 requests of 13 drafts behind a window of 1,024, 12 heads over 2 of 64 channels 16.5 us. 32 bits: 2 x rows x keys x dim FFMA a
+// head, 11 us at the pipes' rate for 4 requests of 13 drafts after 900 keys, 32 heads over 8 of 128 (32 MB: 4.9 us), measured 63 us:
+// three instructions are issued for every one of those (reads of shared memory, the weights doubled for two products an instruction),
+// half of the cycles issue none (waits for shared memory and for sums before). Tiles of 64 keys, two blocks an SM: 74; one product an
+// instruction before that 204.
 #include <math.h>
 
 #include <type_traits>

@@ -15,8 +15,8 @@
 // chunks' lists the candidates are compared in 64 bits behind a threshold of the same kind, where two beams' tie only where the formula's
 // do within 1e-7; where more reach it than there is room for (many equal ones), the best are picked one by one.
 //
-// The logits' bytes bound it in theory. Measured (one B200): 128 rows of 151,936, a fifth of the beams ended, 16 kept 33 us, of them 24 the
-// first kernel (3.2 TB/s of what it reads: a block's first piece, its thresholds and ranking run alone), 4 rows 8.1 us, two launches
+// The logits' bytes bound it in theory. Measured (one B200): 128 rows of 151,936, a fifth of the beams ended, 16 kept 30 us, of them 22 the
+// first kernel (3 TB/s of what it reads: a block's first piece, its thresholds and ranking run alone), 64 rows 14.3 us, 4 rows 8.0 us, two launches
 // of about 4 that wait for memory twice.
 #include <float.h>
 #include <math.h>
@@ -111,7 +111,7 @@ __device__ __forceinline__ float reached_by(float top, int keep, int* keys, floa
 
 // stats [rows][chunks] (maximum, sum of exp(x - maximum)), lists [rows][chunks][keep] of (value, index), best first, (-inf, NONE) behind the last.
 // A chunk is `pieces` of PIECE values. Rows of beams that are not there or have ended are not read, and nothing is written for them.
-constexpr int EACH = 16, PIECE = THREADS * EACH;
+constexpr int EACH = 14, PIECE = THREADS * EACH;
 __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const float* __restrict__ logits, long row_stride, const float* __restrict__ scores,
                                                                 const int* __restrict__ ended, int vocab, int keep, int pieces,
                                                                 float2* __restrict__ stats, float2* __restrict__ lists) {
@@ -321,7 +321,6 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const float* __restr
 
 // A block of the first kernel takes `pieces` of lb_beam_piece() values, chunks = ceil(vocab / (pieces * lb_beam_piece())). Scratch: rows * chunks * (2 + 2
 // keep) words.
-LB_EXPORT int lb_beam_piece() { return PIECE; }
 LB_EXPORT int lb_beam_select(const float* logits, long row_stride, const float* scores, const int* ended, int requests, int beams, int vocab, int keep,
                              int pad, int pieces, void* scratch, long scratch_words, float* next_scores, int* parents, int* tokens, cudaStream_t stream) {
   if (requests <= 0) return 0;

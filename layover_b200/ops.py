@@ -1453,15 +1453,16 @@ BEAM_MAX_KEEP = 32      # the most continuations that `beam_select` chooses
 BEAM_MAX_BEAMS = 64     # the most beams of a request
 
 
-_BEAM_PIECE = 4096      # values of a row that a block of the first kernel looks at together (csrc/beam.cu)
+_BEAM_PIECE = 3584      # values of a row that a block of the first kernel looks at together (csrc/beam.cu)
 
 
 def _beam_pieces(rows: int, vocab: int, sms: int) -> int:
-    """Pieces of a row that one block takes: 2 to 5, by the pieces there are for the SMs. The first costs the block most, but what is left
-    over runs alone. Measured (one B200, us; 2, 4, 5, 6 and 8 pieces): 128 rows of 151,936 41.5, 33.9, 32.8, 33.1 and 32.4 (5 are taken), 64 rows
-    18.2, 17.4, 16.1, 16.9 and 18.5 (5), 16 rows 11.1, 10.4, 10.6, 11.3 and 12.1 (2), 4 rows 8.1, 9.3, 9.7, 10.2 and 11.4 (2), 32 rows of
-    32,768 with 32 kept 19.6, 19.9, 21.5, 23.2 and 24.6 (2)."""
-    return min(5, max(2, -(-10 * rows * -(-vocab // _BEAM_PIECE) // (34 * sms))))
+    """Pieces of a row that one block takes: few where blocks are few, more where several blocks wait for an SM's place (the first costs a
+    block most) and where the second kernel has many chunks to join. Measured (one B200, us; 2, 3, 5, 6 and 9 pieces): 128 rows of 151,936
+    42.7, 35.5, 30.8, 29.9 and 29.4 (6 are taken), 64 rows 18.0, 16.7, 14.3, 15.1 and 16.8 (5), 16 rows 10.8, 10.7, 9.7, 10.2 and 10.8 (5), 32
+    rows of 32,768 with 32 kept 25.1, 20.6, 19.6, 20.8 and 24.4 (5), 4 rows of 151,936 with 2, 3, 4 and 5 8.2, 8.0, 8.2 and 8.7 (3)."""
+    pieces = rows * -(-vocab // _BEAM_PIECE)
+    return 3 if pieces <= 2 * sms else 5 if pieces <= 20 * sms else 6
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, next_scores: torch.Tensor, parents: torch.Tensor, tokens: torch.Tensor,

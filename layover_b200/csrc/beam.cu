@@ -15,8 +15,8 @@
 // chunks' lists the candidates are compared in 64 bits behind a threshold of the same kind, where two beams' tie only where the formula's
 // do within 1e-7; where more reach it than there is room for (many equal ones), the best are picked one by one.
 //
-// The logits' bytes bound it in theory. Measured (one B200): 128 rows of 151,936, a fifth of the beams ended, 16 kept 30 us, of them 22 the
-// first kernel (3 TB/s of what it reads: a block's first piece, its thresholds and ranking run alone), 64 rows 14.3 us, 4 rows 8.0 us, two launches
+// The logits' bytes bound it in theory. Measured (one B200): 128 rows of 151,936, a fifth of the beams ended, 16 kept 26 us, of them 18 to 20 the
+// first kernel (3.3 TB/s of what it reads: a block's first piece, its thresholds and ranking run alone), 64 rows 14 us, 4 rows 8 us, two launches
 // of about 4 that wait for memory twice.
 #include <float.h>
 #include <math.h>
@@ -226,6 +226,13 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const float* __restr
   pdl_wait();
   const int request = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_lists = beams * chunks;
   const float2* mine = lists + (size_t)request * n_lists * keep;
+  // A thread's candidates, of all lists' one after the other; those of the four threads of a group lie 64 apart, so that what is best of a list is in
+  // several groups. The first four are on their way while the sums are joined.
+  const int n_candidates = n_lists * keep, at0 = (threadIdx.x & 3) * 64 + (threadIdx.x >> 2);
+  constexpr int FIRST = 4;
+  float2 held[FIRST];
+#pragma unroll
+  for (int k = 0; k < FIRST; ++k) held[k] = at0 + k * THREADS < n_candidates ? mine[at0 + k * THREADS] : make_float2(-INFINITY, 0.f);
   for (int b = warp; b < beams; b += WARPS) {
     const size_t row = (size_t)request * beams + b;
     const float score = scores[row];
@@ -248,9 +255,8 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const float* __restr
   }
   if (threadIdx.x == 0) count = 0;
   __syncthreads();
-  // candidate c, of all lists' one after the other: an ended beam has one, in its first list
-  const int n_candidates = n_lists * keep;
-  auto candidate = [&](int c, double& v, int& i) {
+  // candidate c, which the lists have as x: an ended beam has one, in its first list
+  auto candidate = [&](int c, float2 x, double& v, int& i) {
     const int l = c / keep, b = l / chunks;
     v = -INFINITY; i = NONE;
     if (offsets[b] == -INFINITY) return;
@@ -258,30 +264,36 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const float* __restr
       if (c == b * chunks * keep) { v = offsets[b]; i = b * vocab + pad; }
       return;
     }
-    const float2 x = mine[c];
     if (x.x > -INFINITY) { v = offsets[b] + (double)x.x; i = b * vocab + __float_as_int(x.y); }
   };
+  auto all = [&](auto look) {
+#pragma unroll
+    for (int k = 0; k < FIRST; ++k) {
+      double v;
+      int i;
+      if (at0 + k * THREADS >= n_candidates) return;
+      candidate(at0 + k * THREADS, held[k], v, i);
+      look(v, i);
+    }
+    for (int c = at0 + FIRST * THREADS; c < n_candidates; c += THREADS) {
+      double v;
+      int i;
+      candidate(c, mine[c], v, i);
+      look(v, i);
+    }
+  };
   double best = -INFINITY;
-  for (int c = threadIdx.x; c < n_candidates; c += THREADS) {
-    double v;
-    int i;
-    candidate(c, v, i);
-    if (v > best) best = v;
-  }
-  // groups of threads 64 apart: what is best of a list lies in different ones
+  all([&](double v, int) { best = v > best ? v : best; });
   // a value that `keep` candidates reach; the lowest one stands for none
   const float lowest = reached_by(__double2float_rd(best), keep, keys, &threshold);
   const double reach = lowest == -FLT_MAX ? -INFINITY : (double)lowest;
   if (best >= reach)
-    for (int c = threadIdx.x; c < n_candidates; c += THREADS) {
-      double v;
-      int i;
-      candidate(c, v, i);
+    all([&](double v, int i) {
       if (v >= reach && i != NONE) {
         const int at = atomicAdd(&count, 1);
         if (at < ROOM) { values[at] = v; indices[at] = i; }
       }
-    }
+    });
   __syncthreads();
   const int n = count;
   auto choose = [&](int k, double v, int i) {
@@ -305,12 +317,9 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const float* __restr
     for (int k = 0; k < keep; ++k) {
       double v = -INFINITY;
       int i = NONE;
-      for (int c = threadIdx.x; c < n_candidates; c += THREADS) {
-        double w;
-        int j;
-        candidate(c, w, j);
+      all([&](double w, int j) {
         if (j != NONE && before(last, last_index, w, j) && before(w, j, v, i)) { v = w; i = j; }
-      }
+      });
       block_best(v, i, part, part_index);
       if (threadIdx.x == 0) choose(k, v, i);
       last = v; last_index = i;
@@ -319,8 +328,7 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const float* __restr
 }
 }  // namespace
 
-// A block of the first kernel takes `pieces` of lb_beam_piece() values, chunks = ceil(vocab / (pieces * lb_beam_piece())). Scratch: rows * chunks * (2 + 2
-// keep) words.
+// A block of the first kernel takes `pieces` of PIECE values, chunks = ceil(vocab / (pieces * PIECE)). Scratch: rows * chunks * (2 + 2 keep) words.
 LB_EXPORT int lb_beam_select(const float* logits, long row_stride, const float* scores, const int* ended, int requests, int beams, int vocab, int keep,
                              int pad, int pieces, void* scratch, long scratch_words, float* next_scores, int* parents, int* tokens, cudaStream_t stream) {
   if (requests <= 0) return 0;

@@ -244,6 +244,50 @@ def test_tree_attention_bounds_may_be_larger_than_the_lengths(dtype):
     case.check(case.run(max_ctx=100))                      # planned for fewer keys: all are read all the same
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nodes, most", [(9, 3), (70, 5), (70, 40)])
+def test_tree_attention_leaves_drafts_behind_the_most_alone(nodes, most, dtype):
+    """Rows of drafts behind `max_nodes` stay as they are; the others are as they would be."""
+    case = Trees([(300, nodes), (40, 2), (0, nodes)], 8, 2, 128, dtype=dtype, seed=nodes).fill()
+    whole, got = case.run(), case.run(max_nodes=most)
+    case.check(whole)
+    for first, n in ((0, nodes), (nodes, 2), (nodes + 2, nodes)):
+        assert (got[first + min(n, most): first + n] == 7.0).all()
+    keep = torch.cat([torch.arange(f, f + min(n, most)) for f, n in ((0, nodes), (nodes, 2), (nodes + 2, nodes))])
+    whole[keep] = got[keep]
+    case.check(whole)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tree_attention_of_very_many_requests(dtype):
+    """More than a block keeps the lengths of; some bring no drafts, some hold nothing."""
+    gen = torch.Generator().manual_seed(3)
+    held, nodes = torch.randint(0, 90, (700,), generator=gen).tolist(), torch.randint(0, 4, (700,), generator=gen).tolist()
+    Trees(list(zip(held, nodes)), 2, 1, 128, dtype=dtype, seed=4).fill().check()
+
+
+@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 128)])
+def test_pages_behind_2_to_the_31_values(dtype, dim):
+    """The same rows in a small pool and at the end of one of over 2^31 values: attention, compaction and copies."""
+    o, (held, n, heads, page) = ops(), (70, 9, 2, 16)
+    gen = torch.Generator().manual_seed(6)
+    put = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    pages, far = 8, (1 << 31) // (heads * page * dim) + 10
+    small = torch.randn(2, pages, heads, page, dim, generator=gen).to(dtype).cuda()
+    q, tree = torch.randn(n, 8 * dim, generator=gen).to(dtype).cuda(), words_of(seen_of(random_tree(gen, n)), 1).cuda()
+    big = torch.empty(2, far, heads, page, dim, dtype=dtype, device="cuda")
+    big[:, -pages:] = small
+    outs = []
+    for pool in (small, big):
+        first = pool.shape[1] - pages
+        table, out = put([[first + i for i in (5, 1, 7, 0, 3)]]), torch.empty_like(q)
+        o.attention_tree(q, pool[0], pool[1], out, table, put([0, n]), put([held + n]), None, tree, 1, 8, heads, dim, page, dim ** -0.5, n, held + n)
+        o.compact_tokens(pool, table, put([held]), put([1, 4, 8]), put([0, 3]))
+        o.copy_pages(pool, put([first + 5, first + 1]), put([first + 2, first + 4]))
+        outs.append((out.cpu(), pool[:, first:].cpu()))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
 def test_tree_attention_writes_to_any_16_bytes():
     case = Trees([(90, 4), (200, 9)], 8, 2, 128, seed=2).fill()
     case.check(case.run(shift=8))
@@ -381,6 +425,16 @@ def test_beam_selection_of_masked_beams_and_tokens():
     for keep in (3, 8, 32):
         check_beams(logits.cuda(), scores, keep)
         check_beams(logits.cuda(), scores, keep, torch.tensor([[0, 1, 1], [0, 0, 1], [1, 1, 0], [1, 0, 1]], dtype=torch.int32), pad=2999)
+
+
+def test_beam_selection_of_the_most_beams():
+    gen = torch.Generator().manual_seed(12)
+    logits = torch.randn(2 * 64, 30_000, generator=gen).cuda()
+    logits[5] = 0.25                                   # a row of equal ones among the others
+    check_beams(logits, -3 * torch.rand(2, 64, generator=gen), 32)
+    few = torch.randn(3, 2, generator=gen).cuda()      # fewer candidates than places
+    values, parents, tokens = select(few, torch.zeros(1, 3), 32)
+    assert parents[0, :6].min() >= 0 and (parents[0, 6:] == -1).all() and (values[0, 6:] == -INF).all() and (tokens[0, 6:] == -1).all()
 
 
 def test_beam_selection_does_not_read_beams_that_are_over():

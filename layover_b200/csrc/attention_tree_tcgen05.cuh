@@ -795,7 +795,8 @@ __global__ void __launch_bounds__(JOIN_THREADS, 4) join_kernel(const __grid_cons
     }
     if (__any_sync(0xffffffffu, odd)) {
       const Sequence s = find_sequence<ROWS2>(a, a.cu_q[border.seq], a.cu_q[border.seq + 1], a.ctx_len[border.seq]);
-      for (int r = warp; r < rows; r += warps) {
+      const int here = (rows + JOIN_ROWS - 1) / JOIN_ROWS * (JOIN_THREADS / 32);      // warps of the blocks that come here
+      for (int r = warp; r < rows; r += here) {
         const int d = r / a.group;
         row_key_by_key(a, s, border.seq, border.head, border.token + d, border.head * a.group + r - d * a.group);
       }

@@ -214,6 +214,15 @@ def test_a_draft_that_is_not_finite_reaches_only_who_sees_it(q_heads, kv_heads, 
     assert torch.equal(torch.nan_to_num(rest, 99.0), torch.nan_to_num(clean[:nodes][~touched], 99.0)) and torch.equal(got[nodes:2 * nodes], clean[nodes:2 * nodes])
 
 
+@pytest.mark.parametrize("nodes, others, held", [(5, 30, 3000), (10, 32, 500), (3, 60, 2000), (40, 64, 9000)])
+def test_drafts_that_are_not_finite_beside_larger_trees(nodes, others, held):
+    """All rows of a small tree are made again where the launch is planned for larger ones."""
+    case = Trees([(held, nodes), (held, others), (20, nodes)], 8, 2, 128, seed=nodes)
+    for seq in (0, 2):
+        case.v[seq][-nodes + 1, 0, 3], case.v[seq][-1, 1, 77] = NAN, INF
+    case.fill().check()
+
+
 def test_tree_attention_of_large_scores():
     """Scores far apart: the weights of all but one key vanish, and nothing overflows."""
     for dtype in (torch.bfloat16, torch.float32):

@@ -18,7 +18,7 @@
 // through parts of it each, on nothing, while the first loads are under way.
 //
 // The keys' and values' bytes bound it. Measured (one B200): 40 requests of 25 drafts after 400 .. 8,000 keys, 32 heads over 8, 155 us (734 MB,
-// 4.7 TB/s); 8 of 32 after 3,000 38 us (104 MB); 2 of 64 after 12,345, 16 over 4, 47 to 51 us (52 MB), 12 of them the join of 18
+// 4.7 TB/s); 8 of 32 after 3,000 38 us (104 MB); 2 of 64 after 12,345, 16 over 4, 46 to 48 us (52 MB), 9 of them the join of 18
 // parts a row; 1 of 8 after 700 12.7 us. What is left is time in which nothing streams: about 4 us until a block's share is known and 4 more
 // until its first scores, 4 to 6 at the border of two segments (partial tiles, results to be stored, instructions that run for the first
 // time), and the join. The same by mma.sync, the rows' keys in chunks: 843, 202 and 167 us.
@@ -752,7 +752,7 @@ __device__ __noinline__ void share_key_by_key(const TreeArgs& a, int b, int bloc
 // The parts of the rows whose keys lie in several blocks' shares, in the order of the keys: eight lanes a row, 16 channels each.
 constexpr int JOIN_THREADS = 256, JOIN_ROWS = JOIN_THREADS / 8;
 template <bool ROWS2>
-__global__ void __launch_bounds__(JOIN_THREADS, 4) join_kernel(const __grid_constant__ TreeArgs a, int blocks) {
+__global__ void __launch_bounds__(JOIN_THREADS, ROWS2 ? 2 : 4) join_kernel(const __grid_constant__ TreeArgs a, int blocks) {
   pdl_launch_dependents();
   pdl_wait();
   const Border border = a.borders[blockIdx.x];
@@ -768,23 +768,28 @@ __global__ void __launch_bounds__(JOIN_THREADS, 4) join_kernel(const __grid_cons
     const float2* stats = reinterpret_cast<const float2*>(a.partials + a.partial_stats);
     float top = a.sinks && row < rows ? a.sinks[row_head] * LOG2E : -INFINITY, total = a.sinks ? 1.f : 0.f;
     float4 sum[4] = {};
-    for (int p0 = border.from; p0 <= border.upto; p0 += 2) {        // two parts on their way at once
-      float2 ml[2];
-      float4 v[2][4];
+    // Parts on their way: tiles of 256 rows are few and have many (2 requests x 64 drafts after 12,345, us for two and four at once: 47.1, 45.6).
+    constexpr int AT_ONCE = ROWS2 ? 4 : 2;
+    for (int p0 = border.from; p0 <= border.upto; p0 += AT_ONCE) {
+      float2 ml[AT_ONCE];
+      float4 v[AT_ONCE][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < AT_ONCE; ++j) {
         const long at = place(min(p0 + j, border.upto));
         ml[j] = stats[at];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[j][i] = *reinterpret_cast<const float4*>(a.partials + at * DIM + channel + 32 * i);
         if (p0 + j > border.upto) ml[j].x = -INFINITY;
       }
-      const float m = fmaxf(fmaxf(ml[0].x, ml[1].x), top), base = m == -INFINITY ? 0.f : m, keep = exp2f(top - base);
+      float m = top;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) m = fmaxf(m, ml[j].x);
+      const float base = m == -INFINITY ? 0.f : m, keep = exp2f(top - base);
       total *= keep;
 #pragma unroll
       for (int i = 0; i < 4; ++i) { sum[i].x *= keep; sum[i].y *= keep; sum[i].z *= keep; sum[i].w *= keep; }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < AT_ONCE; ++j) {
         const float w = exp2f(ml[j].x - base);
         if (w == 0.f) continue;
         total += w * ml[j].y;

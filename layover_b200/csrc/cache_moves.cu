@@ -5,6 +5,10 @@
 // Both are bound by memory: every byte that moves is read once and written once. Measured (one B200): 56 pages of 72 planes, 216 MB in all, 38
 // us (5.7 TB/s of 6.5), 24 states of 2 MB in 3 layers 42 us (6.0), the accepted rows of 64 requests, 55 MB, 17.6 us (3.1: rows of 256
 // bytes in 72 x 8 places each), of one request 3.2 us.
+//
+// Neither kernel lets its dependents start early, and each thread's last act is to make its writes visible to the whole device: decode
+// attention reads a cache's earlier keys ahead of its wait, which is sound only where no kernel that may still run writes them. So
+// whatever is launched behind a move, or behind others that are, starts when the rows have been moved.
 #include "common.cuh"
 
 namespace {
@@ -17,7 +21,6 @@ constexpr int COPY_UNROLL = 4;      // vectors of a thread that are on their way
 template <typename V>
 __global__ void __launch_bounds__(THREADS) copy_pages_kernel(V* __restrict__ pool, const int* __restrict__ src, const int* __restrict__ dst,
                                                              int n_pages, long vecs) {
-  pdl_launch_dependents();
   pdl_wait();
   const int from = src[blockIdx.y], to = dst[blockIdx.y];
   if ((unsigned)from >= (unsigned)n_pages || (unsigned)to >= (unsigned)n_pages || from == to) return;
@@ -32,6 +35,7 @@ __global__ void __launch_bounds__(THREADS) copy_pages_kernel(V* __restrict__ poo
 #pragma unroll
   for (int i = 0; i < COPY_UNROLL; ++i)
     if (at + i * THREADS < vecs) b[at + i * THREADS] = v[i];
+  __threadfence();
 }
 
 // pool [planes][pages][heads][page_tokens][vecs of a row]. Sequence s keeps its drafts picked[cu[s]] < picked[cu[s] + 1] < ...: the
@@ -45,7 +49,6 @@ __global__ void __launch_bounds__(THREADS) compact_tokens_kernel(V* __restrict__
                                                                  const int* __restrict__ cu, int n_picked, int n_pages, int heads, int page_tokens,
                                                                  int vecs, unsigned pieces) {
   __shared__ long from_s[ROWS], to_s[ROWS];
-  pdl_launch_dependents();
   pdl_wait();
   const int seq = blockIdx.y, lo = max(cu[seq], 0), n = min(cu[seq + 1], n_picked) - lo, held = first[seq];
   const int* table = block_table + (size_t)seq * table_width;
@@ -80,6 +83,7 @@ __global__ void __launch_bounds__(THREADS) compact_tokens_kernel(V* __restrict__
         if (from_s[i] >= 0) plane[to_s[i]] = v[i];
     }
   }
+  __threadfence();
 }
 
 // the widest vector that divides a row of `bytes` bytes and the pool's alignment

@@ -85,7 +85,8 @@ static inline int lb_last_error() { return (int)cudaGetLastError(); }
 // a matrix product already streams weights that no kernel is writing) and then wait in `pdl_wait()` until the predecessor has
 // finished and its writes are visible. Every kernel calls `pdl_wait()` before it touches memory
 // that an earlier kernel wrote or that a later kernel may still read, so completion is
-// transitive along the stream. LAYOVER_B200_PDL=0 launches the plain way.
+// transitive along the stream. Decode attention alone reads earlier keys, tables and lengths ahead of its wait: a kernel that writes
+// those outside a step (cache_moves.cu) does not call `pdl_launch_dependents()`. LAYOVER_B200_PDL=0 launches the plain way.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

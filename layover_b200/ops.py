@@ -1413,7 +1413,8 @@ def attention_tree_status() -> int:
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
     """pool[:, dst[i]] = pool[:, src[i]] for every i: pool [planes, pages, ...] of any type (the layers' pages of a cache, or the
     layers' state slots), src and dst int32 [n] on the device. A page may be the source of several copies; no page is written twice or
-    read and written in one call. A pair with an index outside the pool is left out."""
+    read and written in one call. A pair with an index outside the pool is left out. What is launched behind the call, on its stream or in
+    the same graph, finds the pages copied, decode attention too, which reads earlier keys ahead of the kernel before it."""
     _need(pool, None, "pool"); _need(src, torch.int32, "src"); _need(dst, torch.int32, "dst")
     if pool.dim() < 2 or src.dim() != 1 or src.shape != dst.shape:
         raise ValueError("copy_pages: pool [planes, pages, ...], src and dst one index per copy")
@@ -1431,7 +1432,8 @@ def compact_tokens(pool: torch.Tensor, block_table: torch.Tensor, first: torch.T
     pool [planes, pages, heads, page_tokens, channels] of any type, in place: sequence s holds first[s] tokens and keeps its drafts
     picked[cu_picked[s]] < picked[cu_picked[s] + 1] < ...; the row at place first[s] + picked[cu_picked[s] + i] goes to place first[s] + i. All
     indices int32 on the device, block_table [S, W] the sequences' pages. Sequences do not share the pages these places are in. A draft that
-    lies outside its sequence's table, or whose page is outside the pool, is left out."""
+    lies outside its sequence's table, or whose page is outside the pool, is left out. What is launched behind the call, on its stream or in
+    the same graph, finds the rows moved, decode attention too, which reads earlier keys ahead of the kernel before it."""
     _need(pool, None, "pool")
     for name, t in (("block_table", block_table), ("first", first), ("picked", picked), ("cu_picked", cu_picked)):
         _need(t, torch.int32, name)

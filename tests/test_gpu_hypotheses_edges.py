@@ -1,0 +1,70 @@
+"""Operators and searches over several hypotheses of a request, at calls that their documentation allows and that are easily got wrong:
+sinks of -inf, drafts and held tokens that are not finite, very many rows and requests, moves right ahead of decode attention, small pools."""
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_hypotheses import INF, NAN, Trees, feed, fresh, ops
+
+pytestmark = pytest.mark.gpu
+BOTH = [torch.bfloat16, torch.float32]
+
+
+def attend(o, pool, table, ctx, q, out, splits):
+    n = ctx.numel()
+    o.attention_decode_bf16(q, pool[-2], pool[-1], out, table, torch.arange(n + 1, dtype=torch.int32, device="cuda"), ctx, None, n, 32, 8, 128, 16,
+                            128 ** -0.5, splits=splits)
+
+
+@pytest.mark.parametrize("splits", [1, 4])
+@pytest.mark.parametrize("move", ["copy", "compact"])
+def test_decode_attention_right_behind_a_move_sees_the_moved_rows(move, splits):
+    """One graph of a move in all planes of a large pool and the attention over the last two of them, which reads earlier keys ahead of
+    its wait: the bits of a call that was waited for, and the formula's."""
+    o, gen = ops(), torch.Generator(device="cuda").manual_seed(splits)
+    put = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    seqs, width, planes = 8, 100, 12
+    pages = 2 * seqs * width
+    fresh_pool = torch.randn(planes, pages, 8, 16, 128, generator=gen, device="cuda", dtype=torch.bfloat16)
+    pool = fresh_pool.clone()
+    q, outs = torch.randn(seqs, 32 * 128, generator=gen, device="cuda").to(torch.bfloat16), [torch.empty(seqs, 32 * 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    table = torch.arange(seqs * width, dtype=torch.int32, device="cuda").view(seqs, width)
+    if move == "copy":
+        src, dst = torch.arange(seqs * width, pages, dtype=torch.int32, device="cuda"), table.flatten()
+        ctx = put([width * 16 - i for i in range(seqs)])
+        moved = lambda: o.copy_pages(pool, src, dst)
+    else:                                                  # 700 of 1,500 drafts behind ten tokens
+        picks = [sorted(torch.randperm(1500, generator=torch.Generator().manual_seed(s))[:700].tolist()) for s in range(seqs)]
+        first, picked, cu = put([10] * seqs), put([p for row in picks for p in row]), put([700 * s for s in range(seqs + 1)])
+        ctx = put([710] * seqs)
+        moved = lambda: o.compact_tokens(pool, table, first, picked, cu)
+    moved(); attend(o, pool, table, ctx, q, outs[0], splits)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        moved(); attend(o, pool, table, ctx, q, outs[0], splits)
+    for _ in range(5):
+        pool.copy_(fresh_pool); outs[0].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        attend(o, pool, table, ctx, q, outs[1], splits)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1])
+    # the formula, from the rows as they were before the move
+    for s in (0, seqs - 1):
+        n = int(ctx[s])
+        rows = fresh_pool[-2:, src.view(seqs, width)[s].long()] if move == "copy" else fresh_pool[-2:, table[s].long()]
+        rows = rows.transpose(2, 3).reshape(2, -1, 8, 128).double()
+        keep = torch.arange(n, device="cuda") if move == "copy" else torch.tensor(list(range(10)) + [10 + p for p in picks[s]], device="cuda")
+        k, v = rows[0][keep], rows[1][keep]
+        heads = q[s].double().view(8, 4, 128)
+        z = torch.einsum("hgd,khd->hgk", heads, k) * 128 ** -0.5
+        p = torch.softmax(z, 2)
+        want, sums = (torch.einsum("hgk,khd->hgd", p, x).flatten() for x in (v, v.abs()))
+        # weights and result round to bfloat16; scores, exponentials and sums in 32 bits
+        size = float((torch.einsum("hgd,khd->hgk", heads.abs(), k.abs()) * 128 ** -0.5).max())
+        bound = (2 * (132 * 2.0 ** -24 * size + 2.0 ** -18) + 2 * (n + 64) * 2.0 ** -24) * sums
+        bound = bound + 2.0 ** -8 * sums + 2.0 ** -8 * (want.abs() + bound)
+        assert ((outs[0][s].double() - want).abs() <= bound).all()

@@ -321,10 +321,10 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
       const int head = u.head * group + row % group;
       float total = l_run[r];
       float factor = 1.f;
-      if (a.sinks) {                                       // the sink may be the largest of all
-        const float sink = a.sinks[head] * LOG2E, m = m_run[r] * a.scale_log2, top = fmaxf(m, sink);
-        factor = fast_exp2(m - top);
-        total = total * factor + fast_exp2(sink - top);
+      if (a.sinks) {                                       // the sink may be the largest of all, or -inf where nothing is seen either
+        const float sink = a.sinks[head] * LOG2E, m = m_run[r] * a.scale_log2, top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
+        factor = fast_exp2(m - base);
+        total = total * factor + fast_exp2(sink - base);
       }
       const float inv = total == 0.f ? 0.f : factor / total;
       bf16* to = (bf16*)a.out + ((size_t)(u.first + row / group) * a.q_heads + head) * a.dim;
@@ -521,9 +521,9 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f3
       const int head = u.head * group + row % group;
       float total = l_run[i], factor = 1.f;
       if (a.sinks) {
-        const float sink = a.sinks[head] * LOG2E, m = m_run[i] * a.scale_log2, top = fmaxf(m, sink);
-        factor = exp2f(m - top);
-        total = total * factor + exp2f(sink - top);
+        const float sink = a.sinks[head] * LOG2E, m = m_run[i] * a.scale_log2, top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
+        factor = exp2f(m - base);
+        total = total * factor + exp2f(sink - base);
       }
       const float inv = total == 0.f ? 0.f : factor / total;
       float* to = (float*)a.out + ((size_t)(u.first + row / group) * a.q_heads + head) * a.dim;

@@ -617,9 +617,9 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
         if (!split) {
           float total = l_sum, factor = 1.f;
           if (a.sinks && valid) {
-            const float sink = a.sinks[row_head] * LOG2E, top = fmaxf(m_log2, sink);
-            factor = fast_exp2(m_log2 - top);
-            total = total * factor + fast_exp2(sink - top);
+            const float sink = a.sinks[row_head] * LOG2E, top = fmaxf(m_log2, sink), base = top == -INFINITY ? 0.f : top;
+            factor = fast_exp2(m_log2 - base);
+            total = total * factor + fast_exp2(sink - base);
           }
           inv = total == 0.f ? 0.f : __fdividef(factor, total);
         }

@@ -68,3 +68,18 @@ def test_decode_attention_right_behind_a_move_sees_the_moved_rows(move, splits):
         bound = (2 * (132 * 2.0 ** -24 * size + 2.0 ** -18) + 2 * (n + 64) * 2.0 ** -24) * sums
         bound = bound + 2.0 ** -8 * sums + 2.0 ** -8 * (want.abs() + bound)
         assert ((outs[0][s].double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("held, window", [(0, 0), (100, 1), (3000, 2000)])
+def test_a_row_that_sees_nothing_is_zero_also_where_its_sink_is_minus_infinity(held, window, dim, dtype):
+    """One part of the keys and several; a row that sees one key has its value, as without a sink."""
+    empty = torch.zeros(10, 10, dtype=torch.bool)
+    empty[3, 3] = True
+    case = Trees([(held, 10)], 4, 2, dim, dtype=dtype, sinks=True, window=window, seen=[empty], seed=dim).fill()
+    case.sinks[1:3] = -INF
+    case.positions[:10] = held + 5000                      # behind the window nothing held is seen
+    got = case.run()[:10].view(10, 4, dim)
+    assert (got[[0, 1, 2, 4, 5, 6, 7, 8, 9]] == 0).all()
+    assert torch.equal(got[3, 1], case.v[0][held + 3, 0]) and torch.equal(got[3, 2], case.v[0][held + 3, 1])

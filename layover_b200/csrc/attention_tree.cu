@@ -649,8 +649,8 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
 }
 
 // The tcgen05 kernel: bfloat16, heads of 128 channels, at most 128 query heads a key/value head, pages of 8 .. 128 tokens that divide 128. `blocks` blocks
-// share the keys; `rows2`: tiles of twice 128 / group drafts. `scratch` holds lb_attention_tree_scratch(blocks, rows2) floats.
-LB_EXPORT long lb_attention_tree_scratch(int blocks, int rows2) { return wide::scratch_floats(blocks, rows2 != 0); }
+// share the keys; `rows2`: tiles of twice 128 / group drafts. `scratch` holds lb_attention_tree_scratch(blocks, rows2, tokens * q_heads) floats.
+LB_EXPORT long lb_attention_tree_scratch(int blocks, int rows2, long rows) { return wide::scratch_floats(blocks, rows2 != 0, rows); }
 LB_EXPORT int lb_attention_tree_tcgen05(const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
                                         int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words,
                                         int tokens, int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, float scale, int window,
@@ -661,7 +661,7 @@ LB_EXPORT int lb_attention_tree_tcgen05(const void* q, const void* k_pool, const
                                  window, softcap, max_nodes);
   if (refused) return refused;
   if (dim != 128 || q_heads / kv_heads > 128 || page_tokens % 8 || 128 % page_tokens || blocks <= 0 || blocks > 1024 || !scratch ||
-      floats < wide::scratch_floats(blocks, rows2 != 0))
+      floats < wide::scratch_floats(blocks, rows2 != 0, (long)tokens * q_heads))
     return LB_ERR_SIZE;
   if (((uintptr_t)scratch | (uintptr_t)out) & 31) return LB_ERR_ALIGN;
   TreeArgs a{q, k_pool, v_pool, out, block_table, table_width, n_pages, cu_q, ctx_len, positions, tree, tree_words, tokens, q_heads, kv_heads, dim,

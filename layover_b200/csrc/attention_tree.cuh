@@ -28,7 +28,7 @@ struct TreeArgs {
   int n_seqs, max_nodes;
   int group, tile_drafts;       // query heads of a key/value head; drafts of a tile of 128 rows (the tcgen05 kernel's)
   Border* borders;       // the tcgen05 kernel's, for the kernel that joins: per block
-  int* not_finite;              // whether a block met an output that is not finite
+  float2* row_stats;            // its [tokens][q_heads], of its careful pass: a row's maximum, and the sum of its weights and the sink's relative to it
 };
 
 // What a block works on: its rows, and its share of the keys.

@@ -24,17 +24,22 @@
 // time), and the join. The same by mma.sync, the rows' keys in chunks: 843, 202 and 167 us.
 //
 // Rows that the tree does not have cost nothing but the tensor cores' time: their warps only hand tiles on. A draft's values may hold what
-// is not finite, and 0 x NaN is NaN also for rows that do not see the draft: a block whose outputs are not all finite says so, and `join_kernel`
-// makes its rows once more, key by key.
+// is not finite, and 0 x NaN is NaN also for rows that do not see the draft. A block whose outputs are not all finite therefore takes its share once
+// more, carefully: in tiles of which a row may not see every key, zeros stand for values that are not finite, and who sees those gets their
+// terms added afterwards. So who does not see them has the bits that he would have beside finite ones, and a call without them pays nothing: to look at
+// the drafts' values in every call costs 4 of 38 us and 14 to 26 of 156 (8 x 32 and 40 requests), whichever warp does it, for what runs seldom waits for its
+// instructions. With one draft of NaN a call that is waited for takes 122 us instead of 62 (8 x 32) and 537 instead of 194 (40 requests).
 #pragma once
 #include <math.h>
+
+#include <type_traits>
 
 #include "attention_tree.cuh"
 #include "tcgen05.cuh"
 
 namespace {
 
-__device__ int g_tree_error = 0;       // 0 = ok; which wait ran out otherwise: 1 ring, 2 queries, 3 keys, 4 values, 5 weights, 6 scores, 7 and 8 second product
+__device__ int g_tree_error = 0;       // 0 = ok; which wait ran out otherwise: 1 ring, 2 queries, 3 keys, 4 values, 5 weights, 6 scores, 7 and 8 second product, 9 values that are looked at
 
 namespace wide {
 
@@ -43,11 +48,18 @@ constexpr int HALF_BYTES = 128 * 128;           // 64 channels of 128 rows
 constexpr int TILE_BYTES = 2 * HALF_BYTES;
 constexpr int STAGES = 2;                       // tiles of either ring
 constexpr int LOADERS = 4;                      // warps that load: two K, two V, each 64 rows of a tile
-constexpr int FIRST_SOFTMAX = 8;                // then one that issues the products (and three that do nothing), then two warpgroups of softmax
+constexpr int FIRST_SOFTMAX = 8;                // then one that issues the products, one for the borders and two of the careful pass, then two warpgroups of softmax
 constexpr int THREADS = 32 * (FIRST_SOFTMAX + 8);
 constexpr int FEW_REGS = 72, MANY_REGS = 184;   // of a thread of the first eight warps and of the others: 256 * (72 + 184) = 512 * 128, the launch's
 constexpr int SEQ_CACHE = 512;                  // sequences whose lengths are kept there
-constexpr int SMEM_BYTES = (2 + 2 * STAGES) * TILE_BYTES + 1024 + 512 + 2 * 2 * ROWS * 8 + SEQ_CACHE * 16;
+// A pass's barriers: K's, then V's stages are full and empty; a segment's queries have come (two segments, or ROWS2: the first alone) and its last
+// scores are made; a turn's scores are in tensor memory (two warpgroups), its weights are, and the output is rescaled, its second product is
+// finished; a segment's products are finished, its outputs have been read, its maxima and sums are in shared memory; `start` and `known`
+// are; in the careful pass, values that are still to be looked at have come (two halves of a tile, STAGES).
+constexpr int FULL = 0, EMPTY = FULL + 2 * STAGES, Q_FULL = EMPTY + 2 * STAGES, Q_EMPTY = Q_FULL + 2, S_FULL = Q_EMPTY + 2, P_FULL = S_FULL + 2,
+              PV_DONE = P_FULL + 2, O_FULL = PV_DONE + 2, O_EMPTY = O_FULL + 1, STATS_FULL = O_EMPTY + 1, STARTED = STATS_FULL + 1, LANDED = STARTED + 1,
+              BARRIERS = LANDED + 2 * STAGES;
+constexpr int SMEM_BYTES = (2 + 2 * STAGES) * TILE_BYTES + 1024 + (2 * BARRIERS + 8) * 8 + 2 * 2 * ROWS * 8 + SEQ_CACHE * 16;
 constexpr float GROWTH = 8.0f;                  // the maximum that weights are relative to may lag by this, in log2 units
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -67,6 +79,31 @@ __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
       "{\n\t.reg .pred e;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
       "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared(uint32_t p) {
+  uint4 w;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(p) : "memory");
+  return w;
+}
+__device__ __forceinline__ void clear_shared(uint32_t p) { asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(p), "r"(0) : "memory"); }
+// Rows [lo, hi) of a tile of values that are not finite become zeros, by a warp, half of it a row (all its pieces: their order does not matter).
+__device__ __forceinline__ void clear_odd_rows(uint32_t tile, int lo, int hi) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t at = tile + ((lane & 15) >> 3) * HALF_BYTES + (lane & 7) * 16;
+#pragma unroll 1
+  for (int r0 = lo; r0 < hi; r0 += 2) {
+    const int r = r0 + (lane >> 4);
+    const uint4 w = r < hi ? load_shared(at + r * 128) : make_uint4(0, 0, 0, 0);
+    const unsigned odd = __ballot_sync(0xffffffffu, not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w));
+    if (odd >> (lane & 16) & 0xFFFFu) clear_shared(at + r * 128);
+  }
+}
+template <int ID, int N> __device__ __forceinline__ void meet() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+template <int ID, int N> __device__ __forceinline__ bool meet_any(bool mine) {      // whether any of them says so
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"((uint32_t)mine), "n"(ID), "n"(N) : "memory");
+  return any != 0;
 }
 // 16 bytes to shared memory; zeros where `bytes` is 0; an arrival on the barrier when all copies of this thread before it have landed
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -198,6 +235,82 @@ struct Walk {
   }
 };
 
+__device__ __forceinline__ float4 four_values(const void* rows, long row) {      // of 128 a row, a lane's
+  const uint2 w = *reinterpret_cast<const uint2*>((const bf16*)rows + row * DIM + 4 * (threadIdx.x & 31));
+  const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x)), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
+  return make_float4(x.x, x.y, y.x, y.y);
+}
+// Behind a careful pass, by the softmax warps: the values for which zeros stood are found once more, and who sees them gets their terms added,
+// to what the segment's rows left in scratch memory or, where a row tile lies wholly in the block's share, to the output (whose finite channels so
+// round twice). `bits`: four words a key tile, of MOST_LOOKS tiles at a time. Rows whose weights are not finite are NaN already.
+constexpr int MOST_LOOKS = 4 * ROWS * 8 / 16;
+template <bool ROWS2>
+__device__ __forceinline__ void add_odd_values(const TreeArgs& a, const int4* known, const int* start, unsigned* bits, int warp) {
+  constexpr int WARPS = 8;
+  const int lane = threadIdx.x & 31, tile_drafts = a.tile_drafts * (ROWS2 ? 2 : 1);
+  Walk<ROWS2> walk;
+  walk.begin_at(a, known, start[0], start[1], start[2]);
+  while (walk.next(a)) {
+    const Sequence& s = walk.s;
+    const int* table = a.block_table + (size_t)walk.seq * a.table_width;
+    const int first_key = (s.tile_lo + walk.begin) * KEYS, draft0 = walk.row_tile * tile_drafts;
+    const int rows = max(0, min(tile_drafts, min(s.n, a.max_nodes) - draft0)) * a.group;
+    const bool split = walk.count < s.tiles;
+    for (int begin = a.window > 0 ? 0 : max(0, s.held - first_key) / KEYS; begin < walk.count; begin += MOST_LOOKS) {
+      const int tiles = min(MOST_LOOKS, walk.count - begin), base = first_key + begin * KEYS;
+      meet<2, 32 * WARPS>();
+      for (int i = threadIdx.x & (32 * WARPS - 1); i < 4 * tiles; i += 32 * WARPS) bits[i] = 0;
+      meet<2, 32 * WARPS>();
+#pragma unroll 4
+      for (int j = (a.window > 0 ? max(0, s.key_lo - base) : max(0, s.held - base)) + warp; j < min(tiles * KEYS, s.ctx - base); j += WARPS) {
+        const long at = key_row(a, table, base + j, walk.head);
+        const uint2 v = at < 0 ? make_uint2(0, 0) : *reinterpret_cast<const uint2*>((const bf16*)a.v_pool + at * DIM + 4 * lane);
+        if (__any_sync(0xffffffffu, not_finite(v.x) || not_finite(v.y)) && lane == 0) atomicOr(&bits[j >> 5], 1u << (j & 31));
+      }
+      meet<2, 32 * WARPS>();
+      unsigned some = 0;
+      for (int w = 0; w < 4 * tiles; ++w) some |= bits[w];
+      if (!some) continue;
+#pragma unroll 1
+      for (int r = warp; r < rows; r += WARPS) {
+        const int draft = r / a.group, member = r - draft * a.group, token = s.first + draft0 + draft, row_head = walk.head * a.group + member;
+        const long row = (long)token * a.q_heads + row_head;
+        const int local = ROWS2 && draft >= a.tile_drafts ? ROWS + (draft - a.tile_drafts) * a.group + member : r;
+        const long place = ((long)2 * blockIdx.x + (walk.begin == 0 ? 1 : 0)) * (ROWS2 ? 2 * ROWS : ROWS) + local;
+        const float2 of = split ? reinterpret_cast<const float2*>(a.partials + a.partial_stats)[place] : a.row_stats[row];
+        if (!(of.y > 0.f)) continue;                       // it sees nothing here, or its weights are NaN
+        const int oldest = a.window > 0 ? max(a.positions[token], s.held) - a.window + 1 : 0;
+        const int* seen = a.tree + (size_t)token * a.tree_words;
+        const float4 q = four_values(a.q, row);
+        float4 more = make_float4(0.f, 0.f, 0.f, 0.f);
+        bool any = false;
+#pragma unroll 1
+        for (int w = 0; w < 4 * tiles; ++w) {
+          if (!bits[w]) continue;
+          for (unsigned odd = bits[w] & seen_word(a.tree_words, seen, base + 32 * w, s.held, s.ctx, oldest); odd; odd &= odd - 1) {
+            const long at = key_row(a, table, base + 32 * w + __ffs(odd) - 1, walk.head);       // it is there: its values were read
+            const float4 k = four_values(a.k_pool, at), v = four_values(a.v_pool, at);
+            float z = warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w);
+            if (a.cap_in != 0.f) z = a.cap_out - __fdividef(2.f * a.cap_out, 1.f + fast_exp2(z * a.cap_in));
+            const float weight = exp2f(z * a.scale_log2 - of.x) / (split ? 1.f : of.y);
+            if (weight != 0.f) { more.x += weight * v.x; more.y += weight * v.y; more.z += weight * v.z; more.w += weight * v.w; }
+            any = true;
+          }
+        }
+        if (!any) continue;
+        if (split) {
+          float4* to = reinterpret_cast<float4*>(a.partials + place * DIM + 4 * lane);
+          const float4 x = *to;
+          *to = make_float4(x.x + more.x, x.y + more.y, x.z + more.z, x.w + more.w);
+        } else {
+          const float4 x = four_values(a.out, row);
+          *reinterpret_cast<uint2*>((bf16*)a.out + row * DIM + 4 * lane) = make_uint2(pack_bf16(x.x + more.x, x.y + more.y), pack_bf16(x.z + more.z, x.w + more.w));
+        }
+      }
+    }
+  }
+}
+
 template <bool ROWS2>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ TreeArgs a) {
@@ -205,34 +318,29 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
   uint8_t* q_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);      // two tiles: of two segments, or of two halves
   uint8_t* ring = q_s + 2 * TILE_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + 2 * STAGES * TILE_BYTES);
-  uint64_t* full = bars;              // [K, V][STAGES]
-  uint64_t* empty = full + 2 * STAGES;    // [K, V][STAGES]
-  uint64_t* q_full = empty + 2 * STAGES;  // [2] a segment's queries have come (ROWS2: [0] alone)
-  uint64_t* q_empty = q_full + 2;     // [2] its last scores are made
-  uint64_t* s_full = q_empty + 2;     // [2 warpgroups] the scores of a turn are in tensor memory
-  uint64_t* p_full = s_full + 2;      // [2] its weights are, and the output is rescaled
-  uint64_t* pv_done = p_full + 2;     // [2] its second product is finished
-  uint64_t* o_full = pv_done + 2;     // a segment's products are finished
-  uint64_t* o_empty = o_full + 1;     // its outputs have been read
-  uint64_t* stats_full = o_empty + 1; // its maxima and sums are in shared memory
-  uint64_t* started = stats_full + 1; // `start` and `known` are
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(started + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * BARRIERS);
   volatile uint32_t* flag = tmem_slot + 1;        // [0] a wait ran out, [1] an output is not finite
   int* start = const_cast<int*>(reinterpret_cast<volatile int*>(flag + 2));      // where the walk begins: sequence, tile of it, tiles
-  float2* stats = reinterpret_cast<float2*>(bars + 64);      // [2 segments][2 warpgroups][ROWS]
+  float2* stats = reinterpret_cast<float2*>(bars + 2 * BARRIERS + 8);      // [2 segments][2 warpgroups][ROWS]
   int4* known = reinterpret_cast<int4*>(stats + 4 * ROWS);                  // first draft, end, keys and tiles of the first sequences
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  if (threadIdx.x == 32 * LOADERS) {
-    for (int i = 0; i < 2 * STAGES; ++i) { mbar_init(&full[i], 32 * LOADERS / 2); mbar_init(&empty[i], 1); }
+  auto make_barriers = [&]() {
+    for (int i = 0; i < 2 * STAGES; ++i) { mbar_init(&bars[FULL + i], 32 * LOADERS / 2); mbar_init(&bars[EMPTY + i], 1); }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
+      mbar_init(&bars[Q_FULL + i], 1); mbar_init(&bars[Q_EMPTY + i], 1); mbar_init(&bars[S_FULL + i], 1); mbar_init(&bars[P_FULL + i], 4); mbar_init(&bars[PV_DONE + i], 1);
     }
-    mbar_init(o_full, 1); mbar_init(o_empty, 8); mbar_init(stats_full, 8); mbar_init(started, 1);
-    flag[0] = 0; flag[1] = 0;
-    prefetch_map(&q_map);
+    mbar_init(&bars[O_FULL], 1); mbar_init(&bars[O_EMPTY], 8); mbar_init(&bars[STATS_FULL], 8); mbar_init(&bars[STARTED], 1);
+  };
+  auto publish_barriers = [&]() {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
+  };
+  if (threadIdx.x == 32 * LOADERS) {
+    make_barriers();
+    flag[0] = 0; flag[1] = 0;
+    prefetch_map(&q_map);
+    publish_barriers();
   }
   __syncwarp();
   if (warp == LOADERS) tmem_alloc(tmem_slot, 512);
@@ -244,9 +352,24 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
   auto ran_out = [&](int code) { atomicCAS(&g_tree_error, 0, code); flag[0] = 1; return false; };
   bool ok = true;
   pdl_launch_dependents();
+  // The end of the first pass, for all warps: whether there is a careful one, whose barriers they then turn to. (Each pass has code of its own: as one
+  // loop the registers do not suffice.)
+  auto careful_pass = [&]() {
+    fence_before_sync();
+    meet<1, THREADS>();
+    fence_after_sync();
+    if (flag[0] || !flag[1]) return false;
+    bars += BARRIERS;
+    if (threadIdx.x == 32 * LOADERS) {
+      make_barriers();
+      for (int i = 0; i < 2 * STAGES; ++i) mbar_init(&bars[LANDED + i], 32);
+      publish_barriers();
+    }
+    meet<1, THREADS>();
+    return true;
+  };
 
-  if (warp < FIRST_SOFTMAX) {
-    give_registers<FEW_REGS>();
+  auto load_and_issue = [&](auto careful) {
     if (warp < LOADERS) {
       pdl_wait();
       if (warp == 0) {
@@ -300,9 +423,9 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
         }
         if (lane == 0) start[3] = total;
         __syncwarp();
-        if (lane == 0) mbar_arrive(started);
+        if (lane == 0) mbar_arrive(&bars[STARTED]);
       } else {
-        ok = warp_wait(started, 0) || ran_out(1);
+        ok = warp_wait(&bars[STARTED], 0) || ran_out(1);
       }
       // ---------------- K or V, and the first of these warps the queries
       const int n_tiles = ok ? start[2] : 0, values = warp >> 1, row0 = (warp & 1) * 64, page_shift = __ffs(a.page_tokens) - 1;
@@ -315,7 +438,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
       const long lane_from = (lane >> 4) * DIM + (lane & 15) * 8;
       // Up to four tiles of a segment, whose pages are looked up together, four tiles ahead (a read from memory waits behind all copies
       // in flight): lane 8 j + i has the page of rows 8 i .. of tile j.
-      struct Group { int page, key0, count, head, key_lo, ctx, draft; } now, soon;
+      struct Group { int page, key0, count, head, key_lo, ctx, draft, looked_at; } now, soon;
       Walk<ROWS2> ahead;
       ahead.begin_at(a, known, start[0], start[1], n_tiles);
       int tile = 0, segments = 0, taken = 0;
@@ -328,6 +451,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
         }
         g.count = min(4, ahead.count - tile); g.head = ahead.head; g.key0 = (ahead.s.tile_lo + ahead.begin + tile) * KEYS;
         g.key_lo = ahead.s.key_lo; g.ctx = ahead.s.ctx;
+        g.looked_at = !careful || values == 0 ? 0x7fffffff : a.window > 0 ? 0 : ahead.s.held - KEYS + 1;      // tiles from here on
         const int key = g.key0 + (lane >> 3) * KEYS + row0 + (lane & 7) * 8, index = key >> page_shift;
         g.page = index < a.table_width && key < g.ctx ? a.block_table[(size_t)ahead.seq * a.table_width + index] : -1;
         tile += g.count;
@@ -337,9 +461,9 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
         next_group(soon);
         if (warp == 0 && now.draft >= 0) {
           const int buf = ROWS2 ? 0 : segments & 1;
-          ok = warp_wait(&q_empty[buf], ((ROWS2 ? segments : segments >> 1) & 1) ^ 1) || ran_out(2);
+          ok = warp_wait(&bars[Q_EMPTY + buf], ((ROWS2 ? segments : segments >> 1) & 1) ^ 1) || ran_out(2);
           if (!ok) break;
-          const uint32_t bar = smem_u32(&q_full[buf]);
+          const uint32_t bar = smem_u32(&bars[Q_FULL + buf]);
           expect_bytes(bar, (uint32_t)(drafts_tile * group * 128) * (ROWS2 ? 4 : 2));
           const int head = warp_uniform(now.head * group), draft = warp_uniform(now.draft);
           for (int part = 0; part < (ROWS2 ? 2 : 1); ++part)
@@ -353,7 +477,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
         const unsigned there = __ballot_sync(0xffffffffu, first >= 0);
         for (int j = 0; j < now.count; ++j) {
           const int stage = taken % STAGES, key0 = now.key0 + j * KEYS;
-          ok = warp_wait(&empty[values * STAGES + stage], ((taken / STAGES) & 1) ^ 1) || ran_out(1);
+          ok = warp_wait(&bars[EMPTY + values * STAGES + stage], ((taken / STAGES) & 1) ^ 1) || ran_out(1);
           if (!ok || flag[0]) { ok = false; break; }
           const uint32_t at = ring_at + stage * TILE_BYTES;
           if ((there >> (8 * j) & 0xFFu) == 0xFFu && key0 >= now.key_lo && key0 + KEYS <= now.ctx) {
@@ -376,7 +500,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
               }
             }
           }
-          arrive_when_copied(smem_u32(&full[values * STAGES + stage]));
+          arrive_when_copied(smem_u32(key0 < now.looked_at ? &bars[FULL + values * STAGES + stage] : &bars[LANDED + (warp & 1) * STAGES + stage]));
           ++taken;
         }
         now = soon;
@@ -385,7 +509,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
     } else if (warp == LOADERS) {
       // ---------------- the products, turn by turn; the scores are two turns ahead
       pdl_wait();
-      ok = warp_wait(started, 0) || ran_out(2);
+      ok = warp_wait(&bars[STARTED], 0) || ran_out(2);
       const int n_tiles = ok ? start[2] : 0;
       Walk<ROWS2> ahead, walk;
       ahead.begin_at(a, known, start[0], start[1], n_tiles);
@@ -403,36 +527,36 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
             g_left = warp_uniform(ROWS2 ? 2 * walk.count : walk.count);
             g_turn = 0;
             ++g_segment;
-            if (g_segment > 0) ok = warp_wait(o_empty, (g_segment - 1) & 1) || ran_out(8);
+            if (g_segment > 0) ok = warp_wait(&bars[O_EMPTY], (g_segment - 1) & 1) || ran_out(8);
           }
           if (ok && (!ROWS2 || w == 0)) {
             v_stage = STAGES + v_taken % STAGES;
-            ok = warp_wait(&full[v_stage], (v_taken / STAGES) & 1) || ran_out(4);
+            ok = warp_wait(&bars[FULL + v_stage], (v_taken / STAGES) & 1) || ran_out(4);
             ++v_taken;
             fence_async_smem();                              // what cp.async wrote is read by the tensor cores
           }
-          ok = ok && (warp_wait(&p_full[w], (t >> 1) & 1) || ran_out(5));
+          ok = ok && (warp_wait(&bars[P_FULL + w], (t >> 1) & 1) || ran_out(5));
           if (!ok) break;
           fence_after_sync();
           const uint32_t v_addr = smem_u32(ring + v_stage * TILE_BYTES);
 #pragma unroll
           for (int ks = 0; ks < KEYS / 16; ++ks)            // 16 keys: 8 columns of weights, 16 rows of V
             umma_from_tmem(tmem_o + w * 128, tmem_s + w * 128 + ks * 8, desc_mn_major(v_addr + ks * 16 * 128), IDESC_O, (g_turn > 1 || ks > 0) ? 1u : 0u);
-          umma_commit(&pv_done[w]);
-          if (!ROWS2 || w == 1) umma_commit(&empty[v_stage]);
+          umma_commit(&bars[PV_DONE + w]);
+          if (!ROWS2 || w == 1) umma_commit(&bars[EMPTY + v_stage]);
           ++g_turn;
-          if (--g_left == 0) umma_commit(o_full);
+          if (--g_left == 0) umma_commit(&bars[O_FULL]);
         }
         if (t + 2 < turns) {
           if (a_left == 0) {
             ahead.next(a);
             a_left = warp_uniform(ROWS2 ? 2 * ahead.count : ahead.count);
             ++a_segment;
-            ok = warp_wait(&q_full[ROWS2 ? 0 : a_segment & 1], (ROWS2 ? a_segment : a_segment >> 1) & 1) || ran_out(2);
+            ok = warp_wait(&bars[Q_FULL + (ROWS2 ? 0 : a_segment & 1)], (ROWS2 ? a_segment : a_segment >> 1) & 1) || ran_out(2);
           }
           if (ok && (!ROWS2 || w == 0)) {
             k_stage = k_taken % STAGES;
-            ok = warp_wait(&full[k_stage], (k_taken / STAGES) & 1) || ran_out(3);
+            ok = warp_wait(&bars[FULL + k_stage], (k_taken / STAGES) & 1) || ran_out(3);
             ++k_taken;
             fence_async_smem();
           }
@@ -444,15 +568,38 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
             const uint32_t off = (ks >> 2) * HALF_BYTES + (ks & 3) * 32;
             umma_bf16(tmem_s + w * 128, desc_k_major(q_addr + off), desc_k_major(k_addr + off), IDESC_S, ks > 0 ? 1u : 0u);
           }
-          umma_commit(&s_full[w]);
-          if (!ROWS2 || w == 1) umma_commit(&empty[k_stage]);
-          if (--a_left == 0) umma_commit(&q_empty[ROWS2 ? 0 : a_segment & 1]);
+          umma_commit(&bars[S_FULL + w]);
+          if (!ROWS2 || w == 1) umma_commit(&bars[EMPTY + k_stage]);
+          if (--a_left == 0) umma_commit(&bars[Q_EMPTY + (ROWS2 ? 0 : a_segment & 1)]);
+        }
+      }
+    } else if (warp > LOADERS + 1) {
+      // ---------------- the careful pass: values that may not be seen by all rows, each warp what one of the loading warps copied
+      if (careful) {
+        const int part = warp - LOADERS - 2, row0 = part * 64;
+        ok = warp_wait(&bars[STARTED], 0) || ran_out(9);
+        Walk<ROWS2> walk;
+        walk.begin_at(a, known, start[0], start[1], ok ? start[2] : 0);
+        int taken = 0;
+        unsigned phases = 0;                                 // a bit a stage
+        while (ok && walk.next(a)) {
+          const int first_key = (walk.s.tile_lo + walk.begin) * KEYS;
+          for (int j = a.window > 0 ? 0 : max(0, walk.s.held - first_key) / KEYS; j < walk.count && ok; ++j) {
+            const int stage = (taken + j) % STAGES, key0 = first_key + j * KEYS;
+            ok = warp_wait(&bars[LANDED + part * STAGES + stage], phases >> stage & 1u) || ran_out(9);
+            phases ^= 1u << stage;
+            const int from = a.window > 0 ? row0 : max(row0, walk.s.held - key0);      // without a window every row sees what is held
+            clear_odd_rows(smem_u32(ring + (STAGES + stage) * TILE_BYTES), from, min(walk.s.ctx - key0, row0 + 64));
+            fence_async_smem();                              // zeros are read by the tensor cores
+            mbar_arrive(&bars[FULL + STAGES + stage]);              // for a lane of the loading warp
+          }
+          taken += walk.count;
         }
       }
     } else if (warp == LOADERS + 1) {
       // ---------------- for the kernel that joins: the row tile inside which this block's share begins, if it is the first that does
       pdl_wait();
-      ok = warp_wait(started, 0) || ran_out(2);
+      ok = warp_wait(&bars[STARTED], 0) || ran_out(2);
       Walk<ROWS2> walk;
       walk.begin_at(a, known, start[0], start[1], ok ? start[2] : 0);
       Border border = {};
@@ -468,8 +615,8 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
       }
       if (lane == 0) a.borders[blockIdx.x] = border;
     }
-  } else {
-    take_registers<MANY_REGS>();
+  };
+  auto softmax = [&](auto careful) {
     // ---------------- softmax: one row a thread
     const int wg = (warp - FIRST_SOFTMAX) >> 2, quarter = warp & 3, lane_row = quarter * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
@@ -481,11 +628,11 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
     g.begin_at(a, known, 0, 0, 0);
     g.begin = g.row_tile = g.head = g.seq = 0; g.s = Sequence{};
     int turn0 = 0, n_tiles = 0;                            // the segment's first turn; the block's tiles
-    for (int k = -1; ok; ++k) {
+    for (int k = careful ? 0 : -1; ok; ++k) {
       const bool dry = k < 0;
       if (k == 0) {
         pdl_wait();
-        ok = mbar_wait(started, 0) || ran_out(6);
+        ok = mbar_wait(&bars[STARTED], 0) || ran_out(6);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         n_tiles = start[2];
         g.begin_at(a, known, start[0], start[1], n_tiles);
@@ -521,7 +668,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
                                         : seen_word(tree_words, bits, key0 + 32 * i, held, ctx, oldest);
         }
         // a warp without rows waits as well: the turn before has been handed on by all four by then
-        ok = dry || mbar_wait(&s_full[wg], j & 1) || ran_out(6);
+        ok = dry || mbar_wait(&bars[S_FULL + wg], j & 1) || ran_out(6);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         fence_after_sync();
         if (live) {
@@ -562,7 +709,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
             l_sum = l_sum * factor + ((sums[0] + sums[1]) + (sums[2] + sums[3]));
           }
           if ((any_grow && t > t_first) || (dry && quarter == 2)) {
-            ok = dry || mbar_wait(&pv_done[wg], (j - 1) & 1) || ran_out(7);
+            ok = dry || mbar_wait(&bars[PV_DONE + wg], (j - 1) & 1) || ran_out(7);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             fence_after_sync();
 #pragma unroll 2
@@ -579,7 +726,7 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
         }
         fence_before_sync();
         __syncwarp();
-        if (lane == 0 && !dry) mbar_arrive(&p_full[wg]);
+        if (lane == 0 && !dry) mbar_arrive(&bars[P_FULL + wg]);
       }
       if (!ok) break;
       if (dry && quarter != 3) continue;
@@ -590,15 +737,15 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
       if (!dry) {
         pair[wg * ROWS + lane_row] = make_float2(m_ref, l_sum);
         __syncwarp();
-        if (lane == 0) mbar_arrive(stats_full);
-        ok = (mbar_wait(stats_full, k & 1) || ran_out(7)) && (mbar_wait(o_full, k & 1) || ran_out(8));
+        if (lane == 0) mbar_arrive(&bars[STATS_FULL]);
+        ok = (mbar_wait(&bars[STATS_FULL], k & 1) || ran_out(7)) && (mbar_wait(&bars[O_FULL], k & 1) || ran_out(8));
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       }
       fence_after_sync();
       auto release = [&]() {                               // the accumulators may be written again
         fence_before_sync();
         __syncwarp();
-        if (lane == 0 && !dry) mbar_arrive(o_empty);
+        if (lane == 0 && !dry) mbar_arrive(&bars[O_EMPTY]);
       };
       // relative to one maximum: this warpgroup's accumulator by `mine`, the other's by `other`
       float mine = 1.f, other = 0.f;
@@ -615,13 +762,15 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
       if (live) {
         float inv = 1.f;
         if (!split) {
-          float total = l_sum, factor = 1.f;
+          float total = l_sum, factor = 1.f, base = m_log2;
           if (a.sinks && valid) {
-            const float sink = a.sinks[row_head] * LOG2E, top = fmaxf(m_log2, sink), base = top == -INFINITY ? 0.f : top;
+            const float sink = a.sinks[row_head] * LOG2E, top = fmaxf(m_log2, sink);
+            base = top == -INFINITY ? 0.f : top;
             factor = fast_exp2(m_log2 - base);
             total = total * factor + fast_exp2(sink - base);
           }
           inv = total == 0.f ? 0.f : __fdividef(factor, total);
+          if (careful && valid && (ROWS2 || wg == 0)) a.row_stats[(size_t)token * a.q_heads + row_head] = make_float2(base, total);
         }
         // 64 channels at a time: all of its own rows, or, where the rows are both warpgroups', half; `first_acc`: the accumulator of the
         // segment's first turn. The accumulators are free as soon as they lie in registers.
@@ -679,12 +828,23 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
       }
       if (!dry) turn0 += turns;
     }
+  };
+  if (warp < FIRST_SOFTMAX) {
+    give_registers<FEW_REGS>();
+    load_and_issue(std::false_type{});
+    if (careful_pass()) load_and_issue(std::true_type{});
+  } else {
+    take_registers<MANY_REGS>();
+    softmax(std::false_type{});
+    if (careful_pass()) {
+      softmax(std::true_type{});
+      if (!meet_any<2, 256>(flag[0] != 0)) add_odd_values<ROWS2>(a, known, start, reinterpret_cast<unsigned*>(stats), warp - FIRST_SOFTMAX);
+    }
   }
 
   // ---------------- teardown
   fence_before_sync();
   __syncthreads();
-  if (threadIdx.x == 0) a.not_finite[blockIdx.x] = flag[1];
   if (flag[0]) {
     for (int i = 0; i < 2000; ++i) __nanosleep(1000);     // let copies in flight land
     __syncthreads();
@@ -695,72 +855,16 @@ attention_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap q_map, const _
   }
 }
 
-// A row of the output by a warp, key by key: what the products cannot give where values are not finite. Seldom.
-__device__ __noinline__ void row_key_by_key(const TreeArgs& a, const Sequence& s, int seq, int head, int token, int row_head) {
-  const int lane = threadIdx.x & 31, oldest = a.window > 0 ? max(a.positions[token], s.held) - a.window + 1 : 0;
-  const int* table = a.block_table + (size_t)seq * a.table_width;
-  const int* bits = a.tree + (size_t)token * a.tree_words;
-  auto four = [&](const void* pool, long row) {
-    const uint2 w = *reinterpret_cast<const uint2*>((const bf16*)pool + row * DIM + 4 * lane);
-    const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x)), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
-    return make_float4(x.x, x.y, y.x, y.y);
-  };
-  const float4 q = four(a.q, (long)token * a.q_heads + row_head);
-  float top = a.sinks ? a.sinks[row_head] * LOG2E : -INFINITY, total = a.sinks ? 1.f : 0.f;      // in log2 units
-  float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int key = s.key_lo; key < s.ctx; ++key) {
-    if (!sees(a, bits, key, s.held, oldest)) continue;
-    const long at = key_row(a, table, key, head);
-    const float4 k = at < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : four(a.k_pool, at), v = at < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : four(a.v_pool, at);
-    float z = warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w);
-    if (a.cap_in != 0.f) z = a.cap_out - __fdividef(2.f * a.cap_out, 1.f + fast_exp2(z * a.cap_in));
-    z *= a.scale_log2;
-    const float m = fmaxf(top, z), base = m == -INFINITY ? 0.f : m, keep = exp2f(top - base), w = exp2f(z - base);
-    total = total * keep + w;
-    if (keep != 1.f) { out.x *= keep; out.y *= keep; out.z *= keep; out.w *= keep; }
-    if (w != 0.f) { out.x += w * v.x; out.y += w * v.y; out.z += w * v.z; out.w += w * v.w; }
-    top = m;
-  }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  *reinterpret_cast<uint2*>((bf16*)a.out + ((size_t)token * a.q_heads + row_head) * DIM + 4 * lane) =
-      make_uint2(pack_bf16(out.x * inv, out.y * inv), pack_bf16(out.z * inv, out.w * inv));
-}
-// The rows of all row tiles that lie wholly in block b's share, one warp of the column of blocks after the other.
-template <bool ROWS2>
-__device__ __noinline__ void share_key_by_key(const TreeArgs& a, int b, int blocks, int warp, int warps) {
-  int total = 0;
-  for (int seq = 0; seq < a.n_seqs; ++seq) {
-    const Sequence s = find_sequence<ROWS2>(a, a.cu_q[seq], a.cu_q[seq + 1], a.ctx_len[seq]);
-    total += a.kv_heads * s.row_tiles * s.tiles;
-  }
-  const int shares = min(blocks, total);
-  if (b >= shares) return;
-  const int from = share_begin(total, b, shares), upto = share_begin(total, b + 1, shares);
-  int at = 0;                                              // where the row tile begins in the list
-  for (int seq = 0; seq < a.n_seqs; ++seq) {
-    const Sequence s = find_sequence<ROWS2>(a, a.cu_q[seq], a.cu_q[seq + 1], a.ctx_len[seq]);
-    for (int unit = 0; unit < a.kv_heads * s.row_tiles; ++unit, at += s.tiles) {
-      if (at < from || at + s.tiles > upto) continue;
-      const int head = unit / s.row_tiles, draft0 = (unit - head * s.row_tiles) * (ROWS2 ? 2 : 1) * a.tile_drafts;
-      const int rows = min(min(s.n, a.max_nodes) - draft0, (ROWS2 ? 2 : 1) * a.tile_drafts) * a.group;
-      for (int row = warp; row < rows; row += warps)
-        row_key_by_key(a, s, seq, head, s.first + draft0 + row / a.group, head * a.group + row % a.group);
-    }
-  }
-}
-
 // The parts of the rows whose keys lie in several blocks' shares, in the order of the keys: eight lanes a row, 16 channels each.
 constexpr int JOIN_THREADS = 256, JOIN_ROWS = JOIN_THREADS / 8;
 template <bool ROWS2>
-__global__ void __launch_bounds__(JOIN_THREADS, ROWS2 ? 2 : 4) join_kernel(const __grid_constant__ TreeArgs a, int blocks) {
+__global__ void __launch_bounds__(JOIN_THREADS, ROWS2 ? 2 : 4) join_kernel(const __grid_constant__ TreeArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const Border border = a.borders[blockIdx.x];
-  const int lane = threadIdx.x & 31, warp = blockIdx.y * (JOIN_THREADS / 32) + (threadIdx.x >> 5), warps = gridDim.y * (JOIN_THREADS / 32);
+  const int lane = threadIdx.x & 31;
   const int row = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 3), rows = border.drafts * a.group;
   if (rows > blockIdx.y * JOIN_ROWS) {
-    bool odd = false;
-    for (int p = border.from + lane; p <= border.upto; p += 32) odd |= a.not_finite[p] != 0;
     const int draft = row / a.group, member = row - draft * a.group, row_head = border.head * a.group + member;
     const int local = min(ROWS2 && draft >= a.tile_drafts ? ROWS + (draft - a.tile_drafts) * a.group + member : row, (ROWS2 ? 2 * ROWS : ROWS) - 1);
     const int channel = 4 * (lane & 7);                    // and 32, 64, 96 behind it
@@ -798,14 +902,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, ROWS2 ? 2 : 4) join_kernel(const
       }
       top = m;
     }
-    if (__any_sync(0xffffffffu, odd)) {
-      const Sequence s = find_sequence<ROWS2>(a, a.cu_q[border.seq], a.cu_q[border.seq + 1], a.ctx_len[border.seq]);
-      const int here = (rows + JOIN_ROWS - 1) / JOIN_ROWS * (JOIN_THREADS / 32);      // warps of the blocks that come here
-      for (int r = warp; r < rows; r += here) {
-        const int d = r / a.group;
-        row_key_by_key(a, s, border.seq, border.head, border.token + d, border.head * a.group + r - d * a.group);
-      }
-    } else if (row < rows) {
+    if (row < rows) {
       const float inv = total == 0.f ? 0.f : 1.f / total;
       bf16* to = (bf16*)a.out + ((size_t)(border.token + draft) * a.q_heads + row_head) * DIM + channel;
 #pragma unroll
@@ -813,7 +910,6 @@ __global__ void __launch_bounds__(JOIN_THREADS, ROWS2 ? 2 : 4) join_kernel(const
         *reinterpret_cast<uint2*>(to + 32 * i) = make_uint2(pack_bf16(sum[i].x * inv, sum[i].y * inv), pack_bf16(sum[i].z * inv, sum[i].w * inv));
     }
   }
-  if (a.not_finite[blockIdx.x]) share_key_by_key<ROWS2>(a, blockIdx.x, blocks, warp, warps);
 }
 
 // The queries [tokens][q_heads][128]: 128 / group drafts with their heads of a group, 64 channels.
@@ -826,8 +922,8 @@ static bool query_map(CUtensorMap* map, const void* q, long tokens, int q_heads,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// scratch of `blocks` blocks, in floats: two places each of the partial outputs, their maxima and sums; the borders, and whose outputs are not finite
-static long scratch_floats(int blocks, bool rows2) { return 2L * blocks * (rows2 ? 2 * ROWS : ROWS) * (DIM + 2) + 9L * blocks; }
+// scratch of `blocks` blocks, in floats: two places each of the partial outputs, their maxima and sums; the borders; the rows' maxima and sums
+static long scratch_floats(int blocks, bool rows2, long rows) { return 2L * blocks * (rows2 ? 2 * ROWS : ROWS) * (DIM + 2) + 8L * blocks + 2 * rows; }
 
 template <bool ROWS2>
 int launch(TreeArgs a, int blocks, cudaStream_t stream) {
@@ -839,12 +935,12 @@ int launch(TreeArgs a, int blocks, cudaStream_t stream) {
   const long slots = 2L * blocks * (ROWS2 ? 2 * ROWS : ROWS);
   a.partial_stats = slots * DIM;
   a.borders = reinterpret_cast<Border*>(a.partials + slots * (DIM + 2));
-  a.not_finite = reinterpret_cast<int*>(a.borders + blocks);
+  a.row_stats = reinterpret_cast<float2*>(a.borders + blocks);
   a.group = group; a.tile_drafts = ROWS / group;
   int code = lb_launch(attention_tree_tcgen05_kernel<ROWS2>, blocks, THREADS, SMEM_BYTES, stream, q_map, a);
   if (code) return code;
   const int rows = min(a.max_nodes, a.tile_drafts * (ROWS2 ? 2 : 1)) * group;
-  return lb_launch(join_kernel<ROWS2>, dim3(blocks, (rows + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_THREADS, 0, stream, a, blocks);
+  return lb_launch(join_kernel<ROWS2>, dim3(blocks, (rows + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_THREADS, 0, stream, a);
 }
 }  // namespace wide
 }  // namespace

@@ -1313,14 +1313,14 @@ def tree_plan(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: i
 
 @functools.lru_cache(maxsize=1024)
 def tree_share(n_seqs: int, max_nodes: int, max_ctx: int, window: int, q_heads: int, kv_heads: int, sms: int) -> tuple[int, bool, int]:
-    """(blocks, whether a row tile is two tiles of 128 rows, floats of scratch) for the tcgen05 kernel of `attention_tree`: a block an SM, or
-    one for each tile of 128 keys where there are fewer."""
+    """(blocks, whether a row tile is two tiles of 128 rows, floats of the blocks' scratch) for the tcgen05 kernel of `attention_tree`: a block an
+    SM, or one for each tile of 128 keys where there are fewer."""
     drafts = 128 // (q_heads // kv_heads)
     rows2 = max_nodes > drafts
     keys = min(max_ctx, max_nodes + window) if window else max_ctx
     tiles = (-(-keys // 128) + (1 if window else 0)) * n_seqs * kv_heads * -(-max_nodes // (2 * drafts if rows2 else drafts))
     blocks = min(sms, tiles)
-    return blocks, rows2, 2 * blocks * (256 if rows2 else 128) * (128 + 2) + 9 * blocks
+    return blocks, rows2, 2 * blocks * (256 if rows2 else 128) * (128 + 2) + 8 * blocks
 
 
 def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
@@ -1379,6 +1379,7 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     sms = sm_count(device)
     if attention_tree_on_tcgen05(q_heads // kv_heads, dim, page_tokens, dtype) and out_ptr % 32 == 0:      # it stores 32 bytes a thread
         blocks, rows2, floats = tree_share(n_seqs, max_nodes, max_ctx, window, q_heads, kv_heads, sms)
+        floats += 2 * tokens * q_heads               # a row's maximum and sum
         scratch = torch.empty(floats, dtype=torch.float32, device=device)          # of this call alone, on its own stream
         fn = _FUNCTIONS.get("lb_attention_tree_tcgen05") or _fn("attention_tree", "lb_attention_tree_tcgen05",
                  [c_void_p] * 5 + [c_int, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float, c_int, c_void_p, c_float] + [c_int] * 3 + [c_void_p, c_long, c_void_p])

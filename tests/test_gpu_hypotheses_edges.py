@@ -83,3 +83,35 @@ def test_a_row_that_sees_nothing_is_zero_also_where_its_sink_is_minus_infinity(h
     got = case.run()[:10].view(10, 4, dim)
     assert (got[[0, 1, 2, 4, 5, 6, 7, 8, 9]] == 0).all()
     assert torch.equal(got[3, 1], case.v[0][held + 3, 0]) and torch.equal(got[3, 2], case.v[0][held + 3, 1])
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("q_heads, kv_heads, dim, nodes, held", [(4, 1, 128, 3, 40), (8, 2, 128, 20, 61), (4, 2, 128, 70, 1500), (32, 8, 128, 40, 900),
+                                                                (8, 2, 128, 30, 9000), (8, 2, 64, 20, 700), (4, 2, 128, 200, 300)])
+def test_a_draft_that_is_not_finite_changes_no_bit_of_who_does_not_see_it(q_heads, kv_heads, dim, nodes, held, dtype):
+    """Neither of other requests, nor of its own request's drafts, nor of heads whose values are finite; who sees it has what the formula says."""
+    lengths = [(held, nodes), (held // 2, nodes), (5, 2)]
+    case = Trees(lengths, q_heads, kv_heads, dim, dtype=dtype, seed=nodes).fill()
+    finite = case.run()
+    case.check(finite)
+    odd = (nodes // 2, nodes - 1)
+    for i, (place, value) in enumerate(zip(odd, (NAN, -INF))):
+        case.v[0][held + place, 0, 7 + i] = value          # the first key/value head's alone
+    got = case.fill().run()
+    case.check(got)
+    sees = case.seen[0][:, list(odd)].any(1)
+    group = q_heads // kv_heads * dim
+    assert torch.equal(got[:nodes, group:], finite[:nodes, group:])
+    assert torch.equal(got[:nodes][~sees], finite[:nodes][~sees])
+    assert torch.equal(got[nodes:], finite[nodes:])
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_drafts_that_are_not_finite_in_many_requests(dtype):
+    """Requests of several row tiles and parts of the keys, each with drafts that are not finite; the bits of two calls are the same."""
+    case = Trees([(700 + 300 * i, 5 + 9 * i) for i in range(7)], 8, 2, 128, dtype=dtype, seed=3)
+    for i in range(7):
+        case.v[i][-1 - i, i % 2, 11 * i] = (NAN, INF, -INF)[i % 3]
+    got = case.fill().run()
+    case.check(got)
+    assert torch.equal(torch.nan_to_num(got, 99.0), torch.nan_to_num(case.run(), 99.0))

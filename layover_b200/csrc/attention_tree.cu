@@ -20,8 +20,8 @@
 //   attention_tree_f32_kernel   float32, FFMA: 8 x 16 threads, RT / 8 rows and 2 keys (dim / 16 channels) each
 //
 // The values of a draft may be anything (a draft whose arithmetic overflowed): what a row does not see must not reach it, and
-// 0 x NaN is NaN. So in tiles that hold drafts, value rows that are not finite are taken out of the product and added one by
-// one to the rows that see them.
+// 0 x NaN is NaN. So in tiles that hold drafts, or held keys that lie behind the window of some row, value rows that are not finite are
+// taken out of the product and added one by one to the rows that see them.
 //
 // Bounds. bfloat16: the keys' and values' bytes and, with few keys, the time to start two launches and to reach a page through its
 // table; 5 requests of 13 drafts behind a window of 1,024, 12 heads over 2 of 64 channels 16.5 us. 32 bits: 2 x rows x keys x dim FFMA a
@@ -87,7 +87,8 @@ template <int RG, int MAX_DIM>
 __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tree_mma_kernel(const TreeArgs a) {
   constexpr int KG = 4 / RG, NT = KEYS / KG / 8, KSTEPS = MAX_DIM / 16, NT_O = MAX_DIM / 8, STAGES = 2;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  __shared__ unsigned bad_rows[4];                         // per 16 keys of a tile with drafts: value rows that are not finite
+  __shared__ unsigned bad_rows[4];                         // per 16 keys of a tile that is looked at: value rows that are not finite
+  __shared__ int hidden_s[4];                              // per warp: below it are held keys that a row does not see
   const int stride = a.dim + PAD, dk = a.dim >> 4;
   bf16* q_s = reinterpret_cast<bf16*>(smem_raw);           // [16 RG][stride]
   bf16* k_s = q_s + 16 * RG * stride;                      // [STAGES][KEYS][stride]
@@ -127,6 +128,10 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
     bits[r] = a.tree + (size_t)token * a.tree_words;
     oldest[r] = a.window > 0 ? max(a.positions[token], u.held) - a.window + 1 : 0;
   }
+  if (a.window > 0) {
+    const int most = __reduce_max_sync(0xffffffffu, max(oldest[0], oldest[1]));
+    if (lane == 0) hidden_s[warp] = most;
+  }
   uint32_t qf[KSTEPS][4];
   float o[NT_O][4];
 #pragma unroll
@@ -156,14 +161,17 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
     }
     const int key0 = tile * KEYS;
     const bool drafts = key0 + KEYS > u.held;
-    if (drafts) {                                          // two threads look at a value row
+    const int hidden = a.window > 0 ? max(max(hidden_s[0], hidden_s[1]), max(hidden_s[2], hidden_s[3])) : 0;
+    const bool looked = drafts || key0 < hidden;
+    if (looked) {                                          // two threads look at a value row
       bf16* row = v_s + buf * KEYS * stride + (threadIdx.x >> 1) * stride;
       bool bad = false;
       for (int c = (threadIdx.x & 1); c < a.dim >> 3; c += 2) {
         const uint4 w = *reinterpret_cast<const uint4*>(row + c * 8);
         bad |= not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w);
       }
-      const unsigned both = __ballot_sync(0xffffffffu, bad && key0 + (int)(threadIdx.x >> 1) >= u.held);
+      const int key = key0 + (int)(threadIdx.x >> 1);
+      const unsigned both = __ballot_sync(0xffffffffu, bad && (key >= u.held || key < hidden));
       unsigned rows = 0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) rows |= ((both >> (2 * i)) & 3u) ? 1u << i : 0u;
@@ -242,13 +250,13 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
         mma_bf16(o[n + 1], p, b[2], b[3]);
       }
     }
-    if (drafts && (bad_rows[0] | bad_rows[1] | bad_rows[2] | bad_rows[3])) {
+    if (looked && (bad_rows[0] | bad_rows[1] | bad_rows[2] | bad_rows[3])) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         for (int i = 0; i < 8; ++i) {
           const int local = key_w + n * 8 + i;
           if (!(bad_rows[local >> 4] >> (local & 15) & 1u)) continue;
-          const long from = key_row(a, table, key0 + local, u.head);       // a draft's row, which was read: it is there
+          const long from = key_row(a, table, key0 + local, u.head);       // its values were read: it is there
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const float w = __shfl_sync(0xffffffffu, i & 1 ? s[n][2 * r + 1] : s[n][2 * r], (lane & 28) | (i >> 1));
@@ -354,6 +362,7 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f3
   constexpr int RPT = RT / 8, KEYS = F32_KEYS, KPT = KEYS / 16;      // rows and keys of a thread
   extern __shared__ __align__(16) float smem_f[];
   __shared__ unsigned bad_rows[4];
+  __shared__ int hidden_s[4];
   const int stride = a.dim + 4;                            // rows 16 bytes apart modulo 128: eight rows' pieces lie in different banks
   float* q_s = smem_f;                                     // [RT][stride]
   float* k_s = q_s + RT * stride;                          // [KEYS][stride]
@@ -389,6 +398,13 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f3
     bits[i] = a.tree + (size_t)token * a.tree_words;
     oldest[i] = a.window > 0 ? max(a.positions[token], u.held) - a.window + 1 : 0;
   }
+  if (a.window > 0) {
+    int most = oldest[0];
+#pragma unroll
+    for (int i = 1; i < RPT; ++i) most = max(most, oldest[i]);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((threadIdx.x & 31) == 0) hidden_s[threadIdx.x >> 5] = most;
+  }
   float2 o[RPT][MAX_C][2];
   float m_run[RPT], l_run[RPT];
 #pragma unroll
@@ -404,6 +420,7 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f3
     __syncthreads();
     const int key0 = tile * KEYS;
     const bool drafts = key0 + KEYS > u.held;
+    const bool looked = drafts || (a.window > 0 && key0 < max(max(hidden_s[0], hidden_s[1]), max(hidden_s[2], hidden_s[3])));
     float2 pairs[RPT][KPT];                                  // sums over the even and over the odd channels
 #pragma unroll
     for (int i = 0; i < RPT; ++i)
@@ -465,7 +482,7 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f3
     __syncthreads();                                       // values and weights are there, the keys are done with
     if (tile + 1 < u.tile_end) load_tile<KEYS>(k_s, k_pool, a, u, table, tile + 1, stride);
     cp_async_commit();
-    if (drafts) {
+    if (looked) {
       const float* row = v_s + (threadIdx.x >> 2) * stride;                  // four threads look at a value row
       bool bad = false;
       for (int c = threadIdx.x & 3; c < a.dim >> 2; c += 4) {
@@ -476,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f3
       if ((threadIdx.x & 31) == 0) bad_rows[threadIdx.x >> 5] = both;
       __syncthreads();
     }
-    const bool any_bad = drafts && (bad_rows[0] | bad_rows[1] | bad_rows[2] | bad_rows[3]);
+    const bool any_bad = looked && (bad_rows[0] | bad_rows[1] | bad_rows[2] | bad_rows[3]);
     auto values = [&](auto some_bad) {
 #pragma unroll 1
       for (int key = 0; key < KEYS; key += 4) {

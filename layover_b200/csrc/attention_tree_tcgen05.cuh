@@ -28,7 +28,8 @@
 // more, carefully: in tiles of which a row may not see every key, zeros stand for values that are not finite, and who sees those gets their
 // terms added afterwards. So who does not see them has the bits that he would have beside finite ones, and a call without them pays nothing: to look at
 // the drafts' values in every call costs 4 of 38 us and 14 to 26 of 156 (8 x 32 and 40 requests), whichever warp does it, for what runs seldom waits for its
-// instructions. With one draft of NaN a call that is waited for takes 122 us instead of 62 (8 x 32) and 537 instead of 194 (40 requests).
+// instructions. With one draft of NaN a call that is waited for takes 122 us instead of 62 (8 x 32) and 537 instead of 194 (40 requests). (Its rows
+// made again key by key: 10,100 and 21,800.)
 #pragma once
 #include <math.h>
 

@@ -115,3 +115,16 @@ def test_drafts_that_are_not_finite_in_many_requests(dtype):
     got = case.fill().run()
     case.check(got)
     assert torch.equal(torch.nan_to_num(got, 99.0), torch.nan_to_num(case.run(), 99.0))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("q_heads, kv_heads, dim", [(8, 2, 64), (8, 2, 128), (2, 1, 16)])
+@pytest.mark.parametrize("window", [30, 64, 700])
+def test_a_held_value_behind_a_window_reaches_only_who_sees_it(window, q_heads, kv_heads, dim, dtype):
+    """Held tokens at the window's edge, which the first drafts see and the deeper ones do not, may be anything."""
+    n, held = 20, 900
+    case = Trees([(held, n), (held, n)], q_heads, kv_heads, dim, dtype=dtype, window=window, seen=[torch.ones(n, n).tril().bool()] * 2, seed=window)
+    case.v[0][held - window + 6, :, 3], case.v[0][held - window + 11, :, dim - 1] = NAN, INF      # seen by the first 6 and 11 drafts
+    got = case.fill().run()
+    case.check(got)
+    assert torch.isnan(got[:6].float()).any(1).all() and torch.isfinite(got[11:n]).all()

@@ -12,7 +12,7 @@
 // key/value head and the drafts are the rows of one tile (row = draft * group + head of the group), so every key and value is read
 // once for all of them. The reference has no drafts: it decodes one token a request and step (layover/engine.py:176-189).
 //
-// Blocks: (key/value head, sequence x row tile, chunk of the keys). Chunks have the same number of key tiles for every sequence, so
+// Blocks: (sequence x row tile x key/value head, the head fastest; chunk of the keys). Chunks have the same number of key tiles for every sequence, so
 // blocks take equally long whatever the lengths, and one that lies behind its sequence's end leaves at once. Where there is more
 // than one chunk each leaves its maxima, sums and unnormalised outputs in scratch memory of this call, and a second kernel joins them.
 //
@@ -95,9 +95,9 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
   bf16* v_s = k_s + STAGES * KEYS * stride;
   pdl_launch_dependents();
   pdl_wait();
-  const int seq = blockIdx.y / a.row_tiles;
-  const Unit u = find_unit<KEYS>(a, 16 * RG, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
-  if (u.rows <= 0 || (int)blockIdx.z >= u.chunks) return;
+  const int row_tile_of = blockIdx.x / a.kv_heads, seq = row_tile_of / a.row_tiles;
+  const Unit u = find_unit<KEYS>(a, 16 * RG, seq, row_tile_of - seq * a.row_tiles, blockIdx.x - row_tile_of * a.kv_heads, blockIdx.y, gridDim.y);
+  if (u.rows <= 0 || (int)blockIdx.y >= u.chunks) return;
   const int group = a.q_heads / a.kv_heads;
   const int* table = a.block_table + (size_t)seq * a.table_width;
   const bf16 *q = (const bf16*)a.q, *k_pool = (const bf16*)a.k_pool, *v_pool = (const bf16*)a.v_pool;
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, MAX_DIM == 128 ? 2 : 1) attention_tre
     const int local = rg * 16 + g + 8 * r, row = u.row0 + local;
     if (local >= u.rows) continue;
     if (u.chunks > 1) {
-      const long at = (u.index * gridDim.z + blockIdx.z) * (16 * RG) + local;
+      const long at = (u.index * gridDim.y + blockIdx.y) * (16 * RG) + local;
       float* to = a.partials + at * a.dim;
 #pragma unroll
       for (int n = 0; n < NT_O; ++n)
@@ -371,9 +371,9 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f3
   constexpr int P_STRIDE = KEYS + 4;
   pdl_launch_dependents();
   pdl_wait();
-  const int seq = blockIdx.y / a.row_tiles;
-  const Unit u = find_unit<KEYS>(a, RT, seq, blockIdx.y - seq * a.row_tiles, blockIdx.x, blockIdx.z, gridDim.z);
-  if (u.rows <= 0 || (int)blockIdx.z >= u.chunks) return;
+  const int row_tile_of = blockIdx.x / a.kv_heads, seq = row_tile_of / a.row_tiles;
+  const Unit u = find_unit<KEYS>(a, RT, seq, row_tile_of - seq * a.row_tiles, blockIdx.x - row_tile_of * a.kv_heads, blockIdx.y, gridDim.y);
+  if (u.rows <= 0 || (int)blockIdx.y >= u.chunks) return;
   const int group = a.q_heads / a.kv_heads;
   const int* table = a.block_table + (size_t)seq * a.table_width;
   const float *q = (const float*)a.q, *k_pool = (const float*)a.k_pool, *v_pool = (const float*)a.v_pool;
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, MAX_C == 2 ? 4 : 2) attention_tree_f3
     const int local = ty + 8 * i, row = u.row0 + local;
     if (local >= u.rows) continue;
     if (u.chunks > 1) {
-      const long at = (u.index * gridDim.z + blockIdx.z) * RT + local;
+      const long at = (u.index * gridDim.y + blockIdx.y) * RT + local;
 #pragma unroll
       for (int c = 0; c < MAX_C; ++c)
         if (64 * c + 4 * tx < a.dim)
@@ -558,9 +558,9 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) attention_tree_join_kernel(const TreeArgs a, int tile_rows, int n_chunks) {
   pdl_launch_dependents();
   pdl_wait();
-  const int seq = blockIdx.y / a.row_tiles, row_tile = blockIdx.y - seq * a.row_tiles;
-  const Unit u = find_unit<sizeof(T) == 4 ? F32_KEYS : KEYS>(a, tile_rows, seq, row_tile, blockIdx.x, 0, n_chunks);
-  const int local = blockIdx.z * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row_tile_of = blockIdx.x / a.kv_heads, seq = row_tile_of / a.row_tiles;
+  const Unit u = find_unit<sizeof(T) == 4 ? F32_KEYS : KEYS>(a, tile_rows, seq, row_tile_of - seq * a.row_tiles, blockIdx.x - row_tile_of * a.kv_heads, 0, n_chunks);
+  const int local = blockIdx.y * (THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (local >= u.rows || u.chunks <= 1) return;
   const int group = a.q_heads / a.kv_heads, row = u.row0 + local, head = u.head * group + row % group;
   const long at = u.index * n_chunks * tile_rows + local;
@@ -618,11 +618,11 @@ int launch_f32(const TreeArgs& a, dim3 grid, cudaStream_t stream) { return a.dim
 
 // What the two entries below check alike.
 static int check_tree(int dtype, const void* q, const void* k_pool, const void* v_pool, const void* out, int table_width, int n_pages, const int* positions,
-                      int tree_words, int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, int window, float softcap, int max_nodes) {
+                      int tree_words, int tokens, int q_heads, int kv_heads, int dim, int page_tokens, int window, float softcap, int max_nodes) {
   if (dtype != LB_F32 && dtype != LB_BF16) return LB_ERR_DTYPE;
   if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || dim <= 0 || dim > 256 || dim % (dtype == LB_BF16 ? 16 : 4) || page_tokens <= 0 ||
-      table_width <= 0 || n_pages <= 0 || tree_words <= 0 || window < 0 || softcap < 0.f || (window > 0 && !positions) || max_nodes <= 0 || n_seqs > 65535 ||
-      (long)max_nodes * (q_heads / kv_heads) > 65535)
+      table_width <= 0 || n_pages <= 0 || tree_words <= 0 || window < 0 || softcap < 0.f || (window > 0 && !positions) || max_nodes <= 0 ||
+      (long)max(max_nodes, tokens) * (q_heads / kv_heads) > 0x7fffffffL - 256)      // rows are counted in 32 bits
     return LB_ERR_SIZE;
   if (((uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)out) & 15) return LB_ERR_ALIGN;
   return 0;
@@ -636,10 +636,10 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
                                 float softcap, int max_nodes, int tile_rows, int row_tiles, int chunks, int chunk_tiles, float* partials,
                                 long partial_floats, cudaStream_t stream) {
   if (tokens <= 0 || n_seqs <= 0) return 0;
-  const int refused = check_tree(dtype, q, k_pool, v_pool, out, table_width, n_pages, positions, tree_words, n_seqs, q_heads, kv_heads, dim, page_tokens,
+  const int refused = check_tree(dtype, q, k_pool, v_pool, out, table_width, n_pages, positions, tree_words, tokens, q_heads, kv_heads, dim, page_tokens,
                                  window, softcap, max_nodes);
   if (refused) return refused;
-  if (row_tiles <= 0 || chunks <= 0 || chunks > 65535 || chunk_tiles <= 0 || (long)n_seqs * row_tiles > 65535 ||
+  if (row_tiles <= 0 || chunks <= 0 || chunks > 65535 || chunk_tiles <= 0 || (double)n_seqs * row_tiles * kv_heads > 0x7fffffff ||
       (tile_rows != 16 && tile_rows != 32 && (tile_rows != 64 || dtype != LB_BF16)))
     return LB_ERR_SIZE;
   const long partial_rows = (long)n_seqs * kv_heads * row_tiles * chunks * tile_rows;
@@ -649,7 +649,7 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
              page_tokens, scale * LOG2E, 0.f, 0.f, window, sinks, row_tiles, chunk_tiles, chunks > 1 ? partials : nullptr, partial_rows * dim, n_seqs,
              max_nodes, 0, 0, nullptr, nullptr};
   if (softcap > 0.f) { a.cap_in = 2.f * LOG2E * scale / softcap; a.cap_out = softcap / scale; }
-  const dim3 grid(kv_heads, n_seqs * row_tiles, chunks);
+  const dim3 grid((unsigned)(n_seqs * row_tiles * kv_heads), chunks);
   int code;
   if (dtype == LB_F32) {
     code = tile_rows == 16 ? launch_f32<16>(a, grid, stream) : launch_f32<32>(a, grid, stream);
@@ -659,7 +659,7 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
     code = tile_rows == 16 ? launch_mma<1, 256>(a, grid, stream) : tile_rows == 32 ? launch_mma<2, 256>(a, grid, stream) : launch_mma<4, 256>(a, grid, stream);
   }
   if (code || chunks == 1) return code ? code : lb_last_error();
-  const dim3 joined(kv_heads, n_seqs * row_tiles, tile_rows / (THREADS / 32));
+  const dim3 joined(grid.x, tile_rows / (THREADS / 32));
   code = dtype == LB_F32 ? lb_launch(attention_tree_join_kernel<float>, joined, THREADS, 0, stream, a, tile_rows, chunks)
                          : lb_launch(attention_tree_join_kernel<bf16>, joined, THREADS, 0, stream, a, tile_rows, chunks);
   return code ? code : lb_last_error();
@@ -674,10 +674,12 @@ LB_EXPORT int lb_attention_tree_tcgen05(const void* q, const void* k_pool, const
                                         const float* sinks, float softcap, int max_nodes, int blocks, int rows2, float* scratch, long floats,
                                         cudaStream_t stream) {
   if (tokens <= 0 || n_seqs <= 0) return 0;
-  const int refused = check_tree(LB_BF16, q, k_pool, v_pool, out, table_width, n_pages, positions, tree_words, n_seqs, q_heads, kv_heads, dim, page_tokens,
+  const int refused = check_tree(LB_BF16, q, k_pool, v_pool, out, table_width, n_pages, positions, tree_words, tokens, q_heads, kv_heads, dim, page_tokens,
                                  window, softcap, max_nodes);
   if (refused) return refused;
-  if (dim != 128 || q_heads / kv_heads > 128 || page_tokens % 8 || 128 % page_tokens || blocks <= 0 || blocks > 1024 || !scratch ||
+  // key tiles are counted in 32 bits too
+  const double most_tiles = (double)n_seqs * kv_heads * (max_nodes / (128 / max(1, min(128, q_heads / kv_heads))) + 1) * ((double)table_width * page_tokens / 128 + 1);
+  if (most_tiles > 0x7fffffff || dim != 128 || q_heads / kv_heads > 128 || page_tokens % 8 || 128 % page_tokens || blocks <= 0 || blocks > 1024 || !scratch ||
       floats < wide::scratch_floats(blocks, rows2 != 0, (long)tokens * q_heads))
     return LB_ERR_SIZE;
   if (((uintptr_t)scratch | (uintptr_t)out) & 31) return LB_ERR_ALIGN;

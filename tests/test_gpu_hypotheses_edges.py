@@ -128,3 +128,64 @@ def test_a_held_value_behind_a_window_reaches_only_who_sees_it(window, q_heads, 
     got = case.fill().run()
     case.check(got)
     assert torch.isnan(got[:6].float()).any(1).all() and torch.isfinite(got[11:n]).all()
+
+
+def few_keys(q, keys, values, scale):
+    """(outputs, sums of weight times |value|, the largest sum of |q k|) of rows that see the same few keys each: q [R, heads, dim],
+    keys and values [R, keys, dim], in 64 bits."""
+    q, keys, values = q.double(), keys.double(), values.double()
+    z = torch.einsum("rhd,rkd->rhk", q, keys) * scale
+    p = torch.softmax(z, 2)
+    return (torch.einsum("rhk,rkd->rhd", p, values), torch.einsum("rhk,rkd->rhd", p, values.abs()),
+            float((torch.einsum("rhd,rkd->rhk", q.abs(), keys.abs()) * scale).max()))
+
+
+def few_keys_bound(want, sums, size, dim, dtype, n_keys):
+    """As `Trees.check`: a score's dim + 4 roundings, the exponential's 2^-18, a rounding of the sums for each of the keys seen and for each of the tiles
+    (whose other keys add zeros); in bfloat16 the weights' and the result's."""
+    step = 2.0 ** -24
+    bound = (2 * ((dim + 4) * step * size + 2.0 ** -18) + 2 * (n_keys + 300) * step) * sums + 1e-30
+    return bound + 2.0 ** -8 * sums + 2.0 ** -8 * (want.abs() + bound) if dtype == torch.bfloat16 else bound + step * want.abs()
+
+
+@pytest.mark.parametrize("dtype, dim, heads", [(torch.bfloat16, 16, 8), (torch.bfloat16, 128, 8), (torch.float32, 16, 8)])
+def test_tree_attention_of_more_than_65535_rows(dtype, dim, heads):
+    """A long portion beside drafts: its last row is far behind the 65,535th. Each draft sees itself and the one before it."""
+    o, n, page = ops(), 8300, 16
+    gen = torch.Generator().manual_seed(dim)
+    q, k, v = (torch.randn(n, h * dim, generator=gen).to(dtype) for h in (heads, 1, 1))
+    words = -(-n // 32)
+    tree = torch.zeros(n, words, dtype=torch.int64)
+    at = torch.arange(n)
+    tree[at, at // 32] |= 1 << at % 32
+    tree[at[1:], at[:-1] // 32] |= 1 << at[:-1] % 32
+    tree = torch.where(tree >= 1 << 31, tree - (1 << 32), tree).to(torch.int32).cuda()
+    pages = -(-n // page)
+    pools = [torch.zeros(pages * page, dim, dtype=dtype).index_copy_(0, at, x).view(pages, 1, page, dim).cuda() for x in (k, v)]
+    put = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    out = torch.empty(n, heads * dim, dtype=dtype, device="cuda")
+    o.attention_tree(q.cuda(), *pools, out, torch.arange(pages, dtype=torch.int32).view(1, -1).cuda(), put([0, n]), put([n]), None, tree, 1, heads, 1, dim,
+                     page, dim ** -0.5, n, n)
+    assert o.attention_tree_status() == 0
+    pair = torch.stack((at[1:], at[:-1]), 1)
+    want, sums, size = few_keys(q.view(n, heads, dim)[1:], k[pair], v[pair], dim ** -0.5)
+    got = out.cpu().view(n, heads, dim)
+    assert torch.equal(got[0], v[0].expand(heads, dim))
+    assert ((got[1:].double() - want).abs() <= few_keys_bound(want, sums, size, dim, dtype, 2)).all()
+
+
+@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 16), (torch.bfloat16, 128), (torch.float32, 16)])
+def test_tree_attention_of_more_than_65535_requests(dtype, dim):
+    """Each holds one token and brings a draft that sees both."""
+    o, n, page = ops(), 66_000, 8
+    gen = torch.Generator().manual_seed(dim)
+    q = torch.randn(n, 2 * dim, generator=gen).to(dtype)
+    pools = [torch.randn(n, 1, page, dim, generator=gen).to(dtype) for _ in range(2)]
+    order = torch.randperm(n, generator=gen)
+    out = torch.empty(n, 2 * dim, dtype=dtype, device="cuda")
+    o.attention_tree(q.cuda(), pools[0].cuda(), pools[1].cuda(), out, order.to(torch.int32).view(n, 1).cuda(), torch.arange(n + 1, dtype=torch.int32).cuda(),
+                     torch.full((n,), 2, dtype=torch.int32, device="cuda"), None, torch.ones(n, 1, dtype=torch.int32, device="cuda"), n, 2, 1, dim, page,
+                     dim ** -0.5, 1, 2)
+    assert o.attention_tree_status() == 0
+    want, sums, size = few_keys(q.view(n, 2, dim), pools[0][order, 0, :2], pools[1][order, 0, :2], dim ** -0.5)
+    assert ((out.cpu().view(n, 2, dim).double() - want).abs() <= few_keys_bound(want, sums, size, dim, dtype, 2)).all()

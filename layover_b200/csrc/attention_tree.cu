@@ -666,8 +666,7 @@ LB_EXPORT int lb_attention_tree(int dtype, const void* q, const void* k_pool, co
 }
 
 // The tcgen05 kernel: bfloat16, heads of 128 channels, at most 128 query heads a key/value head, pages of 8 .. 128 tokens that divide 128. `blocks` blocks
-// share the keys; `rows2`: tiles of twice 128 / group drafts. `scratch` holds lb_attention_tree_scratch(blocks, rows2, tokens * q_heads) floats.
-LB_EXPORT long lb_attention_tree_scratch(int blocks, int rows2, long rows) { return wide::scratch_floats(blocks, rows2 != 0, rows); }
+// share the keys; `rows2`: tiles of twice 128 / group drafts. `scratch` holds wide::scratch_floats(blocks, rows2, tokens * q_heads) of them.
 LB_EXPORT int lb_attention_tree_tcgen05(const void* q, const void* k_pool, const void* v_pool, void* out, const int* block_table, int table_width,
                                         int n_pages, const int* cu_q, const int* ctx_len, const int* positions, const int* tree, int tree_words,
                                         int tokens, int n_seqs, int q_heads, int kv_heads, int dim, int page_tokens, float scale, int window,

@@ -113,7 +113,7 @@ __device__ __forceinline__ float reached_by(float top, int keep, int* keys, floa
 // A chunk is `pieces` of PIECE values. Rows of beams that are not there or have ended are not read, and nothing is written for them.
 constexpr int EACH = 14, PIECE = THREADS * EACH;
 __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const float* __restrict__ logits, long row_stride, const float* __restrict__ scores,
-                                                                const int* __restrict__ ended, int vocab, int keep, int pieces,
+                                                                const int* __restrict__ ended, int vocab, int keep, int pieces, int chunks,
                                                                 float2* __restrict__ stats, float2* __restrict__ lists) {
   __shared__ __align__(16) int keys[64];
   __shared__ float worth[WARPS][WARP_ROOM], part[WARPS], part_sum[WARPS], threshold, last_threshold;
@@ -121,11 +121,12 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const float* __r
   __shared__ int found[WARPS][WARP_ROOM], total;
   pdl_launch_dependents();
   pdl_wait();
-  const float* row = logits + (size_t)blockIdx.y * row_stride;
-  const int begin = blockIdx.x * pieces * PIECE, end = min(vocab, begin + pieces * PIECE), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row_at = blockIdx.x / chunks;
+  const float* row = logits + (size_t)row_at * row_stride;
+  const int begin = (blockIdx.x - row_at * chunks) * pieces * PIECE, end = min(vocab, begin + pieces * PIECE), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float next[EACH], m = -INFINITY, sum = 0.f, bar = -FLT_MAX;      // what does not reach `bar` is not among the best
   int held = 0;                                            // indices in `found` of this warp, in their order
-  const bool wanted = scores[blockIdx.y] > -INFINITY && !(ended && ended[blockIdx.y]);
+  const bool wanted = scores[row_at] > -INFINITY && !(ended && ended[row_at]);
 #pragma unroll
   for (int j = 0; j < EACH; ++j) next[j] = begin + (int)threadIdx.x + j * THREADS < end ? row[begin + threadIdx.x + j * THREADS] : -INFINITY;
   if (!wanted) return;                                     // the first piece was asked for all the same: the others would wait for this
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const float* __r
   at = __shfl_sync(0xffffffffu, at, 0) + __popc(with & ((1u << lane) - 1u));
   if (v >= bar) all_best[at] = make_float2(v, __int_as_float(i));
   __syncthreads();
-  const size_t chunk = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const size_t chunk = blockIdx.x;
   float2* list = lists + chunk * keep;
   const int n = total;                                     // 32 of each warp at most
   if ((int)threadIdx.x < n) {
@@ -333,13 +334,14 @@ LB_EXPORT int lb_beam_select(const float* logits, long row_stride, const float* 
                              int pad, int pieces, void* scratch, long scratch_words, float* next_scores, int* parents, int* tokens, cudaStream_t stream) {
   if (requests <= 0) return 0;
   if (beams <= 0 || beams > MAX_BEAMS || keep <= 0 || keep > MAX_KEEP || vocab <= 0 || pieces <= 0 || pieces > 0x7fffffff / PIECE || pad < 0 || pad >= vocab ||
-      (long)beams * vocab >= 0x7fffffffL - PIECE || (long)requests * beams > 65535)
+      (long)beams * vocab > 0x7fffffffL - (pieces + 2L) * PIECE)      // places, and the ends of chunks and of the pieces ahead, are counted in 32 bits
     return LB_ERR_SIZE;
   const long rows = (long)requests * beams, chunks = (vocab + (long)PIECE * pieces - 1) / ((long)PIECE * pieces);
+  if (rows * chunks > 0x7fffffffL) return LB_ERR_SIZE;
   if (scratch_words < rows * chunks * (2 + 2 * keep)) return LB_ERR_SIZE;
   if ((uintptr_t)scratch & 7) return LB_ERR_ALIGN;
   float2 *stats = (float2*)scratch, *lists = stats + rows * chunks;
-  int code = lb_launch(beam_chunk_kernel, dim3((unsigned)chunks, (unsigned)rows), THREADS, 0, stream, logits, row_stride, scores, ended, vocab, keep, pieces, stats, lists);
+  int code = lb_launch(beam_chunk_kernel, dim3((unsigned)(rows * chunks)), THREADS, 0, stream, logits, row_stride, scores, ended, vocab, keep, pieces, (int)chunks, stats, lists);
   if (code) return code;
   code = lb_launch(beam_join_kernel, requests, THREADS, 0, stream, scores, ended, beams, vocab, keep, pad, (int)chunks, stats, lists, next_scores, parents, tokens);
   return code ? code : lb_last_error();

@@ -1454,6 +1454,7 @@ def compact_tokens(pool: torch.Tensor, block_table: torch.Tensor, first: torch.T
 
 BEAM_MAX_KEEP = 32      # the most continuations that `beam_select` chooses
 BEAM_MAX_BEAMS = 64     # the most beams of a request
+BEAM_MAX_PLACES = 2 ** 31 - 2 ** 15     # the most beams x vocabulary: places are counted in 32 bits
 
 
 _BEAM_PIECE = 3584      # values of a row that a block of the first kernel looks at together (csrc/beam.cu)
@@ -1477,7 +1478,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, next_scores: torch.T
     with equal ones in the order of b * vocab + v. logits float32 [requests * beams, V] (rows may be strided); scores float32 [requests,
     beams], -inf for a beam that is not there; next_scores float32 [requests, keep], parents and tokens int32 alike, keep up to
     BEAM_MAX_KEEP. `ended` int32 [requests, beams]: an ended beam (not 0) is one candidate, its own score with token `pad`. A beam whose
-    logits hold NaN or +inf, or nothing but -inf, has no candidates; places without a candidate get -inf, -1 and -1."""
+    logits hold NaN or +inf, or nothing but -inf, has no candidates; places without a candidate get -inf, -1 and -1. Beams times vocabulary
+    are at most BEAM_MAX_PLACES."""
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError("beam_select: logits must be float32 [rows, vocab] with a contiguous vocabulary")
     _need(scores, torch.float32, "scores"); _need(next_scores, torch.float32, "next_scores")
@@ -1489,6 +1491,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, next_scores: torch.T
     keep, vocab = next_scores.shape[1], logits.shape[1]
     if not 1 <= keep <= BEAM_MAX_KEEP or not 1 <= beams <= BEAM_MAX_BEAMS or not 0 <= pad < vocab:
         raise ValueError(f"beam_select: keep is 1..{BEAM_MAX_KEEP}, beams 1..{BEAM_MAX_BEAMS}, pad a token of the vocabulary")
+    if beams * vocab > BEAM_MAX_PLACES:
+        raise ValueError(f"beam_select: beams times vocabulary are at most {BEAM_MAX_PLACES}")
     if ended is not None:
         _need(ended, torch.int32, "ended")
         if ended.shape != scores.shape:

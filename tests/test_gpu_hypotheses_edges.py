@@ -189,3 +189,18 @@ def test_tree_attention_of_more_than_65535_requests(dtype, dim):
     assert o.attention_tree_status() == 0
     want, sums, size = few_keys(q.view(n, 2, dim), pools[0][order, 0, :2], pools[1][order, 0, :2], dim ** -0.5)
     assert ((out.cpu().view(n, 2, dim).double() - want).abs() <= few_keys_bound(want, sums, size, dim, dtype, 2)).all()
+
+
+def test_beam_selection_of_more_than_65535_rows():
+    gen = torch.Generator().manual_seed(8)
+    requests, beams, vocab, keep = 17_000, 4, 40, 5
+    logits, scores = torch.randn(requests * beams, vocab, generator=gen), -3 * torch.rand(requests, beams, generator=gen)
+    outs = torch.empty(requests, keep).cuda(), *(torch.empty(requests, keep, dtype=torch.int32).cuda() for _ in range(2))
+    ops().beam_select(logits.cuda(), scores.cuda(), *outs)
+    values, places = (scores.double()[:, :, None] + torch.log_softmax(logits.double(), 1).view(requests, beams, vocab)).flatten(1).topk(keep + 1)
+    got = outs[1].cpu().long() * vocab + outs[2].cpu()
+    # where two lie within 1e-7 either may come first
+    apart = (values[:, :-1] - values[:, 1:]).amin(1) > 1e-6
+    values, places = values[:, :keep], places[:, :keep]
+    assert apart.sum() > 16_000 and torch.equal(got[apart], places[apart])
+    assert ((outs[0].cpu().double() - values).abs() <= 2.0 ** -24 * values.abs() + 2.0 ** -18).all()

@@ -1415,10 +1415,13 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torc
     """pool[:, dst[i]] = pool[:, src[i]] for every i: pool [planes, pages, ...] of any type (the layers' pages of a cache, or the
     layers' state slots), src and dst int32 [n] on the device. A page may be the source of several copies; no page is written twice or
     read and written in one call. A pair with an index outside the pool is left out. What is launched behind the call, on its stream or in
-    the same graph, finds the pages copied, decode attention too, which reads earlier keys ahead of the kernel before it."""
+    the same graph, finds the pages copied, decode attention too, which reads earlier keys ahead of the kernel before it. Planes and copies
+    are at most 65,535."""
     _need(pool, None, "pool"); _need(src, torch.int32, "src"); _need(dst, torch.int32, "dst")
     if pool.dim() < 2 or src.dim() != 1 or src.shape != dst.shape:
         raise ValueError("copy_pages: pool [planes, pages, ...], src and dst one index per copy")
+    if max(pool.shape[0], src.numel()) > 65535:
+        raise ValueError("copy_pages: planes and copies are at most 65535")
     pool_ptr, src_ptr, dst_ptr = _pointers("copy_pages", pool, src, dst)
     planes, pages = pool.shape[:2]
     if pool.numel() == 0 or src.numel() == 0:
@@ -1434,15 +1437,18 @@ def compact_tokens(pool: torch.Tensor, block_table: torch.Tensor, first: torch.T
     picked[cu_picked[s]] < picked[cu_picked[s] + 1] < ...; the row at place first[s] + picked[cu_picked[s] + i] goes to place first[s] + i. All
     indices int32 on the device, block_table [S, W] the sequences' pages. Sequences do not share the pages these places are in. A draft that
     lies outside its sequence's table, or whose page is outside the pool, is left out. What is launched behind the call, on its stream or in
-    the same graph, finds the rows moved, decode attention too, which reads earlier keys ahead of the kernel before it."""
+    the same graph, finds the rows moved, decode attention too, which reads earlier keys ahead of the kernel before it. Sequences are at most
+    65,535, a token's rows in all planes and heads at most 2^31 bytes."""
     _need(pool, None, "pool")
     for name, t in (("block_table", block_table), ("first", first), ("picked", picked), ("cu_picked", cu_picked)):
         _need(t, torch.int32, name)
     n_seqs = first.numel()
     if pool.dim() != 5 or block_table.dim() != 2 or block_table.shape[0] < n_seqs or cu_picked.numel() != n_seqs + 1:
         raise ValueError("compact_tokens: pool [planes, pages, heads, page_tokens, channels], a table row and an end per sequence")
-    pool_ptr, table_ptr, first_ptr, picked_ptr, cu_ptr = _pointers("compact_tokens", pool, block_table, first, picked, cu_picked)
     planes, pages, heads, page_tokens, channels = pool.shape
+    if n_seqs > 65535 or planes * heads * channels * pool.element_size() > 2 ** 31 - 1:
+        raise ValueError("compact_tokens: sequences are at most 65535, a token's rows in all planes and heads at most 2^31 bytes")
+    pool_ptr, table_ptr, first_ptr, picked_ptr, cu_ptr = _pointers("compact_tokens", pool, block_table, first, picked, cu_picked)
     if pool.numel() == 0 or picked.numel() == 0 or block_table.shape[1] == 0:
         return pool
     fn = _FUNCTIONS.get("lb_compact_tokens") or _fn("cache_moves", "lb_compact_tokens",

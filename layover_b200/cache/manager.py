@@ -103,6 +103,8 @@ class SequenceCache:
     tables: list[BlockTable]
     num_tokens: int = 0
     closed: bool = False
+    # the parents of the drafts that the last step computed behind the held tokens (none: empty); None: no step has run yet
+    drafts: list[int] | None = None
 
 
 class CacheManager:
@@ -382,7 +384,7 @@ class CacheManager:
             raise OutOfBlocks(f"forking needs {len(forks)} request slots, {self._slots.num_free} free")
         made, copies = [], [[] for _ in self.paged]
         for (seq, request_id), at in zip(forks, open_page):
-            child = SequenceCache(request_id, self._slots.alloc(1)[0], [], seq.num_tokens)
+            child = SequenceCache(request_id, self._slots.alloc(1)[0], [], seq.num_tokens, drafts=None if seq.drafts is None else [])
             for g, group in enumerate(self.paged):
                 source = seq.tables[g]
                 blocks = source.blocks[: self.blocks_for(seq.num_tokens)]
@@ -410,8 +412,8 @@ class CacheManager:
         return made
 
     def accept(self, accepted: list[tuple[SequenceCache, list[int]]]) -> None:
-        """After a step over drafted tokens: each request keeps the drafts listed (rising places among its drafts, a path down their
-        tree). Their rows move to the places right behind what the request holds, in all layers; they are counted, and the pages
+        """After a step over drafted tokens: each request keeps the drafts listed (rising places among its drafts, a path down the tree
+        that its last step brought). Their rows move to the places right behind what the request holds, in all layers; they are counted, and the pages
         behind them given back."""
         from .. import ops
 
@@ -424,6 +426,9 @@ class CacheManager:
             room = min((len(t.blocks) for t in seq.tables), default=0) * self.block_tokens - seq.num_tokens
             if any(b <= a for a, b in zip([-1, *path], path)) or (path and path[-1] >= room):
                 raise ValueError(f"request {seq.request_id!r}: accepted drafts rise and lie in its pages, got {path} with room for {room}")
+            if seq.drafts is not None and any(node >= len(seq.drafts) or seq.drafts[node] != before for before, node in zip([-1, *path], path)):
+                raise ValueError(f"request {seq.request_id!r}: accepted drafts are a path down those of its last step, whose parents are "
+                                 f"{seq.drafts}, got {path}")
         if self.device is not None and any(place != node for _, path in accepted for place, node in enumerate(path)):
             cu = [0]
             for _, path in accepted:
@@ -439,6 +444,8 @@ class CacheManager:
                     ops.compact_tokens(pool, table.view(len(accepted), width), first, picked, ends)
         for seq, path in accepted:
             self.commit(seq, seq.num_tokens + len(path))
+            if seq.drafts is not None:
+                seq.drafts = []
             keep = self.blocks_for(seq.num_tokens)
             for group, table in zip(self.paged, seq.tables):
                 for block in table.blocks[keep:]:

@@ -165,6 +165,8 @@ class StepFunction:
         if drafts and sampled:
             raise ValueError("drafted tokens are checked against their logits, not sampled")
         self._reserve(entries)
+        for entry in entries:
+            entry.seq.drafts = []           # what an earlier step left behind the held tokens is written over
         with profiling.nvtx_range("step"):
             graph = None if drafts else self._graph_for(entries, sampled)
             if graph is not None:
@@ -191,8 +193,10 @@ class StepFunction:
                 if sampled:
                     out = self.sampler.launch(out, batch)
         for entry in entries:
-            if entry.parents is None:       # drafts are counted when they are accepted
+            if entry.parents is None:
                 self.cache.commit(entry.seq, entry.seq.num_tokens + len(entry.tokens))
+            else:                           # drafts are counted when they are accepted
+                entry.seq.drafts = list(entry.parents)
         self.steps += 1
         return out
 

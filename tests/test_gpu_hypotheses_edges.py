@@ -204,3 +204,31 @@ def test_beam_selection_of_more_than_65535_rows():
     values, places = values[:, :keep], places[:, :keep]
     assert apart.sum() > 16_000 and torch.equal(got[apart], places[apart])
     assert ((outs[0].cpu().double() - values).abs() <= 2.0 ** -24 * values.abs() + 2.0 ** -18).all()
+
+
+def test_only_a_path_down_the_last_steps_drafts_is_accepted(tiny_folders):
+    """Rows that no step wrote, or that are not a branch, do not become part of a request; neither do drafts of a step before the last."""
+    import layover_b200 as lb
+    from conftest import random_prompt
+    model = lb.load_model(str(tiny_folders["a"][0]), device="cuda", dtype="fp32")
+    cache, step = fresh(model)
+    seq, _ = feed(cache, step, "x", random_prompt(256, 9, 1))
+    with pytest.raises(ValueError, match="last step"):
+        cache.accept([(seq, [0])])                         # a step without drafts
+    step([lb.StepEntry(seq, [1, 2, 3, 4], [0], [-1, 0, 0, 2])])
+    (child,) = cache.fork([(seq, "child")])
+    for path in ([0, 5], [1], [0, 1, 2], [0, 3], [2, 3]):
+        with pytest.raises(ValueError, match="last step"):
+            cache.accept([(seq, path)])
+    with pytest.raises(ValueError, match="last step"):
+        cache.accept([(child, [0])])                       # a fork holds what is held, and no drafts
+    cache.accept([(seq, [0, 2, 3])])
+    assert seq.num_tokens == 12
+    with pytest.raises(ValueError, match="last step"):
+        cache.accept([(seq, [0])])
+    step([lb.StepEntry(seq, [1, 2], [0], [-1, 0])])
+    step([lb.StepEntry(seq, [5], [0])])
+    with pytest.raises(ValueError, match="last step"):
+        cache.accept([(seq, [0])])
+    cache.accept([(seq, []), (child, [])])
+    cache.check()

@@ -27,3 +27,29 @@ def test_beam_selection_names_its_largest_sizes(requests, beams, vocab):
 def test_moves_name_their_largest_sizes(call, message):
     with pytest.raises(ValueError, match=message):
         call(lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device="meta"))
+
+
+# ------------------------------------------------------------------------------- books
+def manager(blocks=20, page=4, max_requests=8):
+    from layover_b200.cache import CacheManager
+    from layover_b200.parts.base import PagedKVNeed, StateNeed
+
+    needs = [PagedKVNeed(2, 16, None), PagedKVNeed(2, 16, 6), StateNeed((3,), torch.float32)]
+    return CacheManager([(i, n, None) for i, n in enumerate(needs)], blocks, page, torch.float32, None, max_requests)
+
+
+@pytest.mark.parametrize("path", [[0, 3], [1], [0, 1, 2], [2], [0, 4]])
+def test_accepted_drafts_are_a_branch_of_what_the_last_step_brought(path):
+    m = manager()
+    a = m.open("a")
+    m.grow(a, 13)
+    a.drafts = [-1, 0, 0, 1]                             # as a step leaves them
+    with pytest.raises(ValueError, match="last step"):
+        m.accept([(a, path)])
+    assert a.num_tokens == 0 and a.drafts == [-1, 0, 0, 1]
+    m.accept([(a, [0, 1, 3])])
+    assert a.num_tokens == 3 and a.drafts == []
+    with pytest.raises(ValueError, match="last step"):
+        m.accept([(a, [0])])
+    m.accept([(a, [])])
+    m.check()

@@ -366,8 +366,6 @@ class CacheManager:
         """A new request for each (live request, new request id), holding the same tokens: all of them, or (OutOfBlocks) none. Pages
         that hold nothing but those tokens are shared; the page that is still being written, the state slot and the record are
         copied, in one launch a pool whatever the number of forks. Pages behind the held tokens are not taken over."""
-        from .. import ops
-
         self._need_kernels()
         ids = [request_id for _, request_id in forks]
         if len(set(ids)) != len(ids) or any(i in self.live for i in ids):
@@ -400,16 +398,28 @@ class CacheManager:
             self.live[request_id] = child
             made.append(child)
         if self.device is not None and forks:
-            for group, pairs in zip(self.paged, copies):
-                if pairs:
-                    src, dst = torch.tensor(pairs, dtype=torch.int32).T.contiguous().to(self.device)
-                    for pool in self._paged_pools(group):
-                        ops.copy_pages(pool, src, dst)
-            src, dst = torch.tensor([[seq.slot, child.slot] for (seq, _), child in zip(forks, made)], dtype=torch.int32).T.contiguous().to(self.device)
-            for group in self.states:
-                ops.copy_pages(group.pool, src, dst)
-            ops.copy_pages(self.records.unsqueeze(0), src, dst)
+            try:
+                self._copy_for(forks, made, copies)
+            except Exception:
+                for child in made:
+                    self.close(child)
+                raise
         return made
+
+    def _copy_for(self, forks: list[tuple[SequenceCache, str]], made: list[SequenceCache], copies: list[list[tuple[int, int]]]) -> None:
+        """What forked requests own: pages (per group: from, to), state slots and records."""
+        from .. import ops
+
+        pair = lambda rows: torch.tensor(rows, dtype=torch.int32).T.contiguous().to(self.device)
+        for group, pairs in zip(self.paged, copies):
+            if pairs:
+                src, dst = pair(pairs)
+                for pool in self._paged_pools(group):
+                    ops.copy_pages(pool, src, dst)
+        src, dst = pair([[seq.slot, child.slot] for (seq, _), child in zip(forks, made)])
+        for group in self.states:
+            ops.copy_pages(group.pool, src, dst)
+        ops.copy_pages(self.records.unsqueeze(0), src, dst)
 
     def accept(self, accepted: list[tuple[SequenceCache, list[int]]]) -> None:
         """After a step over drafted tokens: each request keeps the drafts listed (rising places among its drafts, a path down the tree

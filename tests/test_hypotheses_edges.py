@@ -53,3 +53,22 @@ def test_accepted_drafts_are_a_branch_of_what_the_last_step_brought(path):
         m.accept([(a, [0])])
     m.accept([(a, [])])
     m.check()
+
+
+def test_a_fork_whose_copies_fail_leaves_the_books_as_they_were(monkeypatch):
+    m = manager()
+    a = m.open("a")
+    m.grow(a, 10); m.commit(a, 10)
+    m.device = torch.device("cpu")                        # rows would be moved, and that raises: no CPU path
+    m.paged[0].pool = torch.zeros(1, 2, 21, 2, 4, 16)
+    monkeypatch.setattr(m, "_need_kernels", lambda: None)
+    free, slots, tables = m.num_free, m.num_free_slots, [list(t.blocks) for t in a.tables]
+    with pytest.raises(ops.KernelError, match="no CPU path"):
+        m.fork([(a, "b"), (a, "c")])
+    m.check()
+    assert (set(m.live), m.num_free, m.num_free_slots, [t.blocks for t in a.tables]) == ({"a"}, free, slots, tables)
+    assert all(m.paged[0].allocator.holders(b) == 1 for b in a.tables[0].blocks)
+    m.device = None
+    (b,) = m.fork([(a, "b")])                             # and the ids are free
+    m.close(a); m.close(b)
+    m.check()

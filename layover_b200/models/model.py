@@ -105,12 +105,14 @@ class Model:
     @property
     def takes_drafts(self) -> bool:
         """Whether a step may bring drafted tokens that form a tree: every mixer attends, without further options, and behind the window
-        of the pages that it reads."""
+        of the pages that it reads, and no block keeps a state beside it (a token shift)."""
         from ..parts.attention import Attention
+        from ..parts.base import PagedKVNeed
 
         mixers = [getattr(block, "mixer", None) for block in self.blocks]
         schedule = self.spec.schedule
-        return all(isinstance(m, Attention) and not m.general for m in mixers) and all(
+        return all(isinstance(m, Attention) and not m.general and isinstance(b.cache_need(), (PagedKVNeed, type(None)))
+                   for m, b in zip(mixers, self.blocks)) and all(
             e.reads_cache_of is None or mixers[e.layer].window == mixers[schedule[e.reads_cache_of].layer].window for e in schedule)
 
     def tile_sizes(self) -> tuple[int, ...]:

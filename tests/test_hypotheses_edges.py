@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from layover_b200 import ops
+from layover_b200.parts import PartSpec
 
 I32 = torch.int32
 
@@ -72,3 +73,30 @@ def test_a_fork_whose_copies_fail_leaves_the_books_as_they_were(monkeypatch):
     (b,) = m.fork([(a, "b")])                             # and the ids are free
     m.close(a); m.close(b)
     m.check()
+
+
+# ------------------------------------------------------------------------------- which models take drafts, and with what
+def one_block(block):
+    """A model of one block, without weights."""
+    from types import SimpleNamespace
+
+    from layover_b200.models.model import Model
+    from layover_b200.parts import build_part
+
+    model = Model.__new__(Model)
+    model.blocks, model.final_norm = [build_part("block", block, "")], build_part("norm", NORM, "")
+    model.spec = SimpleNamespace(schedule=[SimpleNamespace(layer=0, reads_cache_of=None)])
+    return model
+
+
+NORM = PartSpec("rmsnorm", {"dim": 16, "eps": 1e-5, "weight": "n"})
+ATTENTION = dict(hidden=16, q_heads=2, kv_heads=1, head_dim=16, q="q", k="k", v="v", o="o")
+STREAMS = dict(streams=2, hidden=16, connections=[{k: f"h{q}.{k}" for k in ("in", "out", "mix")} for q in (1, 2)], input_norm=NORM,
+               mixer=PartSpec("attention", ATTENTION))
+
+
+def test_a_block_that_keeps_a_state_beside_its_attention_takes_no_drafts():
+    """A token shift mixes what stands next to one another, which drafts of a tree do not."""
+    assert one_block(PartSpec("hyper_connected", STREAMS)).takes_drafts
+    assert not one_block(PartSpec("hyper_connected", dict(STREAMS, shift="shift"))).takes_drafts
+    assert not one_block(PartSpec("hyper_connected", dict(STREAMS, mixer=PartSpec("attention", dict(ATTENTION, sink="s"))))).takes_drafts

@@ -76,7 +76,7 @@ def generate_with_drafts(model, prompts: list[list[int]], max_new_tokens: int = 
         num_blocks = sum(-(-(len(p) + max_new_tokens + spare) // block_tokens) for p in prompts)
     cache = PagedKVCache(model, max(1, num_blocks), block_tokens=block_tokens, max_requests=max(1, len(prompts)))
     step = StepFunction(model, cache)
-    status, names = ops.status_words(model.device, (*model.kernel_libraries(model.dtype), "attention_tree"))
+    status, names = ops.status_words(model.device, model.kernel_libraries(model.dtype))
     counts = {"steps": 0, "drafted": 0, "accepted": 0}
 
     def choose(logits: torch.Tensor) -> list[int]:

@@ -199,9 +199,11 @@ class Attention(Part):
     def kernel_libraries(self, dtype):
         if self._on_tensor_cores(dtype):
             return ("elementwise", "attention_mma") + (("attention_tcgen05",) if self._on_tcgen05() else ())
-        if dtype == torch.float32 or self.general:
+        if self.general:
             return ("elementwise", "attention_simt")
-        names = ["elementwise", "attention_mma"]
+        if dtype == torch.float32:
+            return ("elementwise", "attention_simt", "attention_tree")
+        names = ["elementwise", "attention_mma", "attention_tree"]
         if ops.attention_tcgen05_takes_heads(self.q_heads, self.kv_heads, self.dim):
             names.append("attention_tcgen05")
         return tuple(names)

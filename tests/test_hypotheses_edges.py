@@ -100,3 +100,14 @@ def test_a_block_that_keeps_a_state_beside_its_attention_takes_no_drafts():
     assert one_block(PartSpec("hyper_connected", STREAMS)).takes_drafts
     assert not one_block(PartSpec("hyper_connected", dict(STREAMS, shift="shift"))).takes_drafts
     assert not one_block(PartSpec("hyper_connected", dict(STREAMS, mixer=PartSpec("attention", dict(ATTENTION, sink="s"))))).takes_drafts
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_model_that_takes_drafts_lists_their_kernels(dtype):
+    """Where a bounded wait of theirs runs out, the sampled step behind it says so: the error words read are those of the libraries listed."""
+    from layover_b200.models.runtime import Runtime
+
+    model = one_block(PartSpec("hyper_connected", STREAMS))
+    assert model.takes_drafts and "attention_tree" in model.kernel_libraries(dtype, Runtime(dtype, torch.device("cpu"), None))
+    sinks = one_block(PartSpec("hyper_connected", dict(STREAMS, mixer=PartSpec("attention", dict(ATTENTION, sink="s")))))
+    assert "attention_tree" not in sinks.kernel_libraries(dtype, Runtime(dtype, torch.device("cpu"), None))

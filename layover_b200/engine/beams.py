@@ -51,7 +51,7 @@ def beam_search(model, prompts: list[list[int]], beams: int = 4, max_new_tokens:
     logits = torch.zeros((count * beams, model.spec.vocab_size), device=device)
     found_before = None
     parents, tokens = (torch.empty((count, beams), dtype=torch.int32, device=device) for _ in range(2))
-    for _ in range(max_new_tokens):
+    for left in range(max_new_tokens - 1, -1, -1):
         places = [(r, b) for r in range(count) for b in range(beams) if rows[r][b] is not None]
         if not places:
             break
@@ -93,13 +93,16 @@ def beam_search(model, prompts: list[list[int]], beams: int = 4, max_new_tokens:
                     made += 1
             next_rows.append(row)
             next_texts.append(text)
+        texts = next_texts
+        if not left:                                         # nobody goes on: the texts are all that is wanted
+            break
         for r in range(count):                               # beams that nobody continues give their pages back first
             for seq in rows[r]:
                 if seq is not None and id(seq) not in keeps:
                     cache.close(seq)
         for (_, _, r, k), child in zip(forks, cache.fork([(seq, name) for seq, name, _, _ in forks])):
             next_rows[r][k] = child
-        rows, texts, ended = next_rows, next_texts, next_ended
+        rows, ended = next_rows, next_ended
     values = scores.tolist()
     for row in rows:
         for seq in row:

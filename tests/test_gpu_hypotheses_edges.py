@@ -232,3 +232,12 @@ def test_only_a_path_down_the_last_steps_drafts_is_accepted(tiny_folders):
         cache.accept([(seq, [0])])
     cache.accept([(seq, []), (child, [])])
     cache.check()
+
+
+def test_a_search_forks_nothing_after_its_last_step(tiny_folders):
+    """A pool with room for every step, but for no fork behind the last, has all beams."""
+    import layover_b200 as lb
+    model = lb.load_model(str(tiny_folders["a"][0]), device="cuda", dtype="fp32")
+    roomy = lb.beam_search(model, [[7]], 4, 1, block_tokens=4)
+    tight = lb.beam_search(model, [[7]], 4, 1, block_tokens=4, num_blocks=1)
+    assert tight == roomy and len(tight[0]) == 4

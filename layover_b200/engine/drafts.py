@@ -63,7 +63,8 @@ def walk(tokens: list[int], parents: list[int], chosen: list[int]) -> list[int]:
 def generate_with_drafts(model, prompts: list[list[int]], max_new_tokens: int = 16, drafts=LookupDrafts(), stop_tokens=frozenset(),
                          num_blocks: int | None = None, block_tokens: int = 16, prefill_chunk: int = 512) -> tuple[list[list[int]], dict]:
     """Greedy continuations of `prompts`, the tokens that `generate` gives at temperature 0 up to the roundings of the kernels that
-    compute them, and the counts {"steps", "drafted", "accepted"}. `drafts(tokens, room)` guesses, see `LookupDrafts`."""
+    compute them, and the counts {"steps", "drafted", "accepted"}. `drafts(tokens, room)` guesses, see `LookupDrafts`; without `num_blocks`
+    the pool has room for twice its `width` x `depth` guesses a request (of a callable without those 8 x 8), and of more the first are taken."""
     from .. import PagedKVCache
     from .step import StepFunction
 
@@ -71,7 +72,8 @@ def generate_with_drafts(model, prompts: list[list[int]], max_new_tokens: int = 
         raise ValueError("a prompt needs tokens, and max_new_tokens is at least 1")
     if not model.takes_drafts:
         raise ValueError("this model's mixers have no form for a tree of drafts")
-    spare = 2 * getattr(drafts, "width", 8) * getattr(drafts, "depth", 8) + 2
+    spare = 2 * max(0, getattr(drafts, "width", 8)) * max(0, getattr(drafts, "depth", 8)) + 2
+    most_guesses = spare if num_blocks is None else model.spec.max_position
     if num_blocks is None:
         num_blocks = sum(-(-(len(p) + max_new_tokens + spare) // block_tokens) for p in prompts)
     cache = PagedKVCache(model, max(1, num_blocks), block_tokens=block_tokens, max_requests=max(1, len(prompts)))
@@ -110,7 +112,8 @@ def generate_with_drafts(model, prompts: list[list[int]], max_new_tokens: int = 
         for i in active:
             room = min(open_ends(i) - 1, step.max_position - seqs[i].num_tokens - 1)
             guesses, parents = drafts(texts[i], room)
-            guesses, parents = guesses[: step.max_position - seqs[i].num_tokens - 1], parents[: step.max_position - seqs[i].num_tokens - 1]
+            most = max(0, min(most_guesses, step.max_position - seqs[i].num_tokens - 1))      # parents come first: the first guesses are a tree
+            guesses, parents = guesses[:most], parents[:most]
             counts["drafted"] += len(guesses)
             tokens = [texts[i][-1], *guesses]
             entries.append(StepEntry(seqs[i], tokens, list(range(len(tokens))), [-1, *(p + 1 for p in parents)]))

@@ -241,3 +241,14 @@ def test_a_search_forks_nothing_after_its_last_step(tiny_folders):
     roomy = lb.beam_search(model, [[7]], 4, 1, block_tokens=4)
     tight = lb.beam_search(model, [[7]], 4, 1, block_tokens=4, num_blocks=1)
     assert tight == roomy and len(tight[0]) == 4
+
+
+def test_more_guesses_than_there_is_room_for(tiny_folders):
+    """A callable may guess as much as it likes: what the default pool has no pages for is not checked, and the text is that of fewer guesses."""
+    import layover_b200 as lb
+    model = lb.load_model(str(tiny_folders["a"][0]), device="cuda", dtype="fp32")
+    prompts = [[5, 6, 7], [9]]
+    want, _ = lb.generate_with_drafts(model, prompts, 12, lambda tokens, room: ([], []), block_tokens=4)
+    every = lambda tokens, room: (list(range(256)), [-1] * 256) if room else ([], [])
+    got, counts = lb.generate_with_drafts(model, prompts, 12, every, block_tokens=4)
+    assert got == want and counts["drafted"] > 0

@@ -31,7 +31,7 @@ class LookupDrafts:
         """(guesses, the place of each one's parent among them or -1), at most `room` of them on any branch."""
         depth, n = min(self.depth, room), self.context
         guesses, parents, children = [], [], {}
-        if depth < 1 or len(tokens) <= n:
+        if depth < 1 or self.width < 1 or len(tokens) <= n:
             return guesses, parents
         key, found = tokens[-n:], 0
         for at in range(len(tokens) - n - 1, -1, -1):

@@ -111,3 +111,11 @@ def test_a_model_that_takes_drafts_lists_their_kernels(dtype):
     assert model.takes_drafts and "attention_tree" in model.kernel_libraries(dtype, Runtime(dtype, torch.device("cpu"), None))
     sinks = one_block(PartSpec("hyper_connected", dict(STREAMS, mixer=PartSpec("attention", dict(ATTENTION, sink="s")))))
     assert "attention_tree" not in sinks.kernel_libraries(dtype, Runtime(dtype, torch.device("cpu"), None))
+
+
+def test_lookup_drafts_without_width_or_depth_guess_nothing():
+    import layover_b200 as lb
+
+    text = [1, 2, 3, 1, 2, 4, 1, 2]
+    assert lb.LookupDrafts(width=0, depth=3)(text, 5) == ([], []) and lb.LookupDrafts(width=2, depth=0)(text, 5) == ([], [])
+    assert lb.LookupDrafts(width=1, depth=3)(text, 5) == ([4, 1, 2], [-1, 0, 1])

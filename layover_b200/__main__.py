@@ -8,7 +8,8 @@ Option names and meanings follow the reference's server where it has them
 --max-batch, --prefill-chunk (also the per-step prompt budget, as server.py:461), --cuda-graphs.
 --ignore-eos is the request option of that name (server.py:183,195). --max-batched-tokens is this
 engine's own: one budget for a whole step, decoded tokens first; so are --beams N (the N most likely continuations of each prompt
-instead of one) and --drafts N (greedy, N guessed tokens a branch checked in every step). The HTTP server itself and the
+instead of one) and --drafts N (greedy, N guessed tokens a branch checked in every step), which take neither a temperature nor
+--pool-gib, --max-batch, --max-batched-tokens and --cuda-graphs (--num-blocks sizes their pool). The HTTP server itself and the
 agent options are not part of this engine. The result is one JSON object on standard output.
 """
 
@@ -28,10 +29,10 @@ def parse_args(argv=None):
     p.add_argument("--seed", type=int, default=0, help="seed of the random weights and of sampling")
     p.add_argument("--device", default="cuda", choices=["cuda"], help="there is no CPU path")
     p.add_argument("--dtype", default="bf16", choices=["bf16", "fp32"])
-    p.add_argument("--pool-gib", type=float, default=2.0, help="KV pool size")
+    p.add_argument("--pool-gib", type=float, default=None, help="KV pool size (default: 2)")
     p.add_argument("--num-blocks", type=int, default=None, help="KV pool size in pages (overrides --pool-gib)")
     p.add_argument("--block-tokens", type=int, default=16)
-    p.add_argument("--max-batch", type=int, default=32)
+    p.add_argument("--max-batch", type=int, default=None, help="most requests of a step (default: 32)")
     p.add_argument("--prefill-chunk", type=int, default=512)
     p.add_argument("--max-batched-tokens", type=int, default=None,
                    help="most tokens of a whole step, decoded tokens first (default: --prefill-chunk prompt tokens a "
@@ -45,7 +46,20 @@ def parse_args(argv=None):
     p.add_argument("--beams", type=int, default=0, help="follow this many beams of each prompt and print all of them")
     p.add_argument("--drafts", type=int, default=0, help="check guesses of up to this many tokens in every step (greedy)")
     p.add_argument("--write-model", default=None, help="write the --preset's random model to this folder and exit")
-    return p.parse_args(argv)
+    args = p.parse_args(argv)
+    if args.beams or args.drafts:          # steps of their own, in a pool of their own (--num-blocks)
+        from .ops import BEAM_MAX_KEEP
+
+        if (args.beams and args.drafts) or args.temperature:
+            p.error("--beams and --drafts exclude one another and a temperature")
+        if args.drafts < 0 or (args.beams and not 1 <= args.beams <= BEAM_MAX_KEEP):
+            p.error(f"--drafts is positive, --beams 1 to {BEAM_MAX_KEEP}")
+        for name in ("cuda_graphs", "max_batch", "pool_gib", "max_batched_tokens"):
+            if getattr(args, name) not in (None, False):
+                p.error(f"--{name.replace('_', '-')} does not go with --beams and --drafts")
+    args.pool_gib = 2.0 if args.pool_gib is None else args.pool_gib
+    args.max_batch = 32 if args.max_batch is None else args.max_batch
+    return args
 
 
 def main(argv=None) -> int:
@@ -79,8 +93,6 @@ def main(argv=None) -> int:
         raise SystemExit("no prompts: give --prompt-ids or --prompt-lens")
     stop = frozenset() if args.ignore_eos or getattr(model.cfg, "eos_token_id", None) is None else frozenset({model.cfg.eos_token_id})
     if args.beams or args.drafts:
-        if (args.beams and args.drafts) or args.temperature:
-            raise SystemExit("--beams and --drafts exclude one another and a temperature")
         began, options = time.perf_counter(), dict(stop_tokens=stop, num_blocks=args.num_blocks, block_tokens=args.block_tokens, prefill_chunk=args.prefill_chunk)
         if args.beams:
             found = lb.beam_search(model, prompts, args.beams, args.max_new_tokens, **options)

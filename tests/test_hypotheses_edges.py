@@ -119,3 +119,26 @@ def test_lookup_drafts_without_width_or_depth_guess_nothing():
     text = [1, 2, 3, 1, 2, 4, 1, 2]
     assert lb.LookupDrafts(width=0, depth=3)(text, 5) == ([], []) and lb.LookupDrafts(width=2, depth=0)(text, 5) == ([], [])
     assert lb.LookupDrafts(width=1, depth=3)(text, 5) == ([4, 1, 2], [-1, 0, 1])
+
+
+# ------------------------------------------------------------------------------- command line
+@pytest.mark.parametrize("options, message", [
+    (["--drafts", "-3"], "positive"), (["--beams", "-1"], "1 to 32"), (["--beams", "40"], "1 to 32"), (["--drafts", "4", "--beams", "2"], "exclude"),
+    (["--beams", "2", "--temperature", "0.5"], "exclude"), (["--beams", "2", "--cuda-graphs"], "--cuda-graphs"), (["--drafts", "2", "--max-batch", "8"], "--max-batch"),
+    (["--drafts", "2", "--pool-gib", "2.0"], "--pool-gib"), (["--beams", "2", "--max-batched-tokens", "64"], "--max-batched-tokens"),
+])
+def test_command_line_refuses_what_beams_and_drafts_do_not_take(options, message, capsys):
+    from layover_b200.__main__ import parse_args
+
+    with pytest.raises(SystemExit):
+        parse_args(["--preset", "tiny-b", "--random-weights", "--prompt-lens", "9", *options])
+    assert message in capsys.readouterr().err
+
+
+def test_command_line_keeps_its_defaults():
+    from layover_b200.__main__ import parse_args
+
+    args = parse_args(["--preset", "tiny-b"])
+    assert (args.pool_gib, args.max_batch, args.max_batched_tokens, args.cuda_graphs, args.beams, args.drafts) == (2.0, 32, None, False, 0, 0)
+    assert parse_args(["--preset", "tiny-b", "--max-batch", "4", "--pool-gib", "0.5"]).max_batch == 4
+    assert parse_args(["--preset", "tiny-b", "--beams", "32", "--num-blocks", "9"]).beams == 32

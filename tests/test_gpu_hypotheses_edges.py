@@ -252,3 +252,46 @@ def test_more_guesses_than_there_is_room_for(tiny_folders):
     every = lambda tokens, room: (list(range(256)), [-1] * 256) if room else ([], [])
     got, counts = lb.generate_with_drafts(model, prompts, 12, every, block_tokens=4)
     assert got == want and counts["drafted"] > 0
+
+
+def spelled_out(cache, step, prompt, beams, new):
+    """Beam search that feeds every beam's whole text anew."""
+    held = [(0.0, [])]
+    for _ in range(new):
+        rows = []
+        for score, tokens in held:
+            seq, logits = feed(cache, step, "t", prompt + tokens)
+            cache.close(seq)
+            rows += [(score + p, tokens + [t]) for t, p in enumerate(torch.log_softmax(logits.double(), 0).tolist())]
+        held = sorted(rows, key=lambda x: -x[0])[:beams]
+    return held
+
+
+def test_beam_search_of_a_model_whose_states_move_with_the_beams():
+    import layover_b200 as lb
+    model = lb.random_model(lb.preset("topidra-tiny"), seed=0, device="cuda", dtype="fp32")
+    vocab = model.spec.vocab_size
+    prompt = [int(t) for t in torch.randint(0, vocab, (21,), generator=torch.Generator().manual_seed(5))]
+    found = lb.beam_search(model, [prompt], 3, 6, block_tokens=8, prefill_chunk=8)[0]
+    cache, step = fresh(model, 400, 8)
+    held = spelled_out(cache, step, prompt, 3, 6)
+    assert [s for s, _ in found] == pytest.approx([s for s, _ in held], abs=2e-3)
+    for (score, tokens), (want, text) in zip(found, held):
+        assert tokens == text or min(abs(want - s) for s, t in held if t != text) < 1e-3
+
+
+@pytest.mark.parametrize("name", ["a", "c"])
+def test_beam_search_in_bfloat16_gives_the_sums_of_its_texts(tiny_folders, name):
+    """Every beam's score is the sum of its tokens' log probabilities, each within the logits' tolerance on both sides of the softmax."""
+    import layover_b200 as lb
+    from conftest import random_prompt, tolerance
+    model = lb.load_model(str(tiny_folders[name][0]), device="cuda", dtype="bf16")
+    prompt = random_prompt(model.spec.vocab_size, 19, 4)
+    found = lb.beam_search(model, [prompt], 4, 8, block_tokens=8)[0]
+    assert len(found) == 4 and len({tuple(t) for _, t in found}) == 4 and [s for s, _ in found] == sorted((s for s, _ in found), reverse=True)
+    cache, step = fresh(model)
+    for i, (score, tokens) in enumerate(found):
+        text = prompt + tokens
+        logits = step([lb.StepEntry(cache.open(f"{i}"), text, list(range(len(prompt) - 1, len(text) - 1)))])
+        sums = torch.log_softmax(logits.double(), 1).gather(1, torch.tensor(tokens, device="cuda")[:, None]).sum()
+        assert abs(score - float(sums)) <= len(tokens) * 2 * tolerance(logits, model.dtype)

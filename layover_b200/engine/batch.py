@@ -66,11 +66,13 @@ def tree_rows(parents: list[int]) -> tuple[list[int], list[int]]:
 
 def tree_rows_in_window(parents: list[int], seen: list[int], window: int) -> list[int]:
     """What each token of a tree sees of it behind a window: itself and the `window - 1` ancestors before it."""
-    lines, rows = [], []
-    for i, p in enumerate(parents):
-        lines.append((lines[p] if p >= 0 else []) + [i])
-        rows.append(seen[i] & ~seen[lines[i][-1 - window]] if len(lines[i]) > window else seen[i])
-    return rows
+    above, up, left = list(range(len(parents))), parents, window      # the ancestor `window` levels up (-1: none), by doubled steps
+    while left:
+        if left & 1:
+            above = [up[a] if a >= 0 else -1 for a in above]
+        up = [up[p] if p >= 0 else -1 for p in up]
+        left >>= 1
+    return [bits & ~seen[a] if a >= 0 else bits for bits, a in zip(seen, above)]
 
 
 @dataclass

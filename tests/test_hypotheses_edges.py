@@ -142,3 +142,32 @@ def test_command_line_keeps_its_defaults():
     assert (args.pool_gib, args.max_batch, args.max_batched_tokens, args.cuda_graphs, args.beams, args.drafts) == (2.0, 32, None, False, 0, 0)
     assert parse_args(["--preset", "tiny-b", "--max-batch", "4", "--pool-gib", "0.5"]).max_batch == 4
     assert parse_args(["--preset", "tiny-b", "--beams", "32", "--num-blocks", "9"]).beams == 32
+
+
+# ------------------------------------------------------------------------------- trees behind a window
+def test_windows_over_trees_and_over_long_portions():
+    """Itself and the nearest ancestors; a portion of thousands of tokens beside drafts takes no memory for every pair of them."""
+    import random
+    import tracemalloc
+
+    from layover_b200.engine.batch import tree_rows, tree_rows_in_window
+
+    rng = random.Random(5)
+    for n in (1, 2, 40, 130):
+        parents = [-1 if i == 0 or rng.random() < 0.1 else rng.randint(max(0, i - 4), i - 1) for i in range(n)]
+        for window in (1, 2, 5, 8, 1000):
+            want = []
+            for i in range(n):
+                bits, at = 0, i
+                for _ in range(window):
+                    if at >= 0:
+                        bits, at = bits | 1 << at, parents[at]
+                want.append(bits)
+            assert tree_rows_in_window(parents, tree_rows(parents)[0], window) == want
+    chain = list(range(-1, 8191))
+    seen, _ = tree_rows(chain)
+    tracemalloc.start()
+    rows = tree_rows_in_window(chain, seen, 4096)
+    peak = tracemalloc.get_traced_memory()[1]
+    tracemalloc.stop()
+    assert rows[8191] == ((1 << 4096) - 1) << 4096 and peak < 32 << 20

@@ -295,3 +295,58 @@ def test_beam_search_in_bfloat16_gives_the_sums_of_its_texts(tiny_folders, name)
         logits = step([lb.StepEntry(cache.open(f"{i}"), text, list(range(len(prompt) - 1, len(text) - 1)))])
         sums = torch.log_softmax(logits.double(), 1).gather(1, torch.tensor(tokens, device="cuda")[:, None]).sum()
         assert abs(score - float(sums)) <= len(tokens) * 2 * tolerance(logits, model.dtype)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("sinks, softcap, window", [(True, 0.0, 0), (False, 20.0, 0), (True, 20.0, 0), (False, 0.0, 300), (True, 20.0, 40)])
+@pytest.mark.parametrize("nodes, group", [(12, 4), (75, 4), (9, 1)])
+def test_drafts_that_are_not_finite_with_sinks_caps_and_windows(nodes, group, sinks, softcap, window, dim, dtype):
+    """Many small requests (whole row tiles in a block's share), long ones (parts of their keys), some of them with drafts that are not finite."""
+    lengths = [(7 * i % 90, 1 + i % nodes) for i in range(40)] + [(2600, nodes), (1300, nodes)]
+    case = Trees(lengths, 2 * group, 2, dim, dtype=dtype, sinks=sinks, softcap=softcap, window=window, seed=nodes + dim).fill()
+    if sinks:
+        case.sinks[0] = -INF
+    finite = case.run()
+    odd = {3: 0, 11: lengths[11][1] - 1, 30: lengths[30][1] // 2, 40: nodes // 2, 41: nodes - 1}
+    sees = torch.zeros(sum(n for _, n in lengths), dtype=torch.bool)
+    for i, place in odd.items():
+        case.v[i][lengths[i][0] + place, i % 2, 5 + i % 7] = (NAN, INF, -INF)[i % 3]
+        first = int(case.cu_q[i])
+        sees[first: first + lengths[i][1]] = case.seen[i][:, place]
+    got = case.fill().run()
+    assert ops().attention_tree_status() == 0
+    rows = len(sees)
+    assert torch.equal(got[:rows][~sees], finite[:rows][~sees]) and (got[rows:] == 7.0).all()
+    if sinks:                       # a sink of -inf beside rows that see something is no sink: heads of a finite one are compared
+        case.sinks[0] = -1e30
+        case.check(case.run())
+    else:
+        case.check(got)
+
+
+def test_a_captured_call_with_drafts_that_are_not_finite():
+    """Replayed on finite values, on others, and on finite ones again: the bits of calls that were not captured."""
+    o = ops()
+    case = Trees([(900, 6), (41, 20), (2000, 40)], 8, 2, 128, seed=11, extra_rows=0).fill()
+    d = {name: getattr(case, name).cuda() for name in ("q", "k_pool", "v_pool", "table", "cu_q", "ctx", "positions", "tree")}
+    out = torch.empty_like(d["q"])
+    call = lambda: o.attention_tree(d["q"], d["k_pool"], d["v_pool"], out, d["table"], d["cu_q"], d["ctx"], None, d["tree"], 3, 8, 2, 128, 16, case.scale, 40, 2040)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    finite = case.v_pool.clone()
+    case.v[2][2000 + 13, 1, 9], case.v[1][41, 0, 100] = NAN, INF
+    odd = case.fill().v_pool
+    for values in (finite, odd, finite):
+        d["v_pool"].copy_(values)
+        out.zero_()
+        graph.replay()
+        got = out.cpu()
+        call()
+        assert torch.equal(torch.nan_to_num(got, 99.0), torch.nan_to_num(out.cpu(), 99.0))
+        if values is odd:
+            case.check(got)
+    assert torch.isfinite(out).all()

@@ -23,6 +23,8 @@
 // 0 x NaN is NaN. So in tiles that hold drafts, or held keys that lie behind the window of some row, value rows that are not finite are
 // taken out of the product and added one by one to the rows that see them.
 //
+// The weights round to bfloat16 for the second product of the bfloat16 kernel (see attention_tree_tcgen05.cuh); all else is held in 32 bits.
+//
 // Bounds. bfloat16: the keys' and values' bytes and, with few keys, the time to start two launches and to reach a page through its
 // table; 5 requests of 13 drafts behind a window of 1,024, 12 heads over 2 of 64 channels 16.5 us. 32 bits: 2 x rows x keys x dim FFMA a
 // head, 11 us at the pipes' rate for 4 requests of 13 drafts after 900 keys, 32 heads over 8 of 128 (32 MB: 4.9 us), measured 63 us:

@@ -17,11 +17,15 @@
 // Code that runs first is slow: a turn of softmax takes four times as long until its instructions have been fetched. So the warps run
 // through parts of it each, on nothing, while the first loads are under way.
 //
-// The keys' and values' bytes bound it. Measured (one B200): 40 requests of 25 drafts after 400 .. 8,000 keys, 32 heads over 8, 155 us (734 MB,
-// 4.7 TB/s); 8 of 32 after 3,000 38 us (104 MB); 2 of 64 after 12,345, 16 over 4, 46 to 48 us (52 MB), 9 of them the join of 18
-// parts a row; 1 of 8 after 700 12.7 us. What is left is time in which nothing streams: about 4 us until a block's share is known and 4 more
-// until its first scores, 4 to 6 at the border of two segments (partial tiles, results to be stored, instructions that run for the first
-// time), and the join. The same by mma.sync, the rows' keys in chunks: 843, 202 and 167 us.
+// The keys' and values' bytes bound it. Measured (one B200): 40 requests of 25 drafts after 400 .. 8,000 keys, 32 heads over 8, 150 us where calls
+// follow one another in a graph over three sets of inputs (734 MB, 4.9 TB/s), 169 as single calls over many (4.3); 8 of 32 after 3,000 37 us (104 MB);
+// 2 of 64 after 12,345, 16 over 4, 44 to 50 us (52 MB), 9 of them the join of 18 parts a row; 1 of 8 after 700 12.1 us. What is left is time in
+// which nothing streams: about 4 us until a block's share is known and 4 more until its first scores, 4 to 6 at the border of two segments (partial
+// tiles, results to be stored, instructions that run for the first time), and the join. The same by mma.sync, the rows' keys in chunks: 843, 202 and
+// 167 us.
+//
+// The weights round to bfloat16 for the second product, as in the package's other kernels of the models that take drafts (the output is off by 0.0023
+// of its size against 64 bits, 0.0017 with weights of 32 bits); their sum, the maxima and the outputs are held in 32 bits.
 //
 // Rows that the tree does not have cost nothing but the tensor cores' time: their warps only hand tiles on. A draft's values may hold what
 // is not finite, and 0 x NaN is NaN also for rows that do not see the draft. A block whose outputs are not all finite therefore takes its share once

@@ -2,19 +2,19 @@
 // moved to the places right behind what their request holds. In all layers of a pool at once. The reference neither forks nor
 // drafts; its nearest relative moves blocks to and from the host (layover/kv/paged_cache.py).
 //
-// Both are bound by memory: every byte that moves is read once and written once. Measured (one B200): 56 pages of 72 planes, 216 MB in all, 38
-// us (5.7 TB/s of 6.5), 24 states of 2 MB in 3 layers 42 us (6.0), the accepted rows of 64 requests, 55 MB, 17.6 us (3.1: rows of 256
-// bytes in 72 x 8 places each), of one request 3.2 us.
+// Both are bound by memory: every byte that moves is read once and written once. Measured (one B200): 56 pages of 72 planes, 216 MB in all, 38.5
+// us (5.6 TB/s of 6.5), 24 states of 2 MB in 3 layers 42.3 us (5.9), the accepted rows of 64 requests, 55 MB, 18.5 us (3.0: rows of 256
+// bytes in 72 x 8 places each), of one request 3.6 us.
 //
 // Neither kernel lets its dependents start early, and each thread's last act is to make its writes visible to the whole device: decode
 // attention reads a cache's earlier keys ahead of its wait, which is sound only where no kernel that may still run writes them. So
-// whatever is launched behind a move, or behind others that are, starts when the rows have been moved.
+// whatever is launched behind a move, or behind others that are, starts when the rows have been moved. (0.4 to 0.9 us a launch.)
 #include "common.cuh"
 
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int MOST_BLOCKS = 512;    // of the compaction (64 sequences of 5 rows in 72 planes of 8 heads: 17.6 us; with 1,024 18.8, with 2,048 19.9)
+constexpr int MOST_BLOCKS = 512;    // of the compaction (64 sequences of 5 rows in 72 planes of 8 heads, us with 512, 1,024 and 2,048, without the fence at the end: 17.6, 18.8, 19.9)
 constexpr int COPY_UNROLL = 4;      // vectors of a thread that are on their way at once
 
 // pool [planes][pages][vecs of a page]: plane p's page dst[i] = its page src[i].

@@ -1288,7 +1288,7 @@ _TREE_SCRATCH_FLOATS = 64 << 20          # the most that the chunks' results may
 
 def attention_tree_on_tcgen05(group: int, dim: int, page_tokens: int, dtype: torch.dtype) -> bool:
     """Whether `attention_tree` takes these heads and pages to its tcgen05 kernel: whatever it takes, however few the rows (one B200, 32 heads
-    over 8, 4 drafts; tcgen05 and mma.sync, us: 1 request of 700 keys 12.6 and 15.2, 8 of 3,000 37 and 67)."""
+    over 8, 4 drafts; tcgen05 and mma.sync, us: 1 request of 700 keys 12.1 and 15.2, 8 of 3,000 37 and 67)."""
     return dtype == torch.bfloat16 and dim == 128 and page_tokens % 8 == 0 and 128 % page_tokens == 0 and group <= 128
 
 
@@ -1338,7 +1338,8 @@ def attention_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     p - j < window; among drafts `tree` alone decides. `sinks` float32 [q_heads] join the softmax's denominator only; `softcap` > 0: a
     scaled score s becomes softcap * tanh(s / softcap). No sequence has more than `max_nodes` drafts or more than `max_ctx` keys
     (what is above is not computed: rows, or not planned for: keys). Rows behind cu_q[n_seqs] stay as they are. Head sizes: multiples of
-    16 (float32: of 4) up to 256. What is in a draft's keys and values reaches only the rows that see it, infinities and NaN too."""
+    16 (float32: of 4) up to 256. What is in a draft's keys and values reaches only the rows that see it, infinities and NaN too (of a held
+    token behind a window as well); the others' bits do not depend on it. In bfloat16 a capped score is off by up to about softcap / 2^21."""
     dtype, tokens = q.dtype, q.shape[0]
     _need(q, None, "q"); _need(out, dtype, "out"); _need(k_pool, dtype, "k_pool"); _need(v_pool, dtype, "v_pool")
     _need(block_table, torch.int32, "block_table"); _need(cu_q, torch.int32, "cu_q"); _need(ctx_len, torch.int32, "ctx_len"); _need(tree, torch.int32, "tree")
@@ -1469,8 +1470,9 @@ _BEAM_PIECE = 3584      # values of a row that a block of the first kernel looks
 def _beam_pieces(rows: int, vocab: int, sms: int) -> int:
     """Pieces of a row that one block takes: few where blocks are few, more where several blocks wait for an SM's place (the first costs a
     block most) and where the second kernel has many chunks to join. Measured (one B200, us; 2, 3, 5, 6 and 9 pieces): 128 rows of 151,936
-    42.7, 35.5, 30.8, 29.9 and 29.4 (6 are taken), 64 rows 18.0, 16.7, 14.3, 15.1 and 16.8 (5), 16 rows 10.8, 10.7, 9.7, 10.2 and 10.8 (5), 32
-    rows of 32,768 with 32 kept 25.1, 20.6, 19.6, 20.8 and 24.4 (5), 4 rows of 151,936 with 2, 3, 4 and 5 8.2, 8.0, 8.2 and 8.7 (3)."""
+    40.2, 35.9, 27.5, 27.3 and 29.9, with 11, all blocks at once, 27.5 (6 are taken), 64 rows 18.7, 16.8, 14.0, 14.9 and 16.8 (5), 16 rows 10.3,
+    10.3, 9.1, 10.3 and 10.5 (5), 32 rows of 32,768 with 32 kept 31.7, 26.0, 22.8, 23.9 and 27.5 (5), 4 rows of 151,936 with 2, 3, 4 and 5 8.2,
+    8.1, 8.0 and 8.6 (3)."""
     pieces = rows * -(-vocab // _BEAM_PIECE)
     return 3 if pieces <= 2 * sms else 5 if pieces <= 20 * sms else 6
 

@@ -900,7 +900,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, ROWS2 ? 2 : 4) join_kernel(const
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) {
         const float w = exp2f(ml[j].x - base);
-        if (w == 0.f) continue;
+        if (w == 0.f && ml[j].y == ml[j].y) continue;      // a part without a score that is a number has no maximum, and a sum of NaN
         total += w * ml[j].y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) { sum[i].x += w * v[j][i].x; sum[i].y += w * v[j][i].y; sum[i].z += w * v[j][i].z; sum[i].w += w * v[j][i].w; }

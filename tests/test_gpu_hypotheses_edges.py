@@ -350,3 +350,19 @@ def test_a_captured_call_with_drafts_that_are_not_finite():
         if values is odd:
             case.check(got)
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("held, nodes", [(256, 3), (128, 40), (1280, 3), (2560, 70)])
+def test_a_draft_whose_key_is_nan_alone_in_its_part_of_the_keys(held, nodes, dim, dtype):
+    """Drafts that see themselves alone begin a key tile, whose scores are one part: where its only one is NaN the row is NaN, and no other."""
+    case = Trees([(held, nodes), (40, 2)], 4, 2, dim, dtype=dtype, seen=[torch.eye(nodes, dtype=torch.bool), torch.eye(2, dtype=torch.bool)], seed=held).fill()
+    finite = case.run()
+    case.check(finite)
+    for place in (1, nodes - 1):
+        case.k[0][held + place] = NAN
+    got = case.fill().run()
+    odd = torch.zeros(nodes + 2, dtype=torch.bool)
+    odd[[1, nodes - 1]] = True
+    assert torch.isnan(got[:nodes + 2][odd]).all() and torch.equal(got[:nodes + 2][~odd], finite[:nodes + 2][~odd])
